@@ -46,6 +46,15 @@ class Int8Artifact(C.Structure):
     ]
 
 
+class Matrix(C.Structure):
+    """aeisu_matrix of include/aeisu.h."""
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("type", C.c_int), ("rows", C.c_int),
+                ("cols", C.c_int), ("batch", C.c_int), ("ld", C.c_int64), ("batch_stride", C.c_int64),
+                ("block_rows", C.c_int), ("transposed", C.c_int)]
+
+
+_MATRIX = C.POINTER(Matrix)
+
 _SIGNATURES = {
     "aeisu_open_int8": (C.c_int, [C.POINTER(Int8Artifact), C.c_int, C.POINTER(C.c_void_p)]),
     "aeisu_open_spyr8": (C.c_int, [C.c_char_p, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
@@ -84,6 +93,16 @@ _SIGNATURES = {
     "aeisu_reconstruct_backward_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                                  C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "aeisu_block_quantize": (C.c_int, [_MATRIX, C.c_int, _MATRIX, _MATRIX, C.c_int, C.c_void_p]),
+    "aeisu_column_sum_workspace": (C.c_uint64, [C.c_int, C.c_int]),
+    "aeisu_column_sum": (C.c_int, [_MATRIX, C.c_void_p, C.c_int, C.c_void_p, C.c_uint64, C.c_int, C.c_void_p]),
+    "aeisu_product_workspace": (C.c_uint64, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "aeisu_product": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_void_p, C.c_uint64, C.c_int,
+                                C.c_void_p]),
+    "aeisu_grouped_product": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_int, C.c_void_p]),
+    "aeisu_grouped_weight_gradient": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int,
+                                                C.c_void_p]),
+    "aeisu_product_status": (C.c_int, [C.c_int, C.POINTER(C.c_int)]),
     "aeisu_synchronize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_double]),
     "aeisu_tensor_peak": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]),
     "aeisu_timings_get": (C.c_int, [C.c_void_p, C.POINTER(Timings)]),

@@ -1,0 +1,27 @@
+// Host helpers shared by the block-scaled quantiser and the matrix products.
+#pragma once
+
+#include "blockscale.h"
+#include "common.h"
+
+namespace aeisu {
+
+// Makes `dev` current for the scope.
+struct OnDevice {
+    int prev = -1;
+    explicit OnDevice(int dev) {
+        AEISU_CUDA(cudaGetDevice(&prev));
+        if (prev != dev) AEISU_CUDA(cudaSetDevice(dev));
+        else prev = -1;
+    }
+    ~OnDevice() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
+inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+inline bool is_code(int t) { return t == kE4M3 || t == kE5M2; }
+
+}  // namespace aeisu

@@ -6,8 +6,10 @@
 #include <iterator>
 #include <memory>
 #include <string>
+#include <utility>
 #include <vector>
 
+#include "blockscale.h"
 #include "common.h"
 #include "engine.h"
 #include "kernels.h"
@@ -57,6 +59,30 @@ aeisu::Engine& engine_of(aeisu_t* h) {
 void check_io(int n, int h, int w, unsigned flags) {
     aeisu::require(n >= 1 && h >= 1 && w >= 1, "Expected CHW RGB image");
     aeisu::require(flags == AEISU_IO_HOST || flags == AEISU_IO_DEVICE, "unknown I/O flags");
+}
+
+aeisu::MatrixRef matrix(const aeisu_matrix* m) {
+    aeisu::require(m != nullptr, "matrix pointer is null");
+    return {m->data, m->type, m->rows, m->cols, (long long)m->ld, m->batch, (long long)m->batch_stride, m->transposed != 0};
+}
+aeisu::ScaleRef scales_of(const aeisu_matrix* m) {
+    aeisu::require(m->block_rows == 1 || m->block_rows == 128, "blocks have 1 or 128 rows");
+    const int blocks = (m->cols + 127) / 128, per = m->block_rows == 1 ? m->rows : (m->rows + 127) / 128;
+    return {m->scales, m->block_rows == 1 ? 0 : 7, per, (long long)blocks * per};
+}
+struct Scales {   // the scales of an FP8 operand, none for a 16-bit one
+    aeisu::ScaleRef ref{};
+    const aeisu::ScaleRef* ptr = nullptr;
+    explicit Scales(const aeisu_matrix* m) {
+        if (m && m->scales) {
+            ref = scales_of(m);
+            ptr = &ref;
+        }
+    }
+};
+aeisu::ProductOut product_out(const aeisu_matrix* out, const void* bias, int bias_type) {
+    aeisu::require(out != nullptr, "output pointer is null");
+    return {const_cast<void*>(out->data), out->type, (long long)out->ld, bias, bias_type};
 }
 
 }  // namespace
@@ -266,6 +292,87 @@ int aeisu_reconstruct_backward_f32(const float* source, const float* metadata, c
         aeisu::reconstruct_backward_f32(source, metadata, basis, grad_out, n, h, w, trim, gradient_stride, phase,
                                         device, grad_metadata, grad_base, grad_basis,
                                         static_cast<cudaStream_t>(stream));
+    });
+}
+
+int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, aeisu_matrix* codes, aeisu_matrix* t_codes,
+                         int device, void* stream) {
+    return guarded([&] {
+        aeisu::require(codes != nullptr, "codes pointer is null");
+        const aeisu::MatrixRef m = matrix(x);
+        aeisu::require(codes->rows == m.rows && codes->cols == m.cols && codes->batch == m.batch,
+                       "codes must have the sizes of the values");
+        aeisu::require(!t_codes || (t_codes->rows == m.cols && t_codes->cols == m.rows && t_codes->batch == m.batch &&
+                                    t_codes->type == codes->type),
+                       "codes of the transpose must have the transposed sizes");
+        aeisu::block_quantize(m, block_rows, codes->type, const_cast<void*>(codes->data), codes->ld,
+                              codes->batch_stride, const_cast<uint8_t*>(codes->scales),
+                              t_codes ? const_cast<void*>(t_codes->data) : nullptr, t_codes ? t_codes->ld : 0,
+                              t_codes ? t_codes->batch_stride : 0,
+                              t_codes ? const_cast<uint8_t*>(t_codes->scales) : nullptr, device,
+                              static_cast<cudaStream_t>(stream));
+    });
+}
+
+uint64_t aeisu_column_sum_workspace(int rows, int cols) {
+    return rows >= 1 && cols >= 1 ? aeisu::column_sum_partials(rows, cols) * sizeof(float) : 0;
+}
+
+int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* workspace, uint64_t workspace_bytes,
+                     int device, void* stream) {
+    return guarded([&] {
+        const aeisu::MatrixRef m = matrix(x);
+        aeisu::require(workspace_bytes >= aeisu_column_sum_workspace(m.rows, m.cols), "workspace is too small");
+        aeisu::column_sum(m, out, out_type, static_cast<float*>(workspace), device, static_cast<cudaStream_t>(stream));
+    });
+}
+
+uint64_t aeisu_product_workspace(int m, int n, int k, int fp8, int device) {
+    uint64_t r = 0;
+    guarded([&] {
+        aeisu::require(m >= 1 && n >= 1 && k >= 1, "matrix sizes are out of range");
+        r = aeisu::product_workspace(m, n, k, fp8 != 0, device);
+    });
+    return r;
+}
+
+int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias, int bias_type, aeisu_matrix* out,
+                  void* workspace, uint64_t workspace_bytes, int device, void* stream) {
+    return guarded([&] {
+        const aeisu::MatrixRef ma = matrix(a), mb = matrix(b);
+        const Scales sa(a), sb(b);
+        aeisu::product(ma, sa.ptr, mb, sb.ptr, product_out(out, bias, bias_type), workspace, size_t(workspace_bytes),
+                       device, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int aeisu_grouped_product(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
+                          aeisu_matrix* out, int device, void* stream) {
+    return guarded([&] {
+        const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
+        const Scales sx(x), sw(weight);
+        aeisu::grouped_product(mx, sx.ptr, mw, sw.ptr, offsets, product_out(out, nullptr, 0), zero_outside != 0, device,
+                               static_cast<cudaStream_t>(stream));
+    });
+}
+
+int aeisu_grouped_weight_gradient(const aeisu_matrix* grad, const aeisu_matrix* x, const int* offsets, int groups,
+                                  void* out, int out_type, int device, void* stream) {
+    return guarded([&] {
+        aeisu::MatrixRef g = matrix(grad), m = matrix(x);
+        // rows of either are contracted: the operands are the transposes, stored as they are
+        for (aeisu::MatrixRef* r : {&g, &m}) {
+            std::swap(r->rows, r->cols);
+            r->trans = !r->trans;
+        }
+        aeisu::grouped_weight_gradient(g, m, offsets, groups, out, out_type, device, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int aeisu_product_status(int device, int* code) {
+    return guarded([&] {
+        aeisu::require(code != nullptr, "code pointer is null");
+        *code = aeisu::product_status(device);
     });
 }
 

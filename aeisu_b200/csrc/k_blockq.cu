@@ -1,0 +1,397 @@
+// Block-scaled FP8 quantisation: codes E4M3 or E5M2, one power-of-two scale (E8M0) for each block
+// of 128 values of a row (block_rows 1) or of 128 x 128 values (block_rows 128).
+//
+// With amax the largest finite magnitude of a block and top the largest finite code (448 or
+// 57344), the scale is the smallest power of two s with amax / s <= top (1 for a block of zeros),
+// and a code is x / s rounded to nearest even.  Division by a power of two is exact, so the one
+// rounding of a code is the rounding to 8 bits, and the result is defined bit for bit.  Infinities
+// and NaN become NaN codes and take no part in amax: they spoil what they would spoil in the
+// product, and nothing else.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "blockscale_host.h"
+
+namespace aeisu {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T> struct Vec;   // sixteen bytes of T
+template <> struct Vec<float> { static constexpr int n = 4; };
+template <> struct Vec<__half> { static constexpr int n = 8; };
+template <> struct Vec<__nv_bfloat16> { static constexpr int n = 8; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Infinity and NaN to NaN, which fmaxf ignores and the conversion keeps.
+__device__ __forceinline__ float finite_or_nan(float v) {
+    return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : v;
+}
+
+// Eight consecutive values of a row as floats; columns at or past `cols` read as zero.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int c, int cols, float* v) {
+    if constexpr (VEC) {
+        constexpr int n = Vec<T>::n;
+#pragma unroll
+        for (int h = 0; h < 8 / n; ++h) {
+            uint4 q = make_uint4(0, 0, 0, 0);
+            if (c + h * n < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + h * n));
+            const T* p = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (int i = 0; i < n; ++i) v[h * n + i] = finite_or_nan(to_f32(p[i]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? finite_or_nan(to_f32(row[c + i])) : 0.f;
+    }
+}
+
+// Biased exponent of the scale.  amax = m 2^e with 0.5 <= m < 1 has the exponent field e + 126; the
+// largest code is 0.875 * 2^top, so s = 2^(e - top), doubled where m > 0.875.
+template <bool E5M2>
+__device__ __forceinline__ uint32_t scale_of(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    const int e = int(b >> 23) + 1 - (E5M2 ? 16 : 9) + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return b == 0 ? 127u : uint32_t(max(e, 0));
+}
+__device__ __forceinline__ float inverse_scale(uint32_t s) { return __uint_as_float((254u - s) << 23); }
+
+template <bool E5M2>
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    if constexpr (E5M2) {
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %2, %1;" : "=h"(lo) : "f"(a), "f"(b));
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
+    } else {
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(lo) : "f"(a), "f"(b));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
+    }
+    return uint32_t(lo) | (uint32_t(hi) << 16);
+}
+
+template <typename T>
+struct QuantJob {
+    const T* x;
+    int rows, cols;
+    long long ld, batch_stride;
+    uint8_t* codes;
+    long long codes_ld, codes_batch;
+    uint8_t* scales;           // [batch][col blocks][row blocks]
+    uint8_t* t_codes;          // codes of the transpose [batch][cols][rows], or null
+    long long t_ld, t_batch;
+    uint8_t* t_scales;         // [batch][row blocks of 128][col blocks or cols]
+    int tiles;
+};
+
+// One scale per row and block column, no transpose.  Eight lanes share a block (two loads of eight
+// values each), a warp takes four neighbouring blocks of four rows, a CTA 32 rows of them; the
+// scales leave through shared memory as 32 contiguous bytes per block column.
+template <typename T, bool E5M2, bool VEC>
+__global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
+    __shared__ uint8_t sh[4][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int col_groups = (j.cols + 4 * kBlock - 1) / (4 * kBlock);
+    const int r0 = int(blockIdx.x / col_groups) * 32, c0 = int(blockIdx.x % col_groups) * 4 * kBlock;
+    const T* x = j.x + blockIdx.y * j.batch_stride;
+    uint8_t* codes = j.codes + blockIdx.y * j.codes_batch;
+    const int c = c0 + (lane >> 3) * kBlock + (lane & 7) * 16;
+    float v[4][16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + warp * 4 + i;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[i][k] = 0.f;
+        if (r < j.rows) {
+            load8<T, VEC>(x + r * j.ld, c, j.cols, v[i]);
+            load8<T, VEC>(x + r * j.ld, c + 8, j.cols, v[i] + 8);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + warp * 4 + i;
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(v[i][k]));
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, d));
+        const uint32_t s = scale_of<E5M2>(amax);
+        const float inv = inverse_scale(s);
+        if ((lane & 7) == 0) sh[lane >> 3][warp * 4 + i] = uint8_t(s);
+        if (r < j.rows && c < j.cols) {
+            uint4 q;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = codes4<E5M2>(v[i][4 * k] * inv, v[i][4 * k + 1] * inv, v[i][4 * k + 2] * inv,
+                                    v[i][4 * k + 3] * inv);
+            *reinterpret_cast<uint4*>(codes + r * j.codes_ld + c) = q;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const int b = threadIdx.x >> 5, r = r0 + lane, col_blocks = (j.cols + kBlock - 1) / kBlock;
+        if (r < j.rows && c0 / kBlock + b < col_blocks)
+            j.scales[(size_t(blockIdx.y) * col_blocks + c0 / kBlock + b) * j.rows + r] = sh[b][lane];
+    }
+}
+
+// A 128 x 128 tile per CTA: codes with one scale per row or per tile and, with BOTH, the codes of the
+// transpose too, from one read of x.  A lane holds four consecutive rows of two runs of eight
+// columns: row maxima over eight lanes, column maxima over a lane's rows, four lanes and eight warps.
+// The transposed codes (four rows to a word) turn in shared memory; the 16-byte chunk of a column is
+// exclusive-or'ed with the column's octet, so that a warp's 32 words fall in 32 banks.
+template <typename T, bool E5M2, bool VEC, bool TILE_SCALE, bool BOTH>
+__global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
+    __shared__ float col_max[8][kBlock];
+    __shared__ uint8_t row_s[kBlock];
+    __shared__ float tile_max[8];
+    __shared__ __align__(16) uint32_t turn[BOTH ? kBlock * 32 : 4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, oct = lane & 7, sub = lane >> 3;
+    const int col_blocks = (j.cols + kBlock - 1) / kBlock, row_blocks = (j.rows + kBlock - 1) / kBlock;
+    const int rb = int(blockIdx.x / col_blocks), cb = int(blockIdx.x % col_blocks);
+    const int r0 = rb * kBlock, c0 = cb * kBlock, rw = warp * 16 + sub * 4;
+    const T* x = j.x + blockIdx.y * j.batch_stride;
+    float v[4][16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + rw + i;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[i][k] = 0.f;
+        if (r < j.rows) {
+            load8<T, VEC>(x + r * j.ld, c0 + oct * 8, j.cols, v[i]);
+            load8<T, VEC>(x + r * j.ld, c0 + 64 + oct * 8, j.cols, v[i] + 8);
+        }
+    }
+    float amax[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        amax[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) amax[i] = fmaxf(amax[i], fabsf(v[i][k]));
+    }
+    if constexpr (TILE_SCALE) {
+        float m = fmaxf(fmaxf(amax[0], amax[1]), fmaxf(amax[2], amax[3]));
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+        if (lane == 0) tile_max[warp] = m;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(~0u, amax[i], d));
+            if (oct == 0) row_s[rw + i] = uint8_t(scale_of<E5M2>(amax[i]));
+        }
+        if constexpr (BOTH) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                float m = fmaxf(fmaxf(fabsf(v[0][k]), fabsf(v[1][k])), fmaxf(fabsf(v[2][k]), fabsf(v[3][k])));
+                m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+                m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+                if (sub == 0) col_max[warp][(k >> 3) * 64 + oct * 8 + (k & 7)] = m;
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t tile_s = 0;
+    if constexpr (TILE_SCALE) {
+        float m = tile_max[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) m = fmaxf(m, tile_max[w]);
+        tile_s = scale_of<E5M2>(m);
+        if (threadIdx.x == 0) {
+            j.scales[(size_t(blockIdx.y) * col_blocks + cb) * row_blocks + rb] = uint8_t(tile_s);
+            if (BOTH) j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * col_blocks + cb] = uint8_t(tile_s);
+        }
+    } else if (threadIdx.x < kBlock && r0 + threadIdx.x < j.rows) {
+        j.scales[(size_t(blockIdx.y) * col_blocks + cb) * j.rows + r0 + threadIdx.x] = row_s[threadIdx.x];
+    }
+    uint8_t* codes = j.codes + blockIdx.y * j.codes_batch;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + rw + i;
+        const float inv = inverse_scale(TILE_SCALE ? tile_s : scale_of<E5M2>(amax[i]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = c0 + h * 64 + oct * 8;
+            const float* p = v[i] + 8 * h;
+            const uint2 q = make_uint2(codes4<E5M2>(p[0] * inv, p[1] * inv, p[2] * inv, p[3] * inv),
+                                       codes4<E5M2>(p[4] * inv, p[5] * inv, p[6] * inv, p[7] * inv));
+            if (r < j.rows && c < j.cols) *reinterpret_cast<uint2*>(codes + r * j.codes_ld + c) = q;
+        }
+    }
+    if constexpr (BOTH) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int c = (k >> 3) * 64 + oct * 8 + (k & 7);
+            uint32_t s = tile_s;
+            if constexpr (!TILE_SCALE) {
+                float m = col_max[0][c];
+#pragma unroll
+                for (int w = 1; w < 8; ++w) m = fmaxf(m, col_max[w][c]);
+                s = scale_of<E5M2>(m);
+                if (warp == 0 && sub == 0 && c0 + c < j.cols)
+                    j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * j.cols + c0 + c] = uint8_t(s);
+            }
+            const float inv = inverse_scale(s);
+            turn[c * 32 + ((rw >> 2) ^ (((c >> 3) & 7) << 2))] =
+                codes4<E5M2>(v[0][k] * inv, v[1][k] * inv, v[2][k] * inv, v[3][k] * inv);
+        }
+        __syncthreads();
+        uint8_t* t_codes = j.t_codes + blockIdx.y * j.t_batch;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = i * kThreads + threadIdx.x, c = at >> 3, chunk = at & 7;
+            const uint4 q = *reinterpret_cast<const uint4*>(turn + c * 32 + ((chunk ^ ((c >> 3) & 7)) << 2));
+            if (c0 + c < j.cols && r0 + chunk * 16 < j.rows)
+                *reinterpret_cast<uint4*>(t_codes + (c0 + c) * j.t_ld + r0 + chunk * 16) = q;
+        }
+    }
+}
+
+// Column sums: each CTA adds a run of rows of 64 columns (lanes: column pairs, warps: every eighth
+// row), then the runs are added in order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_column_runs(const T* x, int rows, int cols, long long ld, int run,
+                                                          float* partial) {
+    __shared__ float sh[8][64];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = int(blockIdx.x) * 64 + lane;
+    const int r1 = min(rows, int(blockIdx.y + 1) * run);
+    float a = 0.f, b = 0.f;
+#pragma unroll 4
+    for (int r = int(blockIdx.y) * run + warp; r < r1; r += 8) {
+        if (c < cols) a += to_f32(x[r * ld + c]);
+        if (c + 32 < cols) b += to_f32(x[r * ld + c + 32]);
+    }
+    sh[warp][lane] = a;
+    sh[warp][lane + 32] = b;
+    __syncthreads();
+    if (threadIdx.x < 64 && int(blockIdx.x) * 64 + int(threadIdx.x) < cols) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x];
+        partial[size_t(blockIdx.y) * cols + blockIdx.x * 64 + threadIdx.x] = s;
+    }
+}
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(1024) k_column_join(const float* partial, int runs, int cols, T* out) {
+    __shared__ float sh[32][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = int(blockIdx.x) * 32 + lane;
+    float a = 0.f;
+    if (c < cols)
+        for (int r = warp; r < runs; r += 32) a += partial[size_t(r) * cols + c];
+    sh[warp][lane] = a;
+    __syncthreads();
+    if (warp == 0 && c < cols) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) s += sh[w][lane];
+        out[c] = from_f32<T>(s);
+    }
+}
+
+// Rows of one run: runs of at least 64 rows, at most 592 (four CTAs on each of 148 SMs) of them.
+int column_run(int rows) { return std::max(64, (rows + 591) / 592); }
+
+template <typename T, bool E5M2, bool VEC>
+void launch_quant(const QuantJob<T>& j, int block_rows, int batch, cudaStream_t stream) {
+    const long long rows32 = (j.rows + 31) / 32, rows128 = (j.rows + 127) / 128;
+    const long long grid = block_rows == 1 && !j.t_codes ? rows32 * ((j.cols + 511) / 512)
+                                                         : rows128 * ((j.cols + 127) / 128);
+    require(grid < (1LL << 31), "matrix is too large");
+    const dim3 g(unsigned(grid), unsigned(batch), 1);
+    if (block_rows == 1) {
+        if (!j.t_codes) k_quant_rows<T, E5M2, VEC><<<g, kThreads, 0, stream>>>(j);
+        else k_quant_tile<T, E5M2, VEC, false, true><<<g, kThreads, 0, stream>>>(j);
+    } else {
+        if (!j.t_codes) k_quant_tile<T, E5M2, VEC, true, false><<<g, kThreads, 0, stream>>>(j);
+        else k_quant_tile<T, E5M2, VEC, true, true><<<g, kThreads, 0, stream>>>(j);
+    }
+    AEISU_CUDA(cudaGetLastError());
+}
+
+template <typename T>
+void quantize_as(const MatrixRef& x, int block_rows, int code_type, void* codes, long long ld, long long batch_stride,
+                 uint8_t* scales, void* t_codes, long long t_ld, long long t_batch, uint8_t* t_scales,
+                 cudaStream_t stream) {
+    QuantJob<T> j{static_cast<const T*>(x.ptr), x.rows, x.cols, x.ld, x.batch_stride, static_cast<uint8_t*>(codes), ld,
+                  batch_stride, scales, static_cast<uint8_t*>(t_codes), t_ld, t_batch, t_scales, 0};
+    constexpr int n = Vec<T>::n;
+    const bool vec = aligned(x.ptr, 16) && x.ld % n == 0 && x.cols % n == 0 && (x.batch == 1 || x.batch_stride % n == 0);
+    if (code_type == kE5M2) {
+        if (vec) launch_quant<T, true, true>(j, block_rows, x.batch, stream);
+        else launch_quant<T, true, false>(j, block_rows, x.batch, stream);
+    } else {
+        if (vec) launch_quant<T, false, true>(j, block_rows, x.batch, stream);
+        else launch_quant<T, false, false>(j, block_rows, x.batch, stream);
+    }
+}
+
+}  // namespace
+
+void block_quantize(const MatrixRef& x, int block_rows, int code_type, void* codes, long long ld,
+                    long long batch_stride, uint8_t* scales, void* t_codes, long long t_ld, long long t_batch_stride,
+                    uint8_t* t_scales, int device, cudaStream_t stream) {
+    require(x.ptr && codes && scales && (!t_codes || t_scales), "tensor pointer is null");
+    require(x.rows >= 1 && x.cols >= 1 && x.batch >= 1 && x.batch <= 65535 && x.ld >= x.cols && !x.trans,
+            "matrix sizes are out of range");
+    require(block_rows == 1 || block_rows == kBlock, "blocks have 1 or 128 rows");
+    require(is_code(code_type), "codes are E4M3 or E5M2");
+    require(ld >= x.cols && ld % 16 == 0 && batch_stride % 16 == 0 && aligned(codes, 16),
+            "code rows must start on 16-byte boundaries");
+    require(!t_codes || (t_ld >= x.rows && t_ld % 16 == 0 && t_batch_stride % 16 == 0 && aligned(t_codes, 16)),
+            "code rows of the transpose must start on 16-byte boundaries");
+    OnDevice on(device);
+    auto go = [&](auto t) {
+        quantize_as<decltype(t)>(x, block_rows, code_type, codes, ld, batch_stride, scales, t_codes, t_ld,
+                                 t_batch_stride, t_scales, stream);
+    };
+    if (x.type == kF32) go(float{});
+    else if (x.type == kF16) go(__half{});
+    else if (x.type == kBF16) go(__nv_bfloat16{});
+    else fail(AEISU_ERR_INVALID_ARG, "values must be float32, float16 or bfloat16");
+}
+
+size_t column_sum_partials(int rows, int cols) {
+    const int run = column_run(rows);
+    return size_t((rows + run - 1) / run) * cols;
+}
+
+void column_sum(const MatrixRef& x, void* out, int out_type, float* partial, int device, cudaStream_t stream) {
+    require(x.ptr && out && partial, "tensor pointer is null");
+    require(x.rows >= 1 && x.cols >= 1 && x.ld >= x.cols && x.batch == 1 && !x.trans, "matrix sizes are out of range");
+    OnDevice on(device);
+    const int run = column_run(x.rows), runs = (x.rows + run - 1) / run;
+    const dim3 grid(unsigned((x.cols + 63) / 64), unsigned(runs), 1);
+    auto in = [&](auto t) {
+        using T = decltype(t);
+        k_column_runs<T><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(x.ptr), x.rows, x.cols, x.ld, run, partial);
+    };
+    auto join = [&](auto t) {
+        using T = decltype(t);
+        k_column_join<T><<<unsigned((x.cols + 31) / 32), 1024, 0, stream>>>(partial, runs, x.cols, static_cast<T*>(out));
+    };
+    if (x.type == kF32) in(float{});
+    else if (x.type == kF16) in(__half{});
+    else if (x.type == kBF16) in(__nv_bfloat16{});
+    else fail(AEISU_ERR_INVALID_ARG, "values must be float32, float16 or bfloat16");
+    AEISU_CUDA(cudaGetLastError());
+    if (out_type == kF32) join(float{});
+    else if (out_type == kF16) join(__half{});
+    else if (out_type == kBF16) join(__nv_bfloat16{});
+    else fail(AEISU_ERR_INVALID_ARG, "sums must be float32, float16 or bfloat16");
+    AEISU_CUDA(cudaGetLastError());
+}
+
+}  // namespace aeisu

@@ -1,0 +1,133 @@
+"""Matrix products grouped by expert: rows sorted by expert, ragged group sizes, one launch.
+
+The grouped layers of the controller give each channel group its own weights; here each *row* (a pixel
+of a tile, a token) belongs to one of E experts.  ``offsets`` [E + 1] bounds the groups: rows
+``offsets[e] : offsets[e + 1]`` of x are multiplied by ``weight[e]``.  The bounds stay on the GPU: the
+call never waits for them, so it may be captured into a CUDA graph and replayed with other bounds.
+
+    y = grouped_matmul(x, weight, offsets)             # x [T, K], weight [E, N, K]: y [T, N]
+
+Float weights (float16 or bfloat16, the type of x) train: gradients of x and weight are products of
+the same kind, an expert without rows gets zeros.  BlockFP8 weights (``quantize(weight, rows=128)``)
+serve: x is quantised in the call, or given as BlockFP8.  Sums are held in float32 and rounded once.
+Rows in no group are zero, or, with ``out``, left as they were there.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from . import _matrices as mx
+from .block_fp8 import BlockFP8, quantize
+
+MAX_GROUPS = 1024
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _weights(weight):
+    """(tensor kept, aeisu_matrix) of weights [E, N, K] stored with either of the last two contiguous."""
+    flip = weight.transpose(1, 2)
+    if mx.row_stride(weight) is None and mx.row_stride(flip) is not None:
+        t, ld = mx.operand(flip)
+        return t, mx.matrix(t, ld, transposed=True)
+    t, ld = mx.operand(weight)
+    return t, mx.matrix(t, ld)
+
+
+def _product(x, weight, offsets, out, zero_outside):
+    """x, weight: (tensors kept, aeisu_matrix)."""
+    mo = mx.matrix(out, mx.row_stride(out))
+    _lib.check(_lib.lib().aeisu_grouped_product(C.byref(x[1]), C.byref(weight[1]), offsets.data_ptr(),
+                                                int(zero_outside), C.byref(mo), out.device.index, mx.stream(out.device)))
+    return out
+
+
+def _rows(x):
+    t, ld = mx.operand(x)
+    return t, mx.matrix(t, ld)
+
+
+class _Grouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets):
+        ctx.save_for_backward(x, weight, offsets)
+        out = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=x.device)
+        if x.shape[0] == 0:
+            return out
+        return _product(_rows(x), _weights(weight), offsets, out, True)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, offsets = ctx.saved_tensors
+        if x.shape[0] == 0:
+            return torch.empty_like(x), torch.zeros_like(weight), None
+        g = _rows(grad)
+        gx = gw = None
+        if ctx.needs_input_grad[0]:
+            gx = _product(g, _weights(weight.transpose(1, 2)), offsets, torch.empty_like(x, memory_format=torch.contiguous_format), True)
+        if ctx.needs_input_grad[1]:
+            gw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+            kept = _rows(x)
+            _lib.check(_lib.lib().aeisu_grouped_weight_gradient(
+                C.byref(g[1]), C.byref(kept[1]), offsets.data_ptr(), weight.shape[0], gw.data_ptr(),
+                mx.TYPES[gw.dtype], gw.device.index, mx.stream(gw.device)))
+        return gx, gw, None
+
+
+def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
+    """``x[t] @ weight[e].T`` for the group e of each row t; see the module's text.
+
+    ``x`` [T, K]; ``weight`` [E, N, K], E at most 1024, either of its last two dimensions contiguous;
+    ``offsets`` int32 [E + 1], not decreasing, within [0, T] (values outside are moved to the nearest
+    allowed one).  The result has x's type; ``dtype`` names it where x is BlockFP8 (default bfloat16).
+    ``out`` [T, N] takes the result instead of a new tensor; no gradients flow through it.
+    """
+    fp8 = isinstance(weight, BlockFP8)
+    coded = isinstance(x, BlockFP8)
+    if coded and not fp8:
+        raise TypeError("a BlockFP8 x needs BlockFP8 weights")
+    if len(x.shape) != 2 or len(weight.shape) != 3 or x.shape[1] != weight.shape[2] or 0 in weight.shape:
+        raise ValueError("Expected x [T, K] and weight [E, N, K]")
+    if weight.shape[0] > MAX_GROUPS:
+        raise ValueError(f"at most {MAX_GROUPS} experts; got {weight.shape[0]}")
+    if not fp8 and (weight.dtype not in _HALVES or x.dtype != weight.dtype):
+        raise TypeError(f"x and weight must both be float16 or bfloat16; got {x.dtype} and {weight.dtype}")
+    if fp8 and not coded and x.dtype not in mx.FLOATS:
+        raise TypeError(f"x must be float32, float16, bfloat16 or BlockFP8; got {x.dtype}")
+    if dtype is not None and not coded:
+        raise ValueError("dtype is for a BlockFP8 x: the result has x's type")
+    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (weight.shape[0] + 1,):
+        raise ValueError(f"Expected offsets int32 [{weight.shape[0] + 1}]")
+    dtype = (dtype or torch.bfloat16) if coded else x.dtype
+    if dtype not in mx.FLOATS:
+        raise TypeError(f"the result is float32, float16 or bfloat16; got {dtype}")
+    t, n = x.shape[0], weight.shape[1]
+    if out is not None and (tuple(out.shape) != (t, n) or out.dtype != dtype or (t and mx.row_stride(out) is None)):
+        raise ValueError(f"Expected out [{t}, {n}] of {dtype} with contiguous rows")
+    mx.need_cuda("grouped_matmul", x.codes if coded else x, weight.codes if fp8 else weight, offsets,
+                 *(() if out is None else (out,)))
+    wants = torch.is_grad_enabled() and any(not isinstance(v, BlockFP8) and v.requires_grad for v in (x, weight))
+    if wants and (fp8 or out is not None):
+        raise ValueError("FP8 weights and out serve without gradients")
+    offsets = offsets.contiguous()
+    if t == 0 and not wants:
+        return torch.empty((0, n), dtype=dtype, device=offsets.device) if out is None else out
+    if wants:
+        with torch.autocast(device_type="cuda", enabled=False):
+            return _Grouped.apply(x, weight, offsets)
+    if fp8:
+        q = x if coded else quantize(x)
+        mx_, mw = q.matrix(), weight.matrix()
+    else:
+        mx_, mw = _rows(x.detach()), _weights(weight.detach())
+    new = out is None
+    if new:
+        out = torch.empty((t, n), dtype=dtype, device=offsets.device)
+    return _product(mx_, mw, offsets, out, new)
+
+
+__all__ = ["grouped_matmul", "MAX_GROUPS"]

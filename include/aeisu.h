@@ -312,6 +312,64 @@ int aeisu_reconstruct_backward_f32(const float* source, const float* metadata, c
                                    int phase, int device, float* grad_metadata, float* grad_base,
                                    float* grad_basis, void* stream);
 
+/* Block-scaled FP8 and matrix products, with no counterpart in the reference (k_blockq.cu,
+ * k_prod.cu): operators for training and serving layers beside the controller's own.  All
+ * pointers are device pointers of GPU `device`; every call only enqueues on `stream` and may be
+ * captured into a CUDA graph.  Workspaces belong to the caller and are free again once the
+ * call's work on the stream is done. */
+enum { AEISU_TYPE_F32 = 0, AEISU_TYPE_F16 = 1, AEISU_TYPE_BF16 = 2, AEISU_TYPE_E4M3 = 3, AEISU_TYPE_E5M2 = 4 };
+
+/* `batch` matrices of rows x cols: element (r, c) at r * ld + c, or at c * ld + r when
+ * `transposed`; batch_stride elements from one matrix to the next.
+ * FP8 types come with `scales`, one E8M0 byte s for each block of block_rows (1 or 128) rows and
+ * 128 columns, which stands for code * 2^(s - 127) (255: NaN): [batch][blocks along a row][blocks
+ * along a column], contiguous.  Operands of a product start each row (each column when
+ * transposed) on a 16-byte boundary. */
+typedef struct aeisu_matrix {
+    const void* data;
+    const uint8_t* scales;
+    int type, rows, cols, batch;
+    int64_t ld, batch_stride;
+    int block_rows, transposed;
+} aeisu_matrix;
+
+/* codes = x quantised in blocks of block_rows x 128 and, where t_codes is given, t_codes = the
+ * transpose of x quantised in blocks of block_rows x 128 of its own, both from one read of x
+ * (float32, float16 or bfloat16, not transposed).  The scale of a block is the smallest power of
+ * two s with amax / s no larger than the largest finite code (1 for a block of zeros; at least
+ * 2^-127), amax over the block's finite values; a code is x / s rounded to nearest even, NaN where x
+ * is not finite.  Writes codes->data, codes->scales; up to 15 bytes after each row of codes, within
+ * ld, are overwritten. */
+int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, aeisu_matrix* codes, aeisu_matrix* t_codes,
+                         int device, void* stream);
+
+/* out[c] = sum over the rows of x[r][c], added in float32 in a fixed order. */
+uint64_t aeisu_column_sum_workspace(int rows, int cols);
+int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* workspace, uint64_t workspace_bytes,
+                     int device, void* stream);
+
+/* out[m][n] = sum_k a[m][k] b[n][k] + bias[n] (bias may be NULL): two FP8 operands with their
+ * scales, or two of one 16-bit type; float32 accumulation, one rounding to out's type (float32,
+ * float16 or bfloat16).  The order of the sum depends on the sizes alone. */
+uint64_t aeisu_product_workspace(int m, int n, int k, int fp8, int device);
+int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias, int bias_type, aeisu_matrix* out,
+                  void* workspace, uint64_t workspace_bytes, int device, void* stream);
+
+/* Rows grouped by expert: out[t][n] = sum_k x[t][k] weight[e][n][k] for t in [offsets[e],
+ * offsets[e + 1]); weight->batch groups (at most 1024), offsets int32 [groups + 1] in device
+ * memory.  Rows in no group are set to zero when zero_outside is nonzero, otherwise left as they
+ * were.  Offsets outside [0, x->rows] or below the one before are moved to the nearest allowed
+ * value.  Types as for aeisu_product. */
+int aeisu_grouped_product(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
+                          aeisu_matrix* out, int device, void* stream);
+/* out[e][n][k] = sum over t in group e of grad[t][n] x[t][k]; zeros for an empty group.  grad and x
+ * float16 or bfloat16, not transposed; out contiguous. */
+int aeisu_grouped_weight_gradient(const aeisu_matrix* grad, const aeisu_matrix* x, const int* offsets, int groups,
+                                  void* out, int out_type, int device, void* stream);
+/* Waits for the device; *code receives 0, or 1 if a product kernel gave up a bounded wait since the
+ * last call (its outputs are then undefined). */
+int aeisu_product_status(int device, int* code);
+
 /* Measurement helper with no counterpart in the reference: the dense tensor-core throughput of
  * GPU `device` for the instructions the controller kernels issue, as the roofline denominator
  * of their stages.  kind 0: tcgen05.mma kind::f16 (f16 operands, K = 16); kind 1: kind::f8f6f4
