@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libaeisu_b200.so"
@@ -46,14 +47,10 @@ class Int8Artifact(C.Structure):
     ]
 
 
-class Matrix(C.Structure):
-    """aeisu_matrix of include/aeisu.h."""
-    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("type", C.c_int), ("rows", C.c_int),
-                ("cols", C.c_int), ("batch", C.c_int), ("ld", C.c_int64), ("batch_stride", C.c_int64),
-                ("block_rows", C.c_int), ("transposed", C.c_int)]
-
-
-_MATRIX = C.POINTER(Matrix)
+# aeisu_matrix of include/aeisu.h, packed by struct: data, scales, type, rows, cols, batch, ld, batch_stride,
+# block_rows, transposed
+MATRIX = struct.Struct("@PPiiiiqqii")
+_MATRIX = C.c_char_p
 
 _SIGNATURES = {
     "aeisu_open_int8": (C.c_int, [C.POINTER(Int8Artifact), C.c_int, C.POINTER(C.c_void_p)]),
@@ -99,6 +96,18 @@ _SIGNATURES = {
     "aeisu_product_workspace": (C.c_uint64, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "aeisu_product": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_void_p, C.c_uint64, C.c_int,
                                 C.c_void_p]),
+    "aeisu_linear_workspace": (C.c_uint64, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "aeisu_linear_kept_bytes": (C.c_uint64, [C.c_int, C.c_int, C.c_int]),
+    "aeisu_linear": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_void_p, C.c_uint64, C.c_int,
+                               C.c_void_p]),
+    "aeisu_linear_forward": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_uint64, C.c_int, C.c_void_p]),
+    "aeisu_linear_backward": (C.c_int, [_MATRIX, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                        C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_uint64, C.c_int,
+                                        C.c_void_p]),
+    "aeisu_grouped_linear_workspace": (C.c_uint64, [C.c_int, C.c_int]),
+    "aeisu_grouped_linear": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_void_p, C.c_uint64, C.c_int,
+                                       C.c_void_p]),
     "aeisu_grouped_product": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_int, C.c_void_p]),
     "aeisu_grouped_weight_gradient": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int,
                                                 C.c_void_p]),

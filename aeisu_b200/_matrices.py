@@ -1,7 +1,6 @@
-"""Tensors as the C ABI's ``aeisu_matrix``: layouts, alignment and the calls shared by the products."""
+"""Tensors as the C ABI's ``aeisu_matrix``: layouts, alignment, workspaces and streams."""
 from __future__ import annotations
 
-import ctypes as C
 import functools
 
 import torch
@@ -12,58 +11,68 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 CODES = (torch.float8_e4m3fn, torch.float8_e5m2)
 BLOCK = 128
+_pack = _lib.MATRIX.pack
 
 
 def blocks(n):
     return -(-n // BLOCK)
 
 
-def stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def stream(index):
+    """Handle of the current stream of CUDA device `index`."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def need_cuda(name, *tensors):
-    """All tensors on one CUDA device."""
-    for t in tensors:
-        if not t.is_cuda:
-            raise ValueError(f"{name} needs CUDA tensors (there is no CPU path)")
-        if t.device != tensors[0].device:
+    """All tensors on one CUDA device; its index."""
+    first = tensors[0].device
+    if first.type != "cuda":
+        raise ValueError(f"{name} needs CUDA tensors (there is no CPU path)")
+    for t in tensors[1:]:
+        if t.device != first:
+            if not t.is_cuda:
+                raise ValueError(f"{name} needs CUDA tensors (there is no CPU path)")
             raise ValueError(f"{name}: the tensors must be on one device")
+    return first.index
 
 
 def row_stride(t):
     """Elements from row to row of a tensor whose rows are contiguous and do not overlap, else None."""
-    r, c = t.shape[-2:]
-    if c > 1 and t.stride(-1) != 1:
+    shape, strides = t.shape, t.stride()
+    r, c = shape[-2], shape[-1]
+    if c > 1 and strides[-1] != 1:
         return None
-    ld = t.stride(-2) if r > 1 else c
-    if ld < c or (t.dim() == 3 and t.shape[0] > 1 and t.stride(0) < (r - 1) * ld + c):
+    ld = strides[-2] if r > 1 else c
+    if ld < c or (len(shape) == 3 and shape[0] > 1 and strides[0] < (r - 1) * ld + c):
         return None
     return ld
 
 
 def matrix(t, ld, scales=None, rows=0, transposed=False):
     """aeisu_matrix of a 2-D or 3-D tensor (of its last two dimensions' transpose when transposed)."""
-    batch = t.shape[0] if t.dim() == 3 else 1
-    r, c = t.shape[-2:]
+    shape = t.shape
+    batch, step = (shape[0], t.stride(0)) if len(shape) == 3 else (1, 0)
+    r, c = shape[-2], shape[-1]
     if transposed:
         r, c = c, r
-    return _lib.Matrix(t.data_ptr(), None if scales is None else scales.data_ptr(), TYPES[t.dtype], r, c, batch, ld,
-                       t.stride(0) if batch > 1 else 0, rows, int(transposed))
+    return _pack(t.data_ptr(), 0 if scales is None else scales.data_ptr(), TYPES[t.dtype], r, c, batch, ld, step, rows,
+                 transposed)
 
 
 def empty_rows(shape, dtype, device):
     """An uninitialised tensor whose rows start on 16-byte boundaries."""
-    per = 16 // torch.empty((), dtype=dtype).element_size()
+    per = 16 // dtype.itemsize
     c = shape[-1]
-    return torch.empty((*shape[:-1], -(-c // per) * per), dtype=dtype, device=device)[..., :c]
+    wide = -(-c // per) * per
+    t = torch.empty((*shape[:-1], wide), dtype=dtype, device=device)
+    return t if wide == c else t[..., :c]
 
 
 def operand(t):
     """(tensor, row stride) fit for a product: t itself where its rows are contiguous and start on 16-byte
     boundaries, else a copy."""
     ld = row_stride(t)
-    size = t.element_size()
+    size = t.dtype.itemsize
     if ld is not None and t.shape[-2] == 1:
         ld = -(-ld * size // 16) * 16 // size   # the stride of a single row is never taken
     if ld is None or ld * size % 16 or t.data_ptr() % 16 or (t.dim() == 3 and t.shape[0] > 1 and t.stride(0) * size % 16):
@@ -75,18 +84,14 @@ def operand(t):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(m, n, k, fp8, device):
-    return _lib.lib().aeisu_product_workspace(m, n, k, fp8, device)
+def product_bytes(m, n, k, fp8, index):
+    return _lib.lib().aeisu_product_workspace(m, n, k, fp8, index)
 
 
-def product(device, ma, mb, bias, dtype):
-    """a @ b.T (+ bias) of two aeisu_matrix operands on the device's current stream."""
-    out = torch.empty((ma.rows, mb.rows), dtype=dtype, device=device)
-    size = _workspace_bytes(ma.rows, mb.rows, ma.cols, int(ma.type >= 3), device.index)
-    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    mo = matrix(out, mb.rows)
-    _lib.check(_lib.lib().aeisu_product(
-        C.byref(ma), C.byref(mb), None if bias is None else bias.data_ptr(),
-        0 if bias is None else TYPES[bias.dtype], C.byref(mo), None if ws is None else ws.data_ptr(), size,
-        device.index, stream(device)))
-    return out
+@functools.lru_cache(maxsize=4096)
+def linear_bytes(m, n, k, train, index):
+    return _lib.lib().aeisu_linear_workspace(m, n, k, train, index)
+
+
+def scratch(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device)

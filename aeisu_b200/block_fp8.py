@@ -26,8 +26,6 @@ captured into a CUDA graph.  float64 is refused rather than computed at a lower 
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -89,8 +87,10 @@ class BlockFP8:
 
 def _empty(shape, rows, dtype, device):
     codes = mx.empty_rows(shape, dtype, device)
-    scales = torch.empty((*shape[:-2], mx.blocks(shape[-1]), -(-shape[-2] // rows)), dtype=torch.uint8, device=device)
-    return BlockFP8(codes, scales.view(_E8M0), rows)
+    scales = torch.empty((*shape[:-2], mx.blocks(shape[-1]), -(-shape[-2] // rows)), dtype=_E8M0, device=device)
+    q = BlockFP8.__new__(BlockFP8)
+    q.codes, q.scales, q.rows = codes, scales, rows
+    return q
 
 
 def _out(q):
@@ -106,21 +106,19 @@ def _quantize(x, rows, dtype, both):
         raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2; got {dtype}")
     if x.dtype not in mx.FLOATS:
         raise TypeError(f"quantize takes float32, float16 or bfloat16; got {x.dtype}")
-    mx.need_cuda("quantize", x)
-    x = x.detach()
-    ld = mx.row_stride(x)
-    if ld is None:
-        x = x.contiguous()
-        ld = x.shape[-1]
+    index = mx.need_cuda("quantize", x)
     if both and x.shape[-2] == 0:
         raise ValueError("Expected values with at least one row")
-    q = _empty(x.shape, rows, dtype, x.device)
-    t = _empty((*x.shape[:-2], x.shape[-1], x.shape[-2]), rows, dtype, x.device) if both else None
+    ld = mx.row_stride(x)
+    if ld is None:
+        x = x.detach().contiguous()
+        ld = x.shape[-1]
+    device = x.device
+    q = _empty(x.shape, rows, dtype, device)
+    t = _empty((*x.shape[:-2], x.shape[-1], x.shape[-2]), rows, dtype, device) if both else None
     if x.numel():
-        mt = None if t is None else _out(t)
-        m, mq = mx.matrix(x, ld), _out(q)
-        _lib.check(_lib.lib().aeisu_block_quantize(C.byref(m), rows, C.byref(mq), None if mt is None else C.byref(mt),
-                                                   x.device.index, mx.stream(x.device)))
+        _lib.check(_lib.lib().aeisu_block_quantize(mx.matrix(x, ld), rows, _out(q), None if t is None else _out(t), index,
+                                                   mx.stream(index)))
     return q, t
 
 
@@ -134,13 +132,15 @@ def quantize_both(x, *, rows=1, dtype=torch.float8_e4m3fn):
     return _quantize(x, rows, dtype, True)
 
 
-def _check_bias(bias, n):
+def _bias(bias, n):
+    """The bias ready for the library; None without one."""
     if bias is None:
-        return
+        return None
     if tuple(bias.shape) != (n,):
         raise ValueError(f"Expected bias [{n}]")
     if bias.dtype not in mx.FLOATS:
         raise TypeError(f"bias must be float32, float16 or bfloat16; got {bias.dtype}")
+    return bias if n == 1 or bias.stride(0) == 1 else bias.contiguous()
 
 
 def matmul(a, b, *, bias=None, dtype=torch.bfloat16):
@@ -151,64 +151,82 @@ def matmul(a, b, *, bias=None, dtype=torch.bfloat16):
         raise ValueError("Expected operands [M, K] and [N, K]")
     if dtype not in mx.FLOATS:
         raise TypeError(f"matmul gives float32, float16 or bfloat16; got {dtype}")
-    _check_bias(bias, b.shape[0])
-    mx.need_cuda("matmul", a.codes, b.codes, *(() if bias is None else (bias,)))
-    if a.shape[0] == 0 or b.shape[0] == 0:
-        return torch.empty((a.shape[0], b.shape[0]), dtype=dtype, device=a.device)
+    (m, k), n = a.shape, b.shape[0]
+    bias = _bias(bias, n)
+    index = mx.need_cuda("matmul", a.codes, b.codes, *(() if bias is None else (bias,)))
+    device = a.codes.device
+    out = torch.empty((m, n), dtype=dtype, device=device)
+    if m == 0 or n == 0:
+        return out
     (ka, ma), (kb, mb) = a.matrix(), b.matrix()
-    return mx.product(a.device, ma, mb, None if bias is None else bias.detach().contiguous(), dtype)
+    size = mx.product_bytes(m, n, k, 1, index)
+    ws = mx.scratch(size, device) if size else None
+    _lib.check(_lib.lib().aeisu_product(ma, mb, None if bias is None else bias.data_ptr(),
+                                        0 if bias is None else mx.TYPES[bias.dtype], mx.matrix(out, n),
+                                        None if ws is None else ws.data_ptr(), size, index, mx.stream(index)))
+    return out
 
 
-def _column_sum(x, dtype):
-    lib = _lib.lib()
-    out = torch.empty(x.shape[1], dtype=dtype, device=x.device)
-    size = lib.aeisu_column_sum_workspace(*x.shape)
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    m = mx.matrix(x, mx.row_stride(x))
-    _lib.check(lib.aeisu_column_sum(C.byref(m), out.data_ptr(), mx.TYPES[dtype], ws.data_ptr(), size, x.device.index,
-                                    mx.stream(x.device)))
+def _rows(x):
+    """(tensor, aeisu_matrix) of values whose rows may start anywhere."""
+    ld = mx.row_stride(x)
+    if ld is None:
+        x = x.contiguous()
+        ld = x.shape[-1]
+    return x, mx.matrix(x, ld)
+
+
+def _forward(x, weight, bias, kept_x, kept_w, index):
+    """The layer on float x and weight, leaving the transposed codes in the kept buffers."""
+    (m, k), n, device = x.shape, weight.shape[0], x.device
+    out = torch.empty((m, n), dtype=x.dtype, device=device)
+    size = mx.linear_bytes(m, n, k, 1, index)
+    ws = mx.scratch(size, device)
+    (x, mat), (weight, mw) = _rows(x), _rows(weight)
+    _lib.check(_lib.lib().aeisu_linear_forward(
+        mat, mw, None if bias is None else bias.data_ptr(), 0 if bias is None else mx.TYPES[bias.dtype],
+        mx.matrix(out, n), None if kept_x is None else kept_x.data_ptr(), None if kept_w is None else kept_w.data_ptr(),
+        ws.data_ptr(), size, index, mx.stream(index)))
     return out
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, grad_dtype):
-        need_x, need_w = ctx.needs_input_grad[:2]
-        ctx.sizes = x.shape, weight.shape
+        (m, k), n, device = x.shape, weight.shape[0], x.device
+        ctx.sizes = m, n, k
         ctx.types = (x.dtype, weight.dtype, None if bias is None else bias.dtype, grad_dtype)
-        if x.shape[0] == 0:
-            ctx.kept = None
-            return x.new_empty(0, weight.shape[0])
-        q, qt = _quantize(x, 1, torch.float8_e4m3fn, need_w)
-        w, wt = _quantize(weight, mx.BLOCK, torch.float8_e4m3fn, need_x)
-        ctx.kept = [None if t is None else t.rows for t in (qt, wt)]
-        ctx.save_for_backward(*(None if t is None else v for t in (qt, wt) for v in (
-            (None, None) if t is None else (t.codes, t.scales))))
-        return matmul(q, w, bias=bias, dtype=x.dtype)
+        need_x, need_w = ctx.needs_input_grad[:2]
+        kept_x = kept_w = None
+        if m == 0:
+            return x.new_empty(0, n)
+        lib = _lib.lib()
+        if need_w:
+            kept_x = mx.scratch(lib.aeisu_linear_kept_bytes(m, k, 1), device)
+        if need_x:
+            kept_w = mx.scratch(lib.aeisu_linear_kept_bytes(n, k, mx.BLOCK), device)
+        ctx.save_for_backward(kept_x, kept_w)
+        return _forward(x, weight, bias, kept_x, kept_w, device.index)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         x_type, w_type, b_type, grad_dtype = ctx.types
-        if ctx.kept is None:   # no rows
-            x_size, w_size = ctx.sizes
-            return (grad.new_empty(x_size, dtype=x_type), grad.new_zeros(w_size, dtype=w_type),
-                    None if b_type is None else grad.new_zeros(w_size[0], dtype=b_type), None)
-        saved = ctx.saved_tensors
-        qt, wt = (None if rows is None else BlockFP8(saved[2 * i], saved[2 * i + 1], rows)
-                  for i, rows in enumerate(ctx.kept))
-        if mx.row_stride(grad) is None:
-            grad = grad.contiguous()
-        gx = gw = gb = None
-        if qt is not None:
-            g, gt = _quantize(grad, 1, grad_dtype, True)
-            gw = matmul(gt, qt, dtype=w_type)
-        elif wt is not None:
-            g = quantize(grad, dtype=grad_dtype)
-        if wt is not None:
-            gx = matmul(g, wt, dtype=x_type)
-        if ctx.needs_input_grad[2]:
-            gb = _column_sum(grad, b_type)
+        (m, n, k), (need_x, need_w, need_b, _), device = ctx.sizes, ctx.needs_input_grad, grad.device
+        new = torch.zeros if m == 0 else torch.empty
+        gx = new((m, k), dtype=x_type, device=device) if need_x else None
+        gw = new((n, k), dtype=w_type, device=device) if need_w else None
+        gb = new((n,), dtype=b_type, device=device) if need_b else None
+        if m == 0:
+            return gx, gw, gb, None
+        kept_x, kept_w = ctx.saved_tensors
+        grad, mg = _rows(grad)
+        size = mx.linear_bytes(m, n, k, 2, device.index)
+        ws = mx.scratch(size, device)
+        _lib.check(_lib.lib().aeisu_linear_backward(
+            mg, k, mx.TYPES[grad_dtype], *(v for t in (kept_x, kept_w) for v in (None if t is None else t.data_ptr(),)),
+            *(v for t in (gx, gw, gb) for v in ((None, 0) if t is None else (t.data_ptr(), mx.TYPES[t.dtype]))),
+            ws.data_ptr(), size, device.index, mx.stream(device.index)))
         return gx, gw, gb, None
 
 
@@ -226,23 +244,32 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
         raise TypeError(f"weight must be float32, float16, bfloat16 or BlockFP8; got {weight.dtype}")
     if grad_dtype not in mx.CODES:
         raise TypeError(f"grad_dtype must be float8_e4m3fn or float8_e5m2; got {grad_dtype}")
-    if x.dim() < 1 or len(weight.shape) != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+    shape, wide = x.shape, weight.shape
+    if len(shape) < 1 or len(wide) != 2 or shape[-1] != wide[1] or 0 in wide:
         raise ValueError("Expected x [..., K] and weight [N, K]")
-    _check_bias(bias, weight.shape[0])
-    mx.need_cuda("linear", x, weight.codes if serving else weight, *(() if bias is None else (bias,)))
-    wants = torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                            for t in (x, None if serving else weight, bias))
-    if serving and wants:
-        raise ValueError("FP8 weights serve without gradients: pass the float weight to train")
-    lead = x.shape[:-1]
-    flat = x.reshape(lead.numel(), x.shape[-1])
-    with torch.autocast(device_type="cuda", enabled=False):
-        if wants:
-            y = _Linear.apply(flat, weight, bias, grad_dtype)
-        else:
-            w = weight if serving else quantize(weight, rows=mx.BLOCK)
-            y = matmul(quantize(flat), w, bias=bias, dtype=x.dtype)
-    return y.reshape(*lead, weight.shape[0])
+    n, k = wide
+    ready = _bias(bias, n)
+    index = mx.need_cuda("linear", x, weight.codes if serving else weight, *(() if bias is None else (bias,)))
+    flat = x if len(shape) == 2 else x.reshape(shape[:-1].numel(), k)
+    if torch.is_grad_enabled() and (x.requires_grad or (not serving and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        if serving:
+            raise ValueError("FP8 weights serve without gradients: pass the float weight to train")
+        y = _Linear.apply(flat, weight, ready, grad_dtype)
+    elif flat.shape[0] == 0:
+        y = flat.new_empty(0, n)
+    elif not serving:
+        y = _forward(flat, weight, ready, None, None, index)
+    else:
+        m, device = flat.shape[0], flat.device
+        y = torch.empty((m, n), dtype=x.dtype, device=device)
+        size = mx.linear_bytes(m, n, k, 0, index)
+        ws = mx.scratch(size, device)
+        (flat, mat), (codes, mw) = _rows(flat), weight.matrix()
+        _lib.check(_lib.lib().aeisu_linear(mat, mw, None if ready is None else ready.data_ptr(),
+                                           0 if ready is None else mx.TYPES[ready.dtype], mx.matrix(y, n), ws.data_ptr(),
+                                           size, index, mx.stream(index)))
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
 
 
 __all__ = ["BlockFP8", "quantize", "quantize_both", "matmul", "linear"]

@@ -53,16 +53,34 @@ struct ProductOut {
     int bias_type;
 };
 size_t product_workspace(int m, int n, int k, bool fp8, int device);
+// after_quantize: the kernel enqueued just before on `stream` is the quantiser of an operand, and the
+// product may start while it runs.
 void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const ScaleRef* sb, const ProductOut& out,
-             void* workspace, size_t workspace_bytes, int device, cudaStream_t stream);
+             void* workspace, size_t workspace_bytes, bool after_quantize, int device, cudaStream_t stream);
 
 // Rows t in [off[e], off[e + 1]) of x [rows][k] times b[e] [n][k]: out[t][n].  Rows outside every
 // group are zeroed when zero_outside is set, otherwise left as they were.
 void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const ScaleRef* sb, const int* off,
-                     const ProductOut& out, bool zero_outside, int device, cudaStream_t stream);
+                     const ProductOut& out, bool zero_outside, bool after_quantize, int device, cudaStream_t stream);
 // out[e][n][k] = sum over t in group e of g[t][n] x[t][k].
 void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* off, int groups, void* out,
                              int out_type, int device, cudaStream_t stream);
+// The linear layer in block-scaled FP8 (linear.cpp): quantiser and products in one call, operands
+// and partial results carved out of one workspace.
+enum LinearPass { kServe = 0, kTrainForward = 1, kTrainBackward = 2 };
+size_t linear_workspace(int m, int n, int k, int pass, int device);
+size_t transposed_codes_bytes(int rows, int cols, int block_rows);   // codes and scales of the transpose
+void linear_serve(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, const ProductOut& out, void* workspace,
+                  size_t workspace_bytes, int device, cudaStream_t stream);
+void linear_train_forward(const MatrixRef& x, const MatrixRef& w, const ProductOut& out, void* kept_x, void* kept_w,
+                          void* workspace, size_t workspace_bytes, int device, cudaStream_t stream);
+void linear_train_backward(const MatrixRef& grad, int k, int code_type, const void* kept_x, const void* kept_w,
+                           void* gx, int gx_type, void* gw, int gw_type, void* gb, int gb_type, void* workspace,
+                           size_t workspace_bytes, int device, cudaStream_t stream);
+size_t grouped_linear_workspace(int rows, int k);
+void grouped_linear(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, const int* off, const ProductOut& out,
+                    bool zero_outside, void* workspace, size_t workspace_bytes, int device, cudaStream_t stream);
+
 // The error code that a product kernel left behind on `device` (0: none), cleared; waits for the device.
 int product_status(int device);
 

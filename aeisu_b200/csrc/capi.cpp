@@ -82,6 +82,7 @@ struct Scales {   // the scales of an FP8 operand, none for a 16-bit one
 };
 aeisu::ProductOut product_out(const aeisu_matrix* out, const void* bias, int bias_type) {
     aeisu::require(out != nullptr, "output pointer is null");
+    aeisu::require(!bias || (bias_type >= 0 && bias_type <= 2), "bias must be float32, float16 or bfloat16");
     return {const_cast<void*>(out->data), out->type, (long long)out->ld, bias, bias_type};
 }
 
@@ -295,7 +296,8 @@ int aeisu_reconstruct_backward_f32(const float* source, const float* metadata, c
     });
 }
 
-int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, aeisu_matrix* codes, aeisu_matrix* t_codes,
+int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, const aeisu_matrix* codes,
+                         const aeisu_matrix* t_codes,
                          int device, void* stream) {
     return guarded([&] {
         aeisu::require(codes != nullptr, "codes pointer is null");
@@ -336,22 +338,85 @@ uint64_t aeisu_product_workspace(int m, int n, int k, int fp8, int device) {
     return r;
 }
 
-int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias, int bias_type, aeisu_matrix* out,
+int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias, int bias_type, const aeisu_matrix* out,
                   void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
         const aeisu::MatrixRef ma = matrix(a), mb = matrix(b);
         const Scales sa(a), sb(b);
         aeisu::product(ma, sa.ptr, mb, sb.ptr, product_out(out, bias, bias_type), workspace, size_t(workspace_bytes),
-                       device, static_cast<cudaStream_t>(stream));
+                       false, device, static_cast<cudaStream_t>(stream));
+    });
+}
+
+uint64_t aeisu_linear_workspace(int m, int n, int k, int pass, int device) {
+    uint64_t r = 0;
+    guarded([&] {
+        aeisu::require(m >= 1 && n >= 1 && k >= 1 && pass >= 0 && pass <= 2, "matrix sizes are out of range");
+        r = aeisu::linear_workspace(m, n, k, pass, device);
+    });
+    return r;
+}
+
+uint64_t aeisu_linear_kept_bytes(int rows, int cols, int block_rows) {
+    if (rows < 1 || cols < 1 || (block_rows != 1 && block_rows != 128)) return 0;
+    return aeisu::transposed_codes_bytes(rows, cols, block_rows);
+}
+
+int aeisu_linear(const aeisu_matrix* x, const aeisu_matrix* weight, const void* bias, int bias_type,
+                 const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
+    return guarded([&] {
+        const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
+        aeisu::require(mx.cols == mw.cols && mx.rows >= 1, "contraction sizes differ");
+        aeisu::require(weight->scales != nullptr, "FP8 operands, and only they, come with scales");
+        aeisu::linear_serve(mx, mw, scales_of(weight), product_out(out, bias, bias_type), workspace,
+                            size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int aeisu_linear_forward(const aeisu_matrix* x, const aeisu_matrix* weight, const void* bias, int bias_type,
+                         const aeisu_matrix* out, void* kept_x, void* kept_weight, void* workspace,
+                         uint64_t workspace_bytes, int device, void* stream) {
+    return guarded([&] {
+        const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
+        aeisu::require(mx.cols == mw.cols && mx.rows >= 1 && mw.rows >= 1, "contraction sizes differ");
+        aeisu::linear_train_forward(mx, mw, product_out(out, bias, bias_type), kept_x, kept_weight, workspace,
+                                    size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int aeisu_linear_backward(const aeisu_matrix* grad, int k, int code_type, const void* kept_x, const void* kept_weight,
+                          void* grad_x, int grad_x_type, void* grad_weight, int grad_weight_type, void* grad_bias,
+                          int grad_bias_type, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
+    return guarded([&] {
+        const aeisu::MatrixRef g = matrix(grad);
+        aeisu::require(g.rows >= 1 && g.cols >= 1, "matrix sizes are out of range");
+        aeisu::linear_train_backward(g, k, code_type, kept_x, kept_weight, grad_x, grad_x_type, grad_weight,
+                                     grad_weight_type, grad_bias, grad_bias_type, workspace, size_t(workspace_bytes),
+                                     device, static_cast<cudaStream_t>(stream));
+    });
+}
+
+uint64_t aeisu_grouped_linear_workspace(int rows, int k) {
+    return rows >= 1 && k >= 1 ? aeisu::grouped_linear_workspace(rows, k) : 0;
+}
+
+int aeisu_grouped_linear(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
+                         const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
+    return guarded([&] {
+        const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
+        aeisu::require(mx.cols == mw.cols && mx.rows >= 1, "contraction sizes differ");
+        aeisu::require(weight->scales != nullptr, "FP8 operands, and only they, come with scales");
+        aeisu::grouped_linear(mx, mw, scales_of(weight), offsets, product_out(out, nullptr, 0), zero_outside != 0,
+                              workspace, size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
     });
 }
 
 int aeisu_grouped_product(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
-                          aeisu_matrix* out, int device, void* stream) {
+                          const aeisu_matrix* out, int device, void* stream) {
     return guarded([&] {
         const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
         const Scales sx(x), sw(weight);
-        aeisu::grouped_product(mx, sx.ptr, mw, sw.ptr, offsets, product_out(out, nullptr, 0), zero_outside != 0, device,
+        aeisu::grouped_product(mx, sx.ptr, mw, sw.ptr, offsets, product_out(out, nullptr, 0), zero_outside != 0, false, device,
                                static_cast<cudaStream_t>(stream));
     });
 }

@@ -89,12 +89,16 @@ struct QuantJob {
     int tiles;
 };
 
+// The product that reads the codes may start its set-up now; it waits for this kernel's end.
+__device__ __forceinline__ void let_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // One scale per row and block column, no transpose.  Eight lanes share a block (two loads of eight
 // values each), a warp takes four neighbouring blocks of four rows, a CTA 32 rows of them; the
 // scales leave through shared memory as 32 contiguous bytes per block column.
 template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
     __shared__ uint8_t sh[4][32];
+    let_dependents_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int col_groups = (j.cols + 4 * kBlock - 1) / (4 * kBlock);
     const int r0 = int(blockIdx.x / col_groups) * 32, c0 = int(blockIdx.x % col_groups) * 4 * kBlock;
@@ -152,6 +156,7 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
     __shared__ uint8_t row_s[kBlock];
     __shared__ float tile_max[8];
     __shared__ __align__(16) uint32_t turn[BOTH ? kBlock * 32 : 4];
+    let_dependents_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, oct = lane & 7, sub = lane >> 3;
     const int col_blocks = (j.cols + kBlock - 1) / kBlock, row_blocks = (j.rows + kBlock - 1) / kBlock;
     const int rb = int(blockIdx.x / col_blocks), cb = int(blockIdx.x % col_blocks);

@@ -56,9 +56,12 @@ struct ProdJob {
     int cols;                    // columns of out
     const void* bias;
     int bias_type;
-    int split, steps_per_split;  // the contraction in `split` parts, each to its own partial output
-    long long split_stride;
+    int split, steps_per_split;  // the contraction in `split` parts:
+    int cluster;                 //   of the CTAs of a cluster, joined in its shared memory (split > 1), or (1)
+    long long split_stride;      //   each to its own partial output
     int zero_outside, zero_rows;
+    int after_quantize;          // starts while the quantiser of its float operand still runs; the other
+                                 // operand and the offsets are older
 };
 
 template <bool FP8, int BN>
@@ -111,6 +114,22 @@ __device__ __forceinline__ void tma_3d(uint32_t smem, const CUtensorMap* map, in
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         :: "r"(smem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar)) : "memory");
+}
+
+// Thread block clusters: rank, barrier and another CTA's shared memory.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_float(uint32_t saddr, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}\n"
+                 : "=f"(v) : "r"(saddr), "r"(rank) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
@@ -330,6 +349,10 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
     const int tiles = tile_count<BN>(j, g);
+    // A cluster takes one tile, each of its CTAs a part of the contraction.
+    const int rank = j.cluster > 1 ? int(cluster_rank()) : 0;
+    const int first_tile = j.cluster > 1 ? rank * (tiles / j.split) + int(blockIdx.x) / j.cluster : int(blockIdx.x);
+    const int stride = j.cluster > 1 ? tiles : int(gridDim.x);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -337,7 +360,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             uint32_t phase = 0;
             bool ok = true;
             long long issued = 0;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            if (j.after_quantize) grid_dep_wait();
+            for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BN>(j, g, t, kStep);
                 const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
                 for (int k = x.k0; k < x.k1; k += kStep) {
@@ -371,7 +395,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             bool ok = true;
             uint64_t* ready = j.grouping == kContraction ? fixed : full;
             const uint32_t a_k = (j.a_mn ? 2048 : 32) >> 4, b_k = (j.b_mn ? 2048 : 32) >> 4;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BN>(j, g, t, kStep);
                 if (!(ok = wait(acc_empty + acc, acc_phase ^ 1))) break;
                 fence_after_sync();
@@ -418,8 +442,9 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         uint32_t phase = 0;
         bool ok = true;
         if constexpr (FP8) {
+            if (j.after_quantize) grid_dep_wait();
             const int blocks = (j.K + kBlock - 1) / kBlock;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BN>(j, g, t, kStep);
                 const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
                 int step = 0;
@@ -444,7 +469,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 }
             }
         } else if (j.grouping == kContraction) {
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BN>(j, g, t, kStep);
                 for (int k = x.k0; k < x.k1; k += kStep) {
                     if (!(ok = wait(full + stage, phase))) break;
@@ -468,7 +493,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         const int quad = warp & 3, row = quad * 32 + lane;
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+        for (int t = first_tile; t < tiles; t += stride) {
             const Tile x = tile_at<BN>(j, g, t, kStep);
             if (!wait(acc_full + acc, acc_phase)) break;
             fence_after_sync();
@@ -485,7 +510,11 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     for (int i = 0; i < W; ++i) v[i] = 0.f;
                 }
                 const int q = x.q0 + c, n = x.q1 - q;
-                if (p < x.p1 && n > 0) {
+                if (j.cluster > 1) {
+                    // every MMA of this CTA is done with the ring: it takes the tile, column by column
+#pragma unroll
+                    for (int i = 0; i < W; ++i) reinterpret_cast<float*>(ring)[(c + i) * kBM + row] = v[i];
+                } else if (p < x.p1 && n > 0) {
                     if (!j.swapped) {
                         if (j.bias)
 #pragma unroll
@@ -513,6 +542,24 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 store_elem(j.out, j.out_type, at * j.out_ld + i % j.cols, 0.f);
             }
         }
+    }
+    if (j.cluster > 1) {
+        // The parts are added in their order, each CTA taking its share of the columns.
+        cluster_sync();
+        if (warp >= 4 && first_tile < tiles) {
+            const Tile x = tile_at<BN>(j, g, first_tile, kStep);
+            const int row = threadIdx.x - 128, p = x.p0 + row, share = BN / j.cluster;
+            const float pb = j.bias && j.swapped && p < x.p1 ? load_elem(j.bias, j.bias_type, p) : 0.f;
+            for (int c = rank * share; c < (rank + 1) * share; ++c) {
+                const int q = x.q0 + c;
+                if (p >= x.p1 || q >= x.q1) continue;
+                float v = 0.f;
+                for (int r = 0; r < j.cluster; ++r) v += peer_float(smem_addr(ring) + (c * kBM + row) * 4, r);
+                if (j.swapped) store_elem(j.out, j.out_type, q * j.out_ld + p, v + pb);
+                else store_elem(j.out, j.out_type, p * j.out_ld + q, v + (j.bias ? load_elem(j.bias, j.bias_type, q) : 0.f));
+            }
+        }
+        cluster_sync();
     }
     fence_before_sync();
     __syncthreads();
@@ -609,8 +656,20 @@ void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long l
             ready[device] = true;
         }
     }
-    k_product<FP8, BN><<<unsigned(std::min<long long>(tiles, sms)), kThreads, smem, stream>>>(a, b, j);
-    AEISU_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(j.cluster > 1 ? tiles : std::min<long long>(tiles, sms)), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = j.after_quantize;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(j.cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = j.cluster > 1 ? 2 : 1;
+    AEISU_CUDA(cudaLaunchKernelEx(&cfg, k_product<FP8, BN>, a, b, j));
 }
 
 template <bool FP8>
@@ -645,6 +704,7 @@ int width_for(int rows, bool trans) {
 struct Plan {
     bool swap;
     int bn, split, steps;   // steps of the contraction per part
+    int cluster;
 };
 
 Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
@@ -656,11 +716,22 @@ Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
     p.bn = width_for(Q, false);
     auto tiles = [&](int bn) { return (long long)((P + kBM - 1) / kBM) * ((Q + bn - 1) / bn); };
     while (p.bn > 64 && tiles(p.bn) < sms) p.bn /= 2;
-    // Parts of at least four steps while SMs are left over.
+    // While SMs are left over, the contraction is cut: into 2, 4 or 8 parts of at least two steps, the CTAs
+    // of a cluster, which need no second kernel; where that fills less than half of the SMs and the
+    // contraction is long, into as many parts as fill them, of at least eight steps, joined by a kernel.
     const long long t = tiles(p.bn);
-    long long split = t >= sms ? 1 : std::min<long long>(sms / t, std::max(1, steps / 4));
-    p.steps = int((steps + split - 1) / split);
-    p.split = (steps + p.steps - 1) / p.steps;
+    p.cluster = p.split = 1;
+    p.steps = steps;
+    while (p.cluster < 8 && t * p.cluster * 2 <= sms && steps >= 4 * p.cluster) p.cluster *= 2;
+    const long long wide = std::min<long long>(sms / t, steps / 8);
+    if (t < sms && wide >= 2 * p.cluster) {
+        p.cluster = 1;
+        p.split = int(wide);
+    } else {
+        p.split = p.cluster;
+    }
+    p.steps = (steps + p.split - 1) / p.split;
+    if (p.cluster == 1) p.split = (steps + p.steps - 1) / p.steps;
     return p;
 }
 
@@ -668,11 +739,11 @@ Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
 
 size_t product_workspace(int m, int n, int k, bool fp8, int device) {
     const Plan p = plan_dense(m, n, k, fp8, sm_count(device));
-    return p.split > 1 ? size_t(p.split) * m * n * sizeof(float) : 0;
+    return p.split > p.cluster ? size_t(p.split) * m * n * sizeof(float) : 0;
 }
 
 void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const ScaleRef* sb, const ProductOut& out,
-             void* workspace, size_t workspace_bytes, int device, cudaStream_t stream) {
+             void* workspace, size_t workspace_bytes, bool after_quantize, int device, cudaStream_t stream) {
     check_operand(a, sa);
     check_operand(b, sb);
     require(a.batch == 1 && b.batch == 1 && !a.trans && !b.trans && a.cols == b.cols, "contraction sizes differ");
@@ -681,7 +752,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     OnDevice on(device);
     const bool fp8 = sa != nullptr;
     const Plan pl = plan_dense(a.rows, b.rows, a.cols, fp8, sm_count(device));
-    const size_t need = pl.split > 1 ? size_t(pl.split) * a.rows * b.rows * sizeof(float) : 0;
+    const size_t need = pl.split > pl.cluster ? size_t(pl.split) * a.rows * b.rows * sizeof(float) : 0;
     require(need == 0 || (workspace && workspace_bytes >= need), "workspace is too small");
     const MatrixRef& A = pl.swap ? b : a;
     const MatrixRef& B = pl.swap ? a : b;
@@ -702,7 +773,9 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     j.cols = b.rows;
     j.split = pl.split;
     j.steps_per_split = pl.steps;
-    if (pl.split > 1) {
+    j.cluster = pl.cluster;
+    j.after_quantize = after_quantize;
+    if (pl.split > pl.cluster) {
         j.out = workspace;
         j.out_type = kF32;
         j.out_ld = b.rows;
@@ -719,7 +792,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM), mb = operand_map(B, B.trans ? 64 : pl.bn);
     if (fp8) launch_width<true>(pl.bn, ma, mb, j, tiles, device, stream);
     else launch_width<false>(pl.bn, ma, mb, j, tiles, device, stream);
-    if (pl.split > 1) {
+    if (pl.split > pl.cluster) {
         const long long n = (long long)a.rows * b.rows;
         k_join_parts<<<unsigned(std::min<long long>((n + 255) / 256, 148 * 8)), 256, 0, stream>>>(
             static_cast<const float*>(workspace), pl.split, j.split_stride, a.rows, b.rows, out.ptr, out.type, out.ld,
@@ -729,7 +802,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
 }
 
 void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const ScaleRef* sb, const int* off,
-                     const ProductOut& out, bool zero_outside, int device, cudaStream_t stream) {
+                     const ProductOut& out, bool zero_outside, bool after_quantize, int device, cudaStream_t stream) {
     check_operand(x, sx);
     check_operand(b, sb);
     require(x.batch == 1 && !x.trans && x.cols == b.cols, "contraction sizes differ");
@@ -769,7 +842,8 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     j.out_ld = out.ld;
     j.swapped = swap;
     j.cols = b.rows;
-    j.split = 1;
+    j.split = j.cluster = 1;
+    j.after_quantize = after_quantize;
     j.zero_outside = zero_outside;
     j.zero_rows = x.rows;
     const int high = swap ? bn : kBM, wide = swap ? kBM : bn;
@@ -808,7 +882,7 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     j.out_ld = x.rows;
     j.out_batch = (long long)g.rows * x.rows;
     j.cols = x.rows;
-    j.split = 1;
+    j.split = j.cluster = 1;
     require(count(bn) < (1LL << 30), "matrix is too large");
     launch_width<false>(bn, operand_map(g, 64), operand_map(x, 64), j, count(bn), device, stream);
 }

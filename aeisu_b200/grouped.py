@@ -14,14 +14,12 @@ Rows in no group are zero, or, with ``out``, left as they were there.
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import _matrices as mx
-from .block_fp8 import BlockFP8, quantize
+from .block_fp8 import BlockFP8
 
 MAX_GROUPS = 1024
 _HALVES = (torch.float16, torch.bfloat16)
@@ -39,9 +37,9 @@ def _weights(weight):
 
 def _product(x, weight, offsets, out, zero_outside):
     """x, weight: (tensors kept, aeisu_matrix)."""
-    mo = mx.matrix(out, mx.row_stride(out))
-    _lib.check(_lib.lib().aeisu_grouped_product(C.byref(x[1]), C.byref(weight[1]), offsets.data_ptr(),
-                                                int(zero_outside), C.byref(mo), out.device.index, mx.stream(out.device)))
+    index = out.device.index
+    _lib.check(_lib.lib().aeisu_grouped_product(x[1], weight[1], offsets.data_ptr(), zero_outside,
+                                                mx.matrix(out, mx.row_stride(out)), index, mx.stream(index)))
     return out
 
 
@@ -68,13 +66,15 @@ class _Grouped(torch.autograd.Function):
         g = _rows(grad)
         gx = gw = None
         if ctx.needs_input_grad[0]:
-            gx = _product(g, _weights(weight.transpose(1, 2)), offsets, torch.empty_like(x, memory_format=torch.contiguous_format), True)
+            gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            _product(g, _weights(weight.transpose(1, 2)), offsets, gx, True)
         if ctx.needs_input_grad[1]:
             gw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
             kept = _rows(x)
-            _lib.check(_lib.lib().aeisu_grouped_weight_gradient(
-                C.byref(g[1]), C.byref(kept[1]), offsets.data_ptr(), weight.shape[0], gw.data_ptr(),
-                mx.TYPES[gw.dtype], gw.device.index, mx.stream(gw.device)))
+            index = gw.device.index
+            _lib.check(_lib.lib().aeisu_grouped_weight_gradient(g[1], kept[1], offsets.data_ptr(), weight.shape[0],
+                                                                gw.data_ptr(), mx.TYPES[gw.dtype], index,
+                                                                mx.stream(index)))
         return gx, gw, None
 
 
@@ -108,26 +108,34 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
     t, n = x.shape[0], weight.shape[1]
     if out is not None and (tuple(out.shape) != (t, n) or out.dtype != dtype or (t and mx.row_stride(out) is None)):
         raise ValueError(f"Expected out [{t}, {n}] of {dtype} with contiguous rows")
-    mx.need_cuda("grouped_matmul", x.codes if coded else x, weight.codes if fp8 else weight, offsets,
-                 *(() if out is None else (out,)))
-    wants = torch.is_grad_enabled() and any(not isinstance(v, BlockFP8) and v.requires_grad for v in (x, weight))
-    if wants and (fp8 or out is not None):
-        raise ValueError("FP8 weights and out serve without gradients")
-    offsets = offsets.contiguous()
-    if t == 0 and not wants:
-        return torch.empty((0, n), dtype=dtype, device=offsets.device) if out is None else out
-    if wants:
-        with torch.autocast(device_type="cuda", enabled=False):
-            return _Grouped.apply(x, weight, offsets)
-    if fp8:
-        q = x if coded else quantize(x)
-        mx_, mw = q.matrix(), weight.matrix()
-    else:
-        mx_, mw = _rows(x.detach()), _weights(weight.detach())
+    index = mx.need_cuda("grouped_matmul", x.codes if coded else x, weight.codes if fp8 else weight, offsets,
+                         *(() if out is None else (out,)))
+    if torch.is_grad_enabled() and ((not coded and x.requires_grad) or (not fp8 and weight.requires_grad)):
+        if fp8 or out is not None:
+            raise ValueError("FP8 weights and out serve without gradients")
+        return _Grouped.apply(x, weight, offsets.contiguous())
+    device = offsets.device
     new = out is None
     if new:
-        out = torch.empty((t, n), dtype=dtype, device=offsets.device)
-    return _product(mx_, mw, offsets, out, new)
+        out = torch.empty((t, n), dtype=dtype, device=device)
+    if t == 0:
+        return out
+    offsets = offsets.contiguous()
+    if not fp8:
+        return _product(_rows(x), _weights(weight), offsets, out, new)
+    if coded:
+        return _product(x.matrix(), weight.matrix(), offsets, out, new)
+    k = x.shape[1]
+    ld = mx.row_stride(x)
+    if ld is None:
+        x = x.detach().contiguous()
+        ld = k
+    size = _lib.lib().aeisu_grouped_linear_workspace(t, k)
+    ws, (codes, mw) = mx.scratch(size, device), weight.matrix()
+    _lib.check(_lib.lib().aeisu_grouped_linear(mx.matrix(x, ld), mw, offsets.data_ptr(), new,
+                                               mx.matrix(out, mx.row_stride(out)), ws.data_ptr(), size, index,
+                                               mx.stream(index)))
+    return out
 
 
 __all__ = ["grouped_matmul", "MAX_GROUPS"]

@@ -340,8 +340,8 @@ typedef struct aeisu_matrix {
  * 2^-127), amax over the block's finite values; a code is x / s rounded to nearest even, NaN where x
  * is not finite.  Writes codes->data, codes->scales; up to 15 bytes after each row of codes, within
  * ld, are overwritten. */
-int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, aeisu_matrix* codes, aeisu_matrix* t_codes,
-                         int device, void* stream);
+int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, const aeisu_matrix* codes,
+                         const aeisu_matrix* t_codes, int device, void* stream);
 
 /* out[c] = sum over the rows of x[r][c], added in float32 in a fixed order. */
 uint64_t aeisu_column_sum_workspace(int rows, int cols);
@@ -352,8 +352,28 @@ int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* works
  * scales, or two of one 16-bit type; float32 accumulation, one rounding to out's type (float32,
  * float16 or bfloat16).  The order of the sum depends on the sizes alone. */
 uint64_t aeisu_product_workspace(int m, int n, int k, int fp8, int device);
-int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias, int bias_type, aeisu_matrix* out,
+int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias, int bias_type, const aeisu_matrix* out,
                   void* workspace, uint64_t workspace_bytes, int device, void* stream);
+
+/* The linear layer in block-scaled FP8, out = x weight^T + bias, as single calls that quantise
+ * their float operands into the workspace.  aeisu_linear serves: x float (quantised to E4M3 in
+ * blocks of 1 x 128), weight FP8 with scales.  aeisu_linear_forward and _backward train: weight is
+ * float too (blocks of 128 x 128); the forward call leaves the codes of the transposes of x and weight
+ * in kept_x and kept_weight (16-byte aligned, aeisu_linear_kept_bytes(rows, cols, 1 or 128) bytes; NULL where the
+ * gradient of the other one is not wanted), and the backward call turns grad [m][n] into
+ * grad_x [m][k], grad_weight [n][k] and grad_bias [n] (each NULL if not wanted; contiguous), grad quantised to
+ * code_type in blocks of 1 x 128 and 128 x 1.  Passes of aeisu_linear_workspace: 0 serving, 1 forward,
+ * 2 backward; workspaces 16-byte aligned. */
+uint64_t aeisu_linear_workspace(int m, int n, int k, int pass, int device);
+uint64_t aeisu_linear_kept_bytes(int rows, int cols, int block_rows);
+int aeisu_linear(const aeisu_matrix* x, const aeisu_matrix* weight, const void* bias, int bias_type,
+                 const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream);
+int aeisu_linear_forward(const aeisu_matrix* x, const aeisu_matrix* weight, const void* bias, int bias_type,
+                         const aeisu_matrix* out, void* kept_x, void* kept_weight, void* workspace,
+                         uint64_t workspace_bytes, int device, void* stream);
+int aeisu_linear_backward(const aeisu_matrix* grad, int k, int code_type, const void* kept_x, const void* kept_weight,
+                          void* grad_x, int grad_x_type, void* grad_weight, int grad_weight_type, void* grad_bias,
+                          int grad_bias_type, void* workspace, uint64_t workspace_bytes, int device, void* stream);
 
 /* Rows grouped by expert: out[t][n] = sum_k x[t][k] weight[e][n][k] for t in [offsets[e],
  * offsets[e + 1]); weight->batch groups (at most 1024), offsets int32 [groups + 1] in device
@@ -361,7 +381,11 @@ int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias
  * were.  Offsets outside [0, x->rows] or below the one before are moved to the nearest allowed
  * value.  Types as for aeisu_product. */
 int aeisu_grouped_product(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
-                          aeisu_matrix* out, int device, void* stream);
+                          const aeisu_matrix* out, int device, void* stream);
+/* The same with x float, quantised to E4M3 in blocks of 1 x 128 into the workspace, and FP8 weights. */
+uint64_t aeisu_grouped_linear_workspace(int rows, int k);
+int aeisu_grouped_linear(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
+                         const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream);
 /* out[e][n][k] = sum over t in group e of grad[t][n] x[t][k]; zeros for an empty group.  grad and x
  * float16 or bfloat16, not transposed; out contiguous. */
 int aeisu_grouped_weight_gradient(const aeisu_matrix* grad, const aeisu_matrix* x, const int* offsets, int groups,
