@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "blockscale_host.h"
 
@@ -19,37 +20,105 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T> struct Vec;   // sixteen bytes of T
-template <> struct Vec<float> { static constexpr int n = 4; };
-template <> struct Vec<__half> { static constexpr int n = 8; };
-template <> struct Vec<__nv_bfloat16> { static constexpr int n = 8; };
+// Sixteen values of a row as they come: pairs of 16-bit values, or floats.
+template <typename T> struct Vals {
+    static constexpr int n = 8;               // values in 16 bytes
+    uint32_t w[8];
+    __device__ __forceinline__ float get(int i) const;
+};
+template <> struct Vals<float> {
+    static constexpr int n = 4;
+    float w[16];
+    __device__ __forceinline__ float get(int i) const { return w[i]; }
+};
+template <> __device__ __forceinline__ float Vals<__nv_bfloat16>::get(int i) const {
+    return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+}
+template <> __device__ __forceinline__ float Vals<__half>::get(int i) const {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
+    return i & 1 ? __high2float(h) : __low2float(h);
+}
+
+// Largest magnitudes, lane by lane of a pair; NaN does not count.  The pair of a float is itself alone.
+template <typename T> struct Pair { using type = uint32_t; };
+template <> struct Pair<float> { using type = float; };
+template <typename T> __device__ __forceinline__ typename Pair<T>::type larger(typename Pair<T>::type a, typename Pair<T>::type b);
+template <> __device__ __forceinline__ float larger<float>(float a, float b) { return fmaxf(fabsf(a), fabsf(b)); }
+template <> __device__ __forceinline__ uint32_t larger<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)),
+                                     __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <> __device__ __forceinline__ uint32_t larger<__half>(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+// The one or two values of a pair of maxima (NaN only where every value was: then zero).
+__device__ __forceinline__ float number_or_zero(float v) { return fmaxf(v, 0.f); }
+template <typename T> __device__ __forceinline__ float first_of(typename Pair<T>::type p);
+template <typename T> __device__ __forceinline__ float second_of(typename Pair<T>::type p);
+template <> __device__ __forceinline__ float first_of<float>(float p) { return number_or_zero(p); }
+template <> __device__ __forceinline__ float second_of<float>(float) { return 0.f; }
+template <> __device__ __forceinline__ float first_of<__nv_bfloat16>(uint32_t p) { return number_or_zero(__uint_as_float(p << 16)); }
+template <> __device__ __forceinline__ float second_of<__nv_bfloat16>(uint32_t p) { return number_or_zero(__uint_as_float(p & 0xffff0000u)); }
+template <> __device__ __forceinline__ float first_of<__half>(uint32_t p) { return number_or_zero(__low2float(*reinterpret_cast<const __half2*>(&p))); }
+template <> __device__ __forceinline__ float second_of<__half>(uint32_t p) { return number_or_zero(__high2float(*reinterpret_cast<const __half2*>(&p))); }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Infinity and NaN to NaN, which fmaxf ignores and the conversion keeps.
-__device__ __forceinline__ float finite_or_nan(float v) {
-    return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : v;
-}
-
-// Eight consecutive values of a row as floats; columns at or past `cols` read as zero.
+// Eight consecutive values of a row, to places 8 h .. of v; columns at or past `cols` read as zero.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int c, int cols, float* v) {
+__device__ __forceinline__ void load8(Vals<T>& v, int h, const T* row, int c, int cols) {
+    constexpr int n = Vals<T>::n;
+    uint4* dst = reinterpret_cast<uint4*>(v.w) + h * (8 / n);
     if constexpr (VEC) {
-        constexpr int n = Vec<T>::n;
 #pragma unroll
-        for (int h = 0; h < 8 / n; ++h) {
-            uint4 q = make_uint4(0, 0, 0, 0);
-            if (c + h * n < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + h * n));
-            const T* p = reinterpret_cast<const T*>(&q);
-#pragma unroll
-            for (int i = 0; i < n; ++i) v[h * n + i] = finite_or_nan(to_f32(p[i]));
+        for (int i = 0; i < 8 / n; ++i) {
+            dst[i] = make_uint4(0, 0, 0, 0);
+            if (c + i * n < cols) dst[i] = __ldg(reinterpret_cast<const uint4*>(row + c + i * n));
         }
     } else {
+        T* e = reinterpret_cast<T*>(dst);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? finite_or_nan(to_f32(row[c + i])) : 0.f;
+        for (int i = 0; i < 8; ++i) e[i] = c + i < cols ? row[c + i] : T(0.f);
     }
+}
+
+// Infinities to NaN, which the maxima ignore and the conversion keeps.
+template <typename T>
+__device__ __forceinline__ void infinities_to_nan(Vals<T>& v) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (isinf(v.w[i])) v.w[i] = __uint_as_float(0x7fffffffu);
+    } else {
+        constexpr uint32_t inf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if ((v.w[i] & 0x7fffu) == inf) v.w[i] |= 0x7fffu;
+            if ((v.w[i] >> 16 & 0x7fffu) == inf) v.w[i] |= 0x7fff0000u;
+        }
+    }
+}
+
+// Largest magnitude of the sixteen values, after infinities became NaN (a rare second pass).
+template <typename T>
+__device__ __forceinline__ float finite_max(Vals<T>& v) {
+    auto largest = [&] {
+        auto m = v.w[0];
+#pragma unroll
+        for (int i = 1; i < int(sizeof(v.w) / 4); ++i) m = larger<T>(m, v.w[i]);
+        if constexpr (sizeof(T) == 4) return fmaxf(fabsf(m), 0.f);
+        else return fmaxf(first_of<T>(m), second_of<T>(m));
+    };
+    float m = largest();
+    if (isinf(m)) {
+        infinities_to_nan(v);
+        m = largest();
+    }
+    return m;
 }
 
 // Biased exponent of the scale.  amax = m 2^e with 0.5 <= m < 1 has the exponent field e + 126; the
@@ -105,23 +174,20 @@ __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
     const T* x = j.x + blockIdx.y * j.batch_stride;
     uint8_t* codes = j.codes + blockIdx.y * j.codes_batch;
     const int c = c0 + (lane >> 3) * kBlock + (lane & 7) * 16;
-    float v[4][16];
+    Vals<T> v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = r0 + warp * 4 + i;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[i][k] = 0.f;
+        v[i] = {};
         if (r < j.rows) {
-            load8<T, VEC>(x + r * j.ld, c, j.cols, v[i]);
-            load8<T, VEC>(x + r * j.ld, c + 8, j.cols, v[i] + 8);
+            load8<T, VEC>(v[i], 0, x + r * j.ld, c, j.cols);
+            load8<T, VEC>(v[i], 1, x + r * j.ld, c + 8, j.cols);
         }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = r0 + warp * 4 + i;
-        float amax = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(v[i][k]));
+        float amax = finite_max(v[i]);
 #pragma unroll
         for (int d = 1; d < 8; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, d));
         const uint32_t s = scale_of<E5M2>(amax);
@@ -132,8 +198,8 @@ __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
             uint32_t* w = reinterpret_cast<uint32_t*>(&q);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                w[k] = codes4<E5M2>(v[i][4 * k] * inv, v[i][4 * k + 1] * inv, v[i][4 * k + 2] * inv,
-                                    v[i][4 * k + 3] * inv);
+                w[k] = codes4<E5M2>(v[i].get(4 * k) * inv, v[i].get(4 * k + 1) * inv, v[i].get(4 * k + 2) * inv,
+                                    v[i].get(4 * k + 3) * inv);
             *reinterpret_cast<uint4*>(codes + r * j.codes_ld + c) = q;
         }
     }
@@ -147,12 +213,16 @@ __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
 
 // A 128 x 128 tile per CTA: codes with one scale per row or per tile and, with BOTH, the codes of the
 // transpose too, from one read of x.  A lane holds four consecutive rows of two runs of eight
-// columns: row maxima over eight lanes, column maxima over a lane's rows, four lanes and eight warps.
-// The transposed codes (four rows to a word) turn in shared memory; the 16-byte chunk of a column is
-// exclusive-or'ed with the column's octet, so that a warp's 32 words fall in 32 banks.
+// columns: row maxima over eight lanes, column maxima over a lane's rows, four lanes and eight warps,
+// pairs of 16-bit values at a time.  The transposed codes (four rows to a word) turn in shared memory; the
+// 16-byte chunk of a column is exclusive-or'ed with the column's octet, so that a warp's 32 words
+// fall in 32 banks.
 template <typename T, bool E5M2, bool VEC, bool TILE_SCALE, bool BOTH>
 __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
-    __shared__ float col_max[8][kBlock];
+    using P = typename Pair<T>::type;
+    constexpr int kPairs = sizeof(Vals<T>) / 4, kPer = 16 / kPairs;   // pairs of a lane's row, values in one
+    __shared__ P col_max[8][kBlock / kPer];
+    __shared__ __align__(16) float col_inv[kBlock];
     __shared__ uint8_t row_s[kBlock];
     __shared__ float tile_max[8];
     __shared__ __align__(16) uint32_t turn[BOTH ? kBlock * 32 : 4];
@@ -162,24 +232,19 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
     const int rb = int(blockIdx.x / col_blocks), cb = int(blockIdx.x % col_blocks);
     const int r0 = rb * kBlock, c0 = cb * kBlock, rw = warp * 16 + sub * 4;
     const T* x = j.x + blockIdx.y * j.batch_stride;
-    float v[4][16];
+    Vals<T> v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = r0 + rw + i;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[i][k] = 0.f;
+        v[i] = {};
         if (r < j.rows) {
-            load8<T, VEC>(x + r * j.ld, c0 + oct * 8, j.cols, v[i]);
-            load8<T, VEC>(x + r * j.ld, c0 + 64 + oct * 8, j.cols, v[i] + 8);
+            load8<T, VEC>(v[i], 0, x + r * j.ld, c0 + oct * 8, j.cols);
+            load8<T, VEC>(v[i], 1, x + r * j.ld, c0 + 64 + oct * 8, j.cols);
         }
     }
     float amax[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        amax[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) amax[i] = fmaxf(amax[i], fabsf(v[i][k]));
-    }
+    for (int i = 0; i < 4; ++i) amax[i] = finite_max(v[i]);
     if constexpr (TILE_SCALE) {
         float m = fmaxf(fmaxf(amax[0], amax[1]), fmaxf(amax[2], amax[3]));
 #pragma unroll
@@ -194,11 +259,11 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
         }
         if constexpr (BOTH) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                float m = fmaxf(fmaxf(fabsf(v[0][k]), fabsf(v[1][k])), fmaxf(fabsf(v[2][k]), fabsf(v[3][k])));
-                m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
-                m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-                if (sub == 0) col_max[warp][(k >> 3) * 64 + oct * 8 + (k & 7)] = m;
+            for (int k = 0; k < kPairs; ++k) {
+                P m = larger<T>(larger<T>(v[0].w[k], v[1].w[k]), larger<T>(v[2].w[k], v[3].w[k]));
+                m = larger<T>(m, __shfl_xor_sync(~0u, m, 8));
+                m = larger<T>(m, __shfl_xor_sync(~0u, m, 16));
+                if (sub == 0) col_max[warp][(k / (kPairs / 2)) * (64 / kPer) + oct * (8 / kPer) + k % (kPairs / 2)] = m;
             }
         }
     }
@@ -213,8 +278,19 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
             j.scales[(size_t(blockIdx.y) * col_blocks + cb) * row_blocks + rb] = uint8_t(tile_s);
             if (BOTH) j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * col_blocks + cb] = uint8_t(tile_s);
         }
-    } else if (threadIdx.x < kBlock && r0 + threadIdx.x < j.rows) {
-        j.scales[(size_t(blockIdx.y) * col_blocks + cb) * j.rows + r0 + threadIdx.x] = row_s[threadIdx.x];
+    } else {
+        if (threadIdx.x < kBlock) {
+            if (r0 + int(threadIdx.x) < j.rows)
+                j.scales[(size_t(blockIdx.y) * col_blocks + cb) * j.rows + r0 + threadIdx.x] = row_s[threadIdx.x];
+        } else if constexpr (BOTH) {
+            const int c = threadIdx.x - kBlock;
+            P m = col_max[0][c / kPer];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) m = larger<T>(m, col_max[w][c / kPer]);
+            const uint32_t s = scale_of<E5M2>(kPer == 2 && (c & 1) ? second_of<T>(m) : first_of<T>(larger<T>(m, m)));
+            col_inv[c] = inverse_scale(s);
+            if (c0 + c < j.cols) j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * j.cols + c0 + c] = uint8_t(s);
+        }
     }
     uint8_t* codes = j.codes + blockIdx.y * j.codes_batch;
 #pragma unroll
@@ -224,28 +300,24 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int c = c0 + h * 64 + oct * 8;
-            const float* p = v[i] + 8 * h;
-            const uint2 q = make_uint2(codes4<E5M2>(p[0] * inv, p[1] * inv, p[2] * inv, p[3] * inv),
-                                       codes4<E5M2>(p[4] * inv, p[5] * inv, p[6] * inv, p[7] * inv));
+            auto at = [&](int k) { return v[i].get(8 * h + k) * inv; };
+            const uint2 q = make_uint2(codes4<E5M2>(at(0), at(1), at(2), at(3)), codes4<E5M2>(at(4), at(5), at(6), at(7)));
             if (r < j.rows && c < j.cols) *reinterpret_cast<uint2*>(codes + r * j.codes_ld + c) = q;
         }
     }
     if constexpr (BOTH) {
+        if constexpr (!TILE_SCALE) __syncthreads();   // col_inv
+        const float tile_inv = inverse_scale(tile_s);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const int c = (k >> 3) * 64 + oct * 8 + (k & 7);
-            uint32_t s = tile_s;
-            if constexpr (!TILE_SCALE) {
-                float m = col_max[0][c];
+        for (int h = 0; h < 2; ++h) {
+            float inv[8];
 #pragma unroll
-                for (int w = 1; w < 8; ++w) m = fmaxf(m, col_max[w][c]);
-                s = scale_of<E5M2>(m);
-                if (warp == 0 && sub == 0 && c0 + c < j.cols)
-                    j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * j.cols + c0 + c] = uint8_t(s);
-            }
-            const float inv = inverse_scale(s);
-            turn[c * 32 + ((rw >> 2) ^ (((c >> 3) & 7) << 2))] =
-                codes4<E5M2>(v[0][k] * inv, v[1][k] * inv, v[2][k] * inv, v[3][k] * inv);
+            for (int k = 0; k < 8; ++k) inv[k] = TILE_SCALE ? tile_inv : col_inv[h * 64 + oct * 8 + k];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                turn[(h * 64 + oct * 8 + k) * 32 + ((rw >> 2) ^ (oct << 2))] =
+                    codes4<E5M2>(v[0].get(8 * h + k) * inv[k], v[1].get(8 * h + k) * inv[k], v[2].get(8 * h + k) * inv[k],
+                                 v[3].get(8 * h + k) * inv[k]);
         }
         __syncthreads();
         uint8_t* t_codes = j.t_codes + blockIdx.y * j.t_batch;
@@ -332,7 +404,7 @@ void quantize_as(const MatrixRef& x, int block_rows, int code_type, void* codes,
                  cudaStream_t stream) {
     QuantJob<T> j{static_cast<const T*>(x.ptr), x.rows, x.cols, x.ld, x.batch_stride, static_cast<uint8_t*>(codes), ld,
                   batch_stride, scales, static_cast<uint8_t*>(t_codes), t_ld, t_batch, t_scales, 0};
-    constexpr int n = Vec<T>::n;
+    constexpr int n = Vals<T>::n;
     const bool vec = aligned(x.ptr, 16) && x.ld % n == 0 && x.cols % n == 0 && (x.batch == 1 || x.batch_stride % n == 0);
     if (code_type == kE5M2) {
         if (vec) launch_quant<T, true, true>(j, block_rows, x.batch, stream);

@@ -1,17 +1,21 @@
 // Matrix products on tcgen05, D[p][q] = sum_k A[p][k] B[q][k]: block-scaled FP8 or 16-bit operands,
 // dense, with the rows of one side grouped by expert, or with the contraction grouped by expert.
 //
-// One persistent, warp-specialised kernel.  A CTA takes output tiles of 128 x BN; per step of 128
-// bytes of the contraction, warp 0 copies the operands' tiles by TMA into a ring of 128-byte
-// swizzled stages, warp 1 issues four MMAs into FP32 accumulators in TMEM, warps 4..7 write the
-// finished tile out (TMEM lane = row of A).  Warp 2 serves the form of the product:
+// One persistent, warp-specialised kernel.  A tile is 128 x BN of the output, taken by one CTA, or
+// 256 x BN, taken by a pair of CTAs (cta_group::2): each holds 128 rows of A and of the accumulator and
+// half of B's rows, so that a pair reads and stages B once.  Per step of 128 bytes of the contraction,
+// warp 0 copies the operands' tiles by TMA into a ring of 128-byte swizzled stages, warp 1 (of the
+// pair's first CTA) issues four MMAs into FP32 accumulators in TMEM, warps 4..11 write the finished tile
+// out (TMEM lane = row of A).  Warp 2 serves the form of the product:
 //   * FP8: kind::mxf8f6f4.block_scale applies a power-of-two scale per row and 32 values inside the
 //     tensor core; a block of 128 is four such steps with the same scale.  The scales of 128 rows and
 //     four blocks form the 512-byte atom that tcgen05.cp spreads over the TMEM lanes (row r, block j at
-//     (r % 32) * 16 + (r / 32) * 4 + j); warp 2 gathers it from global memory once per four steps and
-//     the MMA names the byte j.  The accumulator never leaves TMEM before the tile is done.
+//     (r % 32) * 16 + (r / 32) * 4 + j); warp 2 gathers it from global memory once per four steps, one
+//     atom ahead, and the MMA names the byte j.  The accumulator never leaves TMEM before the tile is done.
 //   * contraction grouped by expert: a group's last step may reach into the next group's rows; warp 2
 //     zeroes those rows of both operands in shared memory before the MMA sees the stage.
+// The writers take a whole tile into registers and hand TMEM back before they store, because 256 columns
+// leave no room for a second accumulator beside the scales.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -31,10 +35,14 @@ using namespace tc;
 
 constexpr int kBM = 128;              // rows of A per tile: the TMEM lanes
 constexpr int kStepBytes = 128;       // contraction bytes per step: one swizzle row
-constexpr int kThreads = 256;
-constexpr int kRing = 200 * 1024;     // shared memory of the operand ring
+constexpr int kWriters = 8;           // warps that write tiles out
+constexpr int kThreads = 128 + 32 * kWriters;
+constexpr int kRing = 201 * 1024 + 512;   // shared memory of the operand ring
+constexpr int kTurn = 2048;           // shared memory of a writer: 32 rows of 64 bytes
 constexpr int kErrWait = 1;           // error code: a wait ran out
 constexpr int kAtom = 512;            // scales of 128 rows and four block columns
+constexpr int kGroupSteps = 4;        // steps that share an atom
+constexpr int kScaleSlots = 4;        // groups of steps whose scales are staged
 
 // What is grouped by the offsets.
 enum Grouping { kDense = 0, kRowsA = 1, kRowsB = 2, kContraction = 3 };
@@ -59,29 +67,34 @@ struct ProdJob {
     int split, steps_per_split;  // the contraction in `split` parts:
     int cluster;                 //   of the CTAs of a cluster, joined in its shared memory (split > 1), or (1)
     long long split_stride;      //   each to its own partial output
+    int out_vec;                 // rows of out start on 16-byte boundaries
     int zero_outside, zero_rows;
     int after_quantize;          // starts while the quantiser of its float operand still runs; the other
                                  // operand and the offsets are older
 };
 
-template <bool FP8, int BN>
+template <bool FP8, int BN, int CTAS>
 struct Shape {
-    static constexpr int kATile = kBM * kStepBytes, kBTile = BN * kStepBytes;
-    static constexpr int kAtomsB = (BN + 127) / 128;
+    static constexpr int kBRows = BN / CTAS;                 // rows of B that a CTA stages
+    static constexpr int kATile = kBM * kStepBytes, kBTile = kBRows * kStepBytes;
+    static constexpr int kAtomsB = (BN + 127) / 128;         // every CTA needs the scales of all BN
     static constexpr int kScaleBytes = FP8 ? kAtom * (1 + kAtomsB) : 0;
     static constexpr int kStage = kATile + kBTile;
-    static constexpr int kStages = kRing / (kStage + kScaleBytes);
-    // Accumulators of two tiles where TMEM's 512 columns hold them beside the scales.
-    static constexpr int kAccs = 2 * BN + (FP8 ? 64 : 0) <= 512 ? 2 : 1;
-    static constexpr int kScaleCol = kAccs * BN;
-    // Each stage has its own scale columns: they are written again only after the MMAs that read them
-    // have been committed with the stage.
+    static constexpr int kStages = (kRing - kScaleSlots * kScaleBytes) / kStage;
+    // Each slot has its own scale columns too: they are written again only after the MMAs that read them
+    // have been committed with the slot.
     static constexpr int kScaleCols = FP8 ? 4 * (1 + kAtomsB) : 0;
-    static constexpr int kColsUsed = kAccs * BN + kStages * kScaleCols;
+    // Accumulators of two tiles where TMEM's 512 columns hold them beside the scales.
+    static constexpr int kAccs = 2 * BN + kScaleSlots * kScaleCols <= 512 ? 2 : 1;
+    static constexpr int kColsUsed = kAccs * BN + kScaleSlots * kScaleCols;
     static constexpr int kCols = kColsUsed <= 32 ? 32 : kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128
                                  : kColsUsed <= 256 ? 256 : 512;
-    static constexpr int kBars = 3 * kStages + 2 * kAccs + 1;
-    static constexpr size_t kSmem = 1024 + size_t(kStages) * (kStage + kScaleBytes) + kBars * 8 + 16;
+    // Writers: one warp per 32 lanes, two where each then has at least 32 columns.
+    static constexpr int kHalves = BN >= 64 ? 2 : 1, kWide = BN / kHalves;
+    static constexpr int kBars = 3 * kStages + 2 * kScaleSlots + 2 * kAccs + 1;
+    static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kScaleSlots * kScaleBytes + kWriters * kTurn + kBars * 8;
+    // Behind it the bias of each writer's columns (dense) or the groups' bounds and tiles.
+    static constexpr size_t kBias = kWriters * kWide * sizeof(float);
 };
 
 // ---- PTX ---------------------------------------------------------------------------------------
@@ -98,22 +111,79 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
+template <int CTAS>
 __device__ __forceinline__ void mma_block_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
                                                  uint32_t sfb, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
-        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
 }
-// A 512-byte scale atom to four TMEM columns, repeated in the lanes of all four warps.
+template <int CTAS>
+__device__ __forceinline__ void mma_half(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    if constexpr (CTAS == 1)
+        mma_f16(d, a, b, idesc, acc);
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+            :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// A 512-byte scale atom to four TMEM columns, repeated in the lanes of all four warps; with a pair, in
+// each CTA from its own shared memory.
+template <int CTAS>
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t saddr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(sdesc(saddr, 128, 128))
-                 : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(sdesc(saddr, 128, 128))
+                     : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(sdesc(saddr, 128, 128))
+                     : "memory");
 }
-__device__ __forceinline__ void tma_3d(uint32_t smem, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        :: "r"(smem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar)) : "memory");
+// Arrive on `bar`, at the same place in every CTA of the tile, when the MMAs issued so far are done.
+template <int CTAS>
+__device__ __forceinline__ void commit_all(uint64_t* bar) {
+    if constexpr (CTAS == 1)
+        commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+            :: "r"(smem_addr(bar)), "h"(uint16_t(3)) : "memory");
+}
+// TMEM columns by one full warp (of each CTA of the tile).
+template <int CTAS>
+__device__ __forceinline__ void columns_alloc(uint32_t* slot, uint32_t n) {
+    if constexpr (CTAS == 1) {
+        tmem_alloc(slot, n);
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_addr(slot)), "r"(n) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void columns_free(uint32_t base, uint32_t n) {
+    if constexpr (CTAS == 1) tmem_free(base, n);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(base), "r"(n) : "memory");
+}
+// Tile load into this CTA's shared memory; `bar` is a cluster address with CTAS == 2.
+template <int CTAS>
+__device__ __forceinline__ void tma_3d(uint32_t smem, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+            :: "r"(smem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+            " [%0], [%1, {%2, %3, %4}], [%5];"
+            :: "r"(smem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
 
 // Thread block clusters: rank, barrier and another CTA's shared memory.
@@ -132,8 +202,42 @@ __device__ __forceinline__ float peer_float(uint32_t saddr, uint32_t rank) {
     return v;
 }
 
+__device__ __forceinline__ uint32_t address_in(uint32_t saddr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    return a;
+}
+// Arrive on a barrier of the tile's first CTA.
+template <int CTAS>
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    if constexpr (CTAS == 1)
+        mbar_arrive(bar);
+    else
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+                     :: "r"(address_in(smem_addr(bar), 0)) : "memory");
+}
+
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
     return mbar_wait_bounded(bar, parity, &g_product_error, kErrWait);
+}
+// As wait, for a phase that threads of the other CTA complete as well.  (An acquire on the barrier: a
+// fence of cluster scope here doubled the time of every step.)
+template <int CTAS>
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
+    if constexpr (CTAS == 1) return wait(bar, parity);
+    const long long t0 = clock64();
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+        if (done) return true;
+        if (clock64() - t0 > 4000000000LL) {
+            atomicCAS(&g_product_error, 0, kErrWait);
+            return false;
+        }
+    }
 }
 
 // ---- tiles -------------------------------------------------------------------------------------
@@ -153,17 +257,17 @@ struct Groups {
     const int* cum;      // [groups + 1] row tiles before each group
 };
 
-template <int BN>
+template <int BM, int BN>
 __device__ __forceinline__ int tile_count(const ProdJob& j, const Groups& g) {
-    const int tp = (j.P + kBM - 1) / kBM, tq = (j.Q + BN - 1) / BN;
+    const int tp = (j.P + BM - 1) / BM, tq = (j.Q + BN - 1) / BN;
     if (j.grouping == kDense) return tp * tq * j.split;
     if (j.grouping == kContraction) return tp * tq * j.groups;
     return g.cum[j.groups] * (j.grouping == kRowsA ? tq : tp);
 }
 
-template <int BN>
+template <int BM, int BN>
 __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t, int step) {
-    const int tp = (j.P + kBM - 1) / kBM, tq = (j.Q + BN - 1) / BN;
+    const int tp = (j.P + BM - 1) / BM, tq = (j.Q + BN - 1) / BN;
     Tile x{0, 0, 0, j.P, j.Q, 0, j.K, 0};
     if (j.grouping == kDense) {
         // Bands of 16 row tiles, walked column by column: CTAs that run at the same time share both
@@ -171,14 +275,14 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
         x.part = t / (tp * tq);
         t -= x.part * tp * tq;
         const int band = t / (16 * tq), first = band * 16, high = min(16, tp - first), in = t - band * 16 * tq;
-        x.p0 = (first + in % high) * kBM;
+        x.p0 = (first + in % high) * BM;
         x.q0 = (in / high) * BN;
         x.k0 = x.part * j.steps_per_split * step;
         x.k1 = min(j.K, x.k0 + j.steps_per_split * step);
     } else if (j.grouping == kContraction) {
         x.e = t / (tp * tq);
         t -= x.e * tp * tq;
-        x.p0 = (t % tp) * kBM;
+        x.p0 = (t % tp) * BM;
         x.q0 = (t / tp) * BN;
         x.k0 = g.bound[x.e];
         x.k1 = g.bound[x.e + 1];
@@ -193,13 +297,13 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
         x.e = lo;
         const int own = g.cum[lo + 1] - g.cum[lo], in = t - g.cum[lo] * other;
         if (j.grouping == kRowsA) {
-            x.p0 = g.bound[lo] + (in % own) * kBM;
+            x.p0 = g.bound[lo] + (in % own) * BM;
             x.p1 = g.bound[lo + 1];
             x.q0 = (in / own) * BN;
         } else {
             x.q0 = g.bound[lo] + (in % own) * BN;
             x.q1 = g.bound[lo + 1];
-            x.p0 = (in / own) * kBM;
+            x.p0 = (in / own) * BM;
         }
     }
     return x;
@@ -207,22 +311,66 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
 
 // ---- scales ------------------------------------------------------------------------------------
 
-// This lane's 16 bytes of the atom of rows row0 .. row0 + 127 and block columns kb .. kb + 3: word w
-// holds row 32 w + lane.  Rows past the end repeat the last one, block columns past the end are
-// not used by any MMA.
-__device__ __forceinline__ uint4 gather_scales(const ScaleRef& s, int e, int row0, int rows, int kb, int blocks) {
-    const uint8_t* base = s.ptr + e * s.batch_stride;
+// How the scales of an operand are read.
+enum ScaleWay { kPerBlock, kPerRow, kPerRowWords };
+
+// What this lane reads for the atom of rows row0 .. row0 + 127 and block columns kb .. kb + 3, all loads
+// at once and nothing made of them yet, so that they are in flight while the previous atom is waited for.
+// Rows past the end repeat earlier ones, block columns past the end the last one; neither is used.
+struct RawScales {
+    uint32_t v[16];
+};
+__device__ __forceinline__ void load_scales(RawScales& r, const ScaleRef& s, ScaleWay way, int e, int row0, int rows,
+                                            int kb, int blocks) {
     const int lane = threadIdx.x & 31;
-    uint32_t w[4];
+    const uint8_t* col[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = min(row0 + 32 * i + lane, rows - 1) >> s.shift;
-        w[i] = 0;
+    for (int b = 0; b < 4; ++b) col[b] = s.ptr + e * s.batch_stride + (long long)min(kb + b, blocks - 1) * s.ld;
+    if (way == kPerBlock) {
+        // A tile of such an operand starts on a block of 128 rows or in its middle and does not leave it.
+        const int at = min(row0, rows - 1) >> s.shift;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) r.v[b] = __ldg(col[b] + at);
+    } else if (way == kPerRowWords) {
+        const int at = min(row0 + 4 * lane, rows - 4);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) r.v[b] = __ldg(reinterpret_cast<const uint32_t*>(col[b] + at));
+    } else {
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-            w[i] |= uint32_t(__ldg(base + (long long)min(kb + b, blocks - 1) * s.ld + at)) << (8 * b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.v[4 * b + i] = __ldg(col[b] + min(row0 + 32 * i + lane, rows - 1));
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The atom into shared memory: row r, block j at (r % 32) * 16 + (r / 32) * 4 + j.
+__device__ __forceinline__ void store_scales(const RawScales& r, ScaleWay way, uint8_t* atom) {
+    const int lane = threadIdx.x & 31;
+    if (way == kPerBlock) {
+        const uint32_t w = r.v[0] | r.v[1] << 8 | r.v[2] << 16 | r.v[3] << 24;
+        reinterpret_cast<uint4*>(atom)[lane] = make_uint4(w, w, w, w);
+    } else if (way == kPerRowWords) {
+        // four rows of four blocks: a 4 x 4 byte transpose
+        const uint32_t a = __byte_perm(r.v[0], r.v[1], 0x5140), b = __byte_perm(r.v[2], r.v[3], 0x5140);
+        const uint32_t c = __byte_perm(r.v[0], r.v[1], 0x7362), d = __byte_perm(r.v[2], r.v[3], 0x7362);
+        const uint32_t w[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x5410),
+                               __byte_perm(c, d, 0x7632)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 4 * lane + i;
+            *reinterpret_cast<uint32_t*>(atom + (row & 31) * 16 + (row >> 5) * 4) = w[i];
+        }
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = r.v[i] | r.v[4 + i] << 8 | r.v[8 + i] << 16 | r.v[12 + i] << 24;
+        reinterpret_cast<uint4*>(atom)[lane] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+// Words of four rows where every tile starts at a multiple of four rows and the columns are as aligned.
+__device__ __forceinline__ ScaleWay scale_way(const ScaleRef& s, int rows, bool ragged) {
+    if (s.shift) return kPerBlock;
+    return !ragged && rows >= 4 && s.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(s.ptr) & 3) == 0 &&
+                   s.batch_stride % 4 == 0 ? kPerRowWords : kPerRow;
 }
 
 // ---- epilogue ----------------------------------------------------------------------------------
@@ -237,93 +385,124 @@ __device__ __forceinline__ void store_elem(void* p, int type, long long i, float
     else if (type == kF16) static_cast<__half*>(p)[i] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
-__device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
-    if (type == kF16) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-// `n` of up to W consecutive values at element index i; whole 16-byte stores where they fit.
+template <typename T> __device__ __forceinline__ T rounded(float v);
+template <> __device__ __forceinline__ float rounded<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Columns of this thread's lane into registers, without the wait.
 template <int W>
-__device__ __forceinline__ void store_run(void* p, int type, long long i, const float* v, int n) {
-    if (n >= W) {
-        if (type == kF32) {
-            float* q = static_cast<float*>(p) + i;
-            if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
+    if constexpr (W == 16) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr));
+    } else {
 #pragma unroll
-                for (int c = 0; c < W; c += 4)
-                    *reinterpret_cast<float4*>(q + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-                return;
-            }
-        } else {
-            uint16_t* q = static_cast<uint16_t*>(p) + i;
-            if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
-#pragma unroll
-                for (int c = 0; c < W; c += 8)
-                    *reinterpret_cast<uint4*>(q + c) =
-                        make_uint4(pack2(type, v[c], v[c + 1]), pack2(type, v[c + 2], v[c + 3]),
-                                   pack2(type, v[c + 4], v[c + 5]), pack2(type, v[c + 6], v[c + 7]));
-                return;
-            }
-        }
+        for (int c = 0; c < W; c += 32) tmem_ld_x32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
     }
-#pragma unroll
-    for (int c = 0; c < W; ++c)
-        if (c < n) store_elem(p, type, i + c, v[c]);
 }
 
-template <int W>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[W]);
-template <>
-__device__ __forceinline__ void tmem_load<32>(uint32_t taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
-template <>
-__device__ __forceinline__ void tmem_load<16>(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// The warp's 32 rows by W columns to out[p][q]: runs of 64 bytes turn through shared memory, so that
+// four lanes store one row's run.  Its 16-byte pieces are exclusive-or'ed with the row pair: no bank
+// conflicts either way.  Where rows do not start on 16-byte boundaries, or columns end, elements are
+// stored one by one, neighbouring lanes at neighbouring addresses.
+template <typename T, int W>
+__device__ __forceinline__ void write_rows(const ProdJob& j, const uint32_t* v, const float* bias, uint8_t* turn,
+                                           long long base, int p0, int p1, int q0, int q1) {
+    constexpr int kRun = 64 / sizeof(T) < W ? 64 / sizeof(T) : W, kPieces = kRun * sizeof(T) / 16;
+    const int lane = threadIdx.x & 31;
+    T* out = static_cast<T*>(j.out) + base;
+    const bool whole = j.out_vec && base % (16 / sizeof(T)) == 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    for (int c = 0; c < W; c += kRun) {
+        if (q0 + c >= q1) break;
+        uint4 piece[kPieces];
+        T* e = reinterpret_cast<T*>(piece);
+#pragma unroll
+        for (int i = 0; i < kRun; ++i)
+            e[i] = rounded<T>(__uint_as_float(v[c + i]) + (j.bias ? bias[c + i] : 0.f));
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            *reinterpret_cast<uint4*>(turn + lane * 64 + ((i ^ ((lane >> 1) & (kPieces - 1))) << 4)) = piece[i];
+        __syncwarp();
+        if (whole && q0 + c + kRun <= q1) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int at = i * 32 + lane, r = at / kPieces, k = at % kPieces;
+                const uint4 q = *reinterpret_cast<const uint4*>(turn + r * 64 + ((k ^ ((r >> 1) & (kPieces - 1))) << 4));
+                if (p0 + r < p1)
+                    *reinterpret_cast<uint4*>(out + (p0 + r) * j.out_ld + q0 + c + k * (16 / sizeof(T))) = q;
+            }
+        } else {
+            for (int at = lane; at < 32 * kRun; at += 32) {
+                const int r = at / kRun, k = at % kRun, b = k * int(sizeof(T));
+                if (p0 + r < p1 && q0 + c + k < q1)
+                    out[(p0 + r) * j.out_ld + q0 + c + k] = *reinterpret_cast<const T*>(
+                        turn + r * 64 + (((b >> 4) ^ ((r >> 1) & (kPieces - 1))) << 4) + (b & 15));
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// The same to out[q][p]: a column's 32 values lie together.
+template <typename T, int W>
+__device__ __forceinline__ void write_columns(const ProdJob& j, const uint32_t* v, long long base, int p, int p1, int q0,
+                                              int q1) {
+    T* out = static_cast<T*>(j.out) + base;
+    if (p >= p1) return;
+    const float b = j.bias ? load_elem(j.bias, j.bias_type, p) : 0.f;
+#pragma unroll
+    for (int c = 0; c < W; ++c)
+        if (q0 + c < q1) out[(q0 + c) * j.out_ld + p] = rounded<T>(__uint_as_float(v[c]) + b);
 }
 
 // ---- the kernel --------------------------------------------------------------------------------
 
-template <bool FP8, int BN>
+template <bool FP8, int BN, int CTAS>
 __global__ void __launch_bounds__(kThreads, 1)
 k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
           const __grid_constant__ ProdJob j) {
-    using S = Shape<FP8, BN>;
+    using S = Shape<FP8, BN, CTAS>;
     constexpr int kStep = FP8 ? kStepBytes : kStepBytes / 2;   // contraction values per step
+    constexpr int BM = kBM * CTAS;
     extern __shared__ uint8_t raw[];
     __shared__ uint32_t tmem_slot;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t* scales = ring + S::kStages * S::kStage;
-    uint64_t* full = reinterpret_cast<uint64_t*>(scales + S::kStages * S::kScaleBytes);
+    uint8_t* turns = scales + kScaleSlots * S::kScaleBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(turns + kWriters * kTurn);
     uint64_t* empty = full + S::kStages;
     uint64_t* fixed = empty + S::kStages;
-    uint64_t* acc_full = fixed + S::kStages;
+    uint64_t* scales_full = fixed + S::kStages;
+    uint64_t* scales_empty = scales_full + kScaleSlots;
+    uint64_t* acc_full = scales_empty + kScaleSlots;
     uint64_t* acc_empty = acc_full + S::kAccs;
     uint64_t* drain = acc_empty + S::kAccs;
     int* bound = reinterpret_cast<int*>(drain + 1);
     int* cum = bound + j.groups + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // A pair takes a tile; otherwise a cluster takes one tile, each of its CTAs a part of the contraction.
+    const int rank = CTAS == 2 || j.cluster > 1 ? int(cluster_rank()) : 0;
 
-    if (warp == 3) tmem_alloc(&tmem_slot, S::kCols);
+    if (warp == 3) columns_alloc<CTAS>(&tmem_slot, S::kCols);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(full + i, FP8 ? 2 : 1);
+            mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
-            mbar_init(fixed + i, 1);
+            mbar_init(fixed + i, CTAS);
+        }
+        for (int i = 0; i < kScaleSlots; ++i) {
+            mbar_init(scales_full + i, CTAS);
+            mbar_init(scales_empty + i, 1);
         }
         for (int i = 0; i < S::kAccs; ++i) {
             mbar_init(acc_full + i, 1);
-            mbar_init(acc_empty + i, 128);
+            mbar_init(acc_empty + i, 4 * S::kHalves * CTAS);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -331,7 +510,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     const Groups g{bound, cum};
     if (j.grouping != kDense) {
         const int rows = j.grouping == kContraction ? j.K : j.grouping == kRowsA ? j.P : j.Q;
-        const int high = j.grouping == kRowsB ? BN : kBM;
+        const int high = j.grouping == kRowsB ? BN : BM;
         for (int i = threadIdx.x; i <= j.groups; i += kThreads) bound[i] = min(max(j.off[i], 0), rows);
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -346,13 +525,15 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     }
     fence_before_sync();
     __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
-    const int tiles = tile_count<BN>(j, g);
-    // A cluster takes one tile, each of its CTAs a part of the contraction.
-    const int rank = j.cluster > 1 ? int(cluster_rank()) : 0;
-    const int first_tile = j.cluster > 1 ? rank * (tiles / j.split) + int(blockIdx.x) / j.cluster : int(blockIdx.x);
-    const int stride = j.cluster > 1 ? tiles : int(gridDim.x);
+    const int tiles = tile_count<BM, BN>(j, g);
+    const int first_tile = CTAS == 2       ? int(blockIdx.x) / 2
+                           : j.cluster > 1 ? rank * (tiles / j.split) + int(blockIdx.x) / j.cluster
+                                           : int(blockIdx.x);
+    const int stride = CTAS == 2 ? int(gridDim.x) / 2 : j.cluster > 1 ? tiles : int(gridDim.x);
+    const int a_off = CTAS == 2 ? rank * kBM : 0, b_off = CTAS == 2 ? rank * S::kBRows : 0;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -362,192 +543,240 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             long long issued = 0;
             if (j.after_quantize) grid_dep_wait();
             for (int t = first_tile; ok && t < tiles; t += stride) {
-                const Tile x = tile_at<BN>(j, g, t, kStep);
+                const Tile x = tile_at<BM, BN>(j, g, t, kStep);
                 const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
                 for (int k = x.k0; k < x.k1; k += kStep) {
                     if (!(ok = wait(empty + stage, phase ^ 1))) break;
                     const uint32_t a = smem_addr(ring + stage * S::kStage), b = a + S::kATile;
-                    mbar_arrive_expect_tx(full + stage, S::kStage);
+                    const uint32_t local = smem_addr(full + stage);
+                    // A pair's copies all count on its first CTA's barrier; where rows have to be zeroed first,
+                    // each CTA's on its own.
+                    const bool own = CTAS == 1 || (j.grouping == kContraction && k + kStep > x.k1);
+                    const uint32_t bar = CTAS == 1 ? local : address_in(local, own ? rank : 0);
+                    if (own || rank == 0) mbar_arrive_expect_tx(full + stage, own ? S::kStage : S::kStage * CTAS);
                     if (j.a_mn) {
-                        for (int c = 0; c < kBM / 64; ++c) tma_3d(a + c * 8192, &ma, x.p0 + c * 64, k, ea, full + stage);
+                        for (int c = 0; c < kBM / 64; ++c) tma_3d<CTAS>(a + c * 8192, &ma, x.p0 + a_off + c * 64, k, ea, bar);
                     } else {
-                        tma_3d(a, &ma, k, x.p0, ea, full + stage);
+                        tma_3d<CTAS>(a, &ma, k, x.p0 + a_off, ea, bar);
                     }
                     if (j.b_mn) {
-                        for (int c = 0; c < BN / 64; ++c) tma_3d(b + c * 8192, &mb, x.q0 + c * 64, k, eb, full + stage);
+                        for (int c = 0; c < S::kBRows / 64; ++c)
+                            tma_3d<CTAS>(b + c * 8192, &mb, x.q0 + b_off + c * 64, k, eb, bar);
                     } else {
-                        tma_3d(b, &mb, k, x.q0, eb, full + stage);
+                        tma_3d<CTAS>(b, &mb, k, x.q0 + b_off, eb, bar);
                     }
                     ++issued;
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
                 }
             }
-            // Every copy has landed before the CTA may end: those that no MMA waited for are waited for here.
-            for (int i = 0; !ok && i < S::kStages && issued - i > 0; ++i) {
+            // Every copy has landed before the CTA may end: those that no MMA waited for are waited for here
+            // (a pair's by its first CTA; the other one cannot end before it).
+            for (int i = 0; !ok && (CTAS == 1 || rank == 0) && i < S::kStages && issued - i > 0; ++i) {
                 const long long n = issued - 1 - i;
                 wait(full + n % S::kStages, uint32_t(n / S::kStages) & 1);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && (CTAS == 1 || rank == 0)) {
             int stage = 0, acc = 0;
-            uint32_t phase = 0, acc_phase = 0;
+            uint32_t phase = 0, acc_phase = 0, fixed_phase = 0, slot_phase = 0;
+            int slot = 0;
             bool ok = true;
-            uint64_t* ready = j.grouping == kContraction ? fixed : full;
             const uint32_t a_k = (j.a_mn ? 2048 : 32) >> 4, b_k = (j.b_mn ? 2048 : 32) >> 4;
             for (int t = first_tile; ok && t < tiles; t += stride) {
-                const Tile x = tile_at<BN>(j, g, t, kStep);
-                if (!(ok = wait(acc_empty + acc, acc_phase ^ 1))) break;
+                const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+                if (!(ok = wait_all<CTAS>(acc_empty + acc, acc_phase ^ 1))) break;
                 fence_after_sync();
                 const uint32_t d = tmem + acc * BN;
                 uint32_t first = 0;
                 int step = 0;
                 for (int k = x.k0; k < x.k1; k += kStep, ++step) {
-                    if (!(ok = wait(ready + stage, phase))) break;
+                    if (j.grouping == kContraction && k + kStep > x.k1) {
+                        if (!(ok = wait_all<CTAS>(fixed + stage, (fixed_phase >> stage) & 1))) break;
+                        fixed_phase ^= 1u << stage;
+                    } else {
+                        if (!(ok = wait(full + stage, phase))) break;
+                    }
+                    if (FP8 && step % kGroupSteps == 0 && !(ok = wait_all<CTAS>(scales_full + slot, slot_phase))) break;
                     fence_after_sync();
                     const uint32_t sa = smem_addr(ring + stage * S::kStage), sb = sa + S::kATile;
                     const uint64_t da = j.a_mn ? desc_mnmajor(sa) : desc_kmajor(sa);
                     const uint64_t db = j.b_mn ? desc_mnmajor(sb) : desc_kmajor(sb);
                     if constexpr (FP8) {
-                        const uint32_t sf = tmem + S::kScaleCol + stage * S::kScaleCols;
-                        const uint32_t src = smem_addr(scales + stage * S::kScaleBytes);
+                        const uint32_t sf = tmem + S::kAccs * BN + slot * S::kScaleCols, byte = step % kGroupSteps;
+                        if (byte == 0) {
+                            const uint32_t src = smem_addr(scales + slot * S::kScaleBytes);
 #pragma unroll
-                        for (int i = 0; i <= S::kAtomsB; ++i) scales_to_tmem(sf + 4 * i, src + i * kAtom);
-                        const uint32_t id = j.idesc | (uint32_t(step & 3) << 4) | (uint32_t(step & 3) << 29);
+                            for (int i = 0; i <= S::kAtomsB; ++i) scales_to_tmem<CTAS>(sf + 4 * i, src + i * kAtom);
+                        }
+                        const uint32_t id = j.idesc | (byte << 4) | (byte << 29);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            mma_block_scaled(d, da + i * 2, db + i * 2, id, sf, sf + 4, first);
+                            mma_block_scaled<CTAS>(d, da + i * 2, db + i * 2, id, sf, sf + 4, first);
                             first = 1;
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            mma_f16(d, da + i * a_k, db + i * b_k, j.idesc, first);
+                            mma_half<CTAS>(d, da + i * a_k, db + i * b_k, j.idesc, first);
                             first = 1;
                         }
                     }
-                    commit(empty + stage);
+                    commit_all<CTAS>(empty + stage);
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
+                    if (FP8 && (step % kGroupSteps == kGroupSteps - 1 || k + kStep >= x.k1)) {
+                        commit_all<CTAS>(scales_empty + slot);
+                        if (++slot == kScaleSlots) slot = 0, slot_phase ^= 1;
+                    }
                 }
-                commit(acc_full + acc);
+                commit_all<CTAS>(acc_full + acc);
                 if (++acc == S::kAccs) acc = 0, acc_phase ^= 1;
             }
             if (!ok) {   // let the MMAs in flight land before TMEM goes
-                commit(drain);
+                commit_all<CTAS>(drain);
                 wait(drain, 0);
             }
         }
     } else if (warp == 2) {
-        int stage = 0;
+        [[maybe_unused]] int stage = 0;
         uint32_t phase = 0;
-        bool ok = true;
+        [[maybe_unused]] bool ok = true;
         if constexpr (FP8) {
             if (j.after_quantize) grid_dep_wait();
             const int blocks = (j.K + kBlock - 1) / kBlock;
-            for (int t = first_tile; ok && t < tiles; t += stride) {
-                const Tile x = tile_at<BN>(j, g, t, kStep);
+            const ScaleWay way_a = scale_way(j.sa, j.a_rows, j.grouping == kRowsA);
+            const ScaleWay way_b = scale_way(j.sb, j.b_rows, j.grouping == kRowsB);
+            RawScales raw_a, raw_b[S::kAtomsB];
+            auto load = [&](const Tile& x, int k) {
                 const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
-                int step = 0;
-                uint4 s[1 + S::kAtomsB];
-                for (int k = x.k0; ok && k < x.k1; k += kStep, ++step) {
-                    if ((step & 3) == 0) {
-                        const int kb = k / kBlock;
-                        s[0] = gather_scales(j.sa, ea, x.p0, j.a_rows, kb, blocks);
+                load_scales(raw_a, j.sa, way_a, ea, x.p0 + a_off, j.a_rows, k / kBlock, blocks);
 #pragma unroll
-                        for (int i = 0; i < S::kAtomsB; ++i)
-                            s[1 + i] = gather_scales(j.sb, eb, x.q0 + 128 * i, j.b_rows, kb, blocks);
-                    }
-                    ok = wait(empty + stage, phase ^ 1);
-                    if (!ok) break;
-                    uint4* dst = reinterpret_cast<uint4*>(scales + stage * S::kScaleBytes);
-#pragma unroll
-                    for (int i = 0; i <= S::kAtomsB; ++i) dst[i * 32 + lane] = s[i];
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full + stage);
-                    if (++stage == S::kStages) stage = 0, phase ^= 1;
+                for (int i = 0; i < S::kAtomsB; ++i)
+                    load_scales(raw_b[i], j.sb, way_b, eb, x.q0 + 128 * i, j.b_rows, k / kBlock, blocks);
+            };
+            int t = first_tile, k = 0;
+            Tile x{};
+            // To the first step of a tile that has one.
+            auto settle = [&] {
+                while (t < tiles) {
+                    x = tile_at<BM, BN>(j, g, t, kStep);
+                    k = x.k0;
+                    if (x.k0 < x.k1) break;
+                    t += stride;
                 }
+            };
+            settle();
+            if (t < tiles) load(x, k);
+            int slot = 0;
+            for (bool more = t < tiles; more;) {
+                if (!wait(scales_empty + slot, phase ^ 1)) break;
+                uint8_t* dst = scales + slot * S::kScaleBytes;
+                store_scales(raw_a, way_a, dst);
+#pragma unroll
+                for (int i = 0; i < S::kAtomsB; ++i) store_scales(raw_b[i], way_b, dst + (1 + i) * kAtom);
+                fence_async_smem();
+                __syncwarp();
+                // (One release of cluster scope per group: one per step cost more than the step.)
+                if (lane == 0) arrive_first<CTAS>(scales_full + slot);
+                if (++slot == kScaleSlots) slot = 0, phase ^= 1;
+                k += kGroupSteps * kStep;
+                if (k >= x.k1) {
+                    t += stride;
+                    settle();
+                }
+                more = t < tiles;
+                if (more) load(x, k);
             }
         } else if (j.grouping == kContraction) {
+            uint32_t own_phase = 0;   // of the barriers of a pair's second CTA, which only these steps use
             for (int t = first_tile; ok && t < tiles; t += stride) {
-                const Tile x = tile_at<BN>(j, g, t, kStep);
+                const Tile x = tile_at<BM, BN>(j, g, t, kStep);
                 for (int k = x.k0; k < x.k1; k += kStep) {
-                    if (!(ok = wait(full + stage, phase))) break;
                     const int rows = x.k1 - k;
+                    // (A phase may be waited for only in turn: the first CTA's barriers see every step.)
+                    if (rank == 0 && !(ok = wait(full + stage, phase))) break;
                     if (rows < kStep) {
+                        if (rank == 1 && !(ok = wait(full + stage, (own_phase >> stage) & 1))) break;
+                        own_phase ^= 1u << stage;
                         uint8_t* base = ring + stage * S::kStage;
                         const int tail = (kStep - rows) * 8;   // 16-byte pieces per chunk
                         for (int i = lane; i < tail * (S::kStage / 8192); i += 32)
                             *reinterpret_cast<uint4*>(base + (i / tail) * 8192 + rows * 128 + (i % tail) * 16) =
                                 make_uint4(0, 0, 0, 0);
                         fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) arrive_first<CTAS>(fixed + stage);
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(fixed + stage);
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
                 }
             }
         }
-    } else if (warp >= 4) {
-        constexpr int W = BN < 32 ? BN : 32;
-        const int quad = warp & 3, row = quad * 32 + lane;
-        int acc = 0;
+    } else if (warp >= 4 && warp < 4 + 4 * S::kHalves) {
+        const int quad = warp & 3, half = (warp - 4) >> 2, col = half * S::kWide;
+        uint8_t* turn = turns + (warp - 4) * kTurn;
+        float* bias = reinterpret_cast<float*>(bound) + (warp - 4) * S::kWide;
+        int acc = 0, bias_q = -1;
         uint32_t acc_phase = 0;
         for (int t = first_tile; t < tiles; t += stride) {
-            const Tile x = tile_at<BN>(j, g, t, kStep);
+            const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+            if (j.bias && !j.swapped && bias_q != x.q0) {
+                for (int i = lane; i < S::kWide; i += 32)
+                    bias[i] = x.q0 + col + i < j.Q ? load_elem(j.bias, j.bias_type, x.q0 + col + i) : 0.f;
+                __syncwarp();
+                bias_q = x.q0;
+            }
             if (!wait(acc_full + acc, acc_phase)) break;
             fence_after_sync();
-            const bool any = x.k0 < x.k1;
-            const int p = x.p0 + row;
-            const long long base = x.part * j.split_stride + (j.grouping == kContraction ? x.e * j.out_batch : 0);
+            uint32_t v[S::kWide];
+            if (x.k0 < x.k1) {
+                tmem_load<S::kWide>(tmem + (uint32_t(quad * 32) << 16) + acc * BN + col, v);
+                tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < BN; c += W) {
-                float v[W];
-                if (any) {
-                    tmem_load<W>(tmem + (uint32_t(quad * 32) << 16) + acc * BN + c, v);
-                } else {
+                for (int i = 0; i < S::kWide; ++i) asm volatile("" : "+r"(v[i]));
+            } else {
 #pragma unroll
-                    for (int i = 0; i < W; ++i) v[i] = 0.f;
-                }
-                const int q = x.q0 + c, n = x.q1 - q;
-                if (j.cluster > 1) {
-                    // every MMA of this CTA is done with the ring: it takes the tile, column by column
-#pragma unroll
-                    for (int i = 0; i < W; ++i) reinterpret_cast<float*>(ring)[(c + i) * kBM + row] = v[i];
-                } else if (p < x.p1 && n > 0) {
-                    if (!j.swapped) {
-                        if (j.bias)
-#pragma unroll
-                            for (int i = 0; i < W; ++i)
-                                if (i < n) v[i] += load_elem(j.bias, j.bias_type, q + i);
-                        store_run<W>(j.out, j.out_type, base + p * j.out_ld + q, v, n);
-                    } else {
-                        const float b = j.bias ? load_elem(j.bias, j.bias_type, p) : 0.f;
-#pragma unroll
-                        for (int i = 0; i < W; ++i)
-                            if (i < n) store_elem(j.out, j.out_type, base + (q + i) * j.out_ld + p, v[i] + b);
-                    }
-                }
-                __syncwarp();
+                for (int i = 0; i < S::kWide; ++i) v[i] = 0;
             }
             fence_before_sync();
-            mbar_arrive(acc_empty + acc);
+            __syncwarp();
+            if (lane == 0) arrive_first<CTAS>(acc_empty + acc);
             if (++acc == S::kAccs) acc = 0, acc_phase ^= 1;
+
+            const int p0 = x.p0 + a_off + quad * 32, q0 = x.q0 + col;
+            const long long base = x.part * j.split_stride + (j.grouping == kContraction ? x.e * j.out_batch : 0);
+            if (CTAS == 1 && j.cluster > 1) {
+                // every MMA of this CTA is done with the ring: it takes the tile, column by column
+#pragma unroll
+                for (int i = 0; i < S::kWide; ++i)
+                    reinterpret_cast<uint32_t*>(ring)[(col + i) * kBM + quad * 32 + lane] = v[i];
+            } else if (j.swapped) {
+                if (j.out_type == kF32) write_columns<float, S::kWide>(j, v, base, p0 + lane, x.p1, q0, x.q1);
+                else if (j.out_type == kF16) write_columns<__half, S::kWide>(j, v, base, p0 + lane, x.p1, q0, x.q1);
+                else write_columns<__nv_bfloat16, S::kWide>(j, v, base, p0 + lane, x.p1, q0, x.q1);
+            } else {
+                if (j.out_type == kF32) write_rows<float, S::kWide>(j, v, bias, turn, base, p0, x.p1, q0, x.q1);
+                else if (j.out_type == kF16) write_rows<__half, S::kWide>(j, v, bias, turn, base, p0, x.p1, q0, x.q1);
+                else write_rows<__nv_bfloat16, S::kWide>(j, v, bias, turn, base, p0, x.p1, q0, x.q1);
+            }
+            __syncwarp();
         }
         if (j.zero_outside) {
             const int before = bound[0], after = bound[j.groups], skip = after - before;
             const long long todo = (long long)(j.zero_rows - skip) * j.cols;
-            for (long long i = (long long)blockIdx.x * 128 + (threadIdx.x - 128); i < todo; i += (long long)gridDim.x * 128) {
+            constexpr int kLanes = 128 * S::kHalves;
+            for (long long i = (long long)blockIdx.x * kLanes + (threadIdx.x - 128); i < todo;
+                 i += (long long)gridDim.x * kLanes) {
                 const int r = int(i / j.cols), at = r < before ? r : r + skip;
                 store_elem(j.out, j.out_type, at * j.out_ld + i % j.cols, 0.f);
             }
         }
     }
-    if (j.cluster > 1) {
+    if (CTAS == 1 && j.cluster > 1) {
         // The parts are added in their order, each CTA taking its share of the columns.
+        __syncwarp();
         cluster_sync();
-        if (warp >= 4 && first_tile < tiles) {
-            const Tile x = tile_at<BN>(j, g, first_tile, kStep);
+        if (warp >= 4 && warp < 8 && first_tile < tiles) {
+            const Tile x = tile_at<BM, BN>(j, g, first_tile, kStep);
             const int row = threadIdx.x - 128, p = x.p0 + row, share = BN / j.cluster;
             const float pb = j.bias && j.swapped && p < x.p1 ? load_elem(j.bias, j.bias_type, p) : 0.f;
             for (int c = rank * share; c < (rank + 1) * share; ++c) {
@@ -559,12 +788,13 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 else store_elem(j.out, j.out_type, p * j.out_ld + q, v + (j.bias ? load_elem(j.bias, j.bias_type, q) : 0.f));
             }
         }
-        cluster_sync();
     }
     fence_before_sync();
     __syncthreads();
+    // No CTA ends while another one may still read its shared memory or signal its barriers.
+    if (CTAS == 2 || j.cluster > 1) cluster_sync();
     fence_after_sync();
-    if (warp == 3) tmem_free(tmem, S::kCols);
+    if (warp == 3) columns_free<CTAS>(tmem, S::kCols);
 }
 
 // out = sum of the parts in order, plus the bias of the column.
@@ -640,24 +870,29 @@ int sm_count(int device) {
     return known[device];
 }
 
-template <bool FP8, int BN>
+template <bool FP8, int BN, int CTAS>
 void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long long tiles, int device,
             cudaStream_t stream) {
-    using S = Shape<FP8, BN>;
-    const size_t smem = S::kSmem + (j.grouping == kDense ? 0 : 2 * size_t(j.groups + 1) * sizeof(int));
+    using S = Shape<FP8, BN, CTAS>;
+    constexpr size_t most = S::kSmem + std::max(S::kBias, 2 * (kMaxGroups + 1) * sizeof(int));
+    static_assert(most <= 227 * 1024, "shared memory of a CTA");
+    const size_t smem = S::kSmem + (j.grouping == kDense ? S::kBias : 2 * size_t(j.groups + 1) * sizeof(int));
     static std::mutex mu;
     static bool ready[64] = {};
     const int sms = sm_count(device);
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[device]) {
-            AEISU_CUDA(cudaFuncSetAttribute(k_product<FP8, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            int(S::kSmem + 2 * (kMaxGroups + 1) * sizeof(int))));
+            AEISU_CUDA(cudaFuncSetAttribute(k_product<FP8, BN, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            int(most)));
             ready[device] = true;
         }
     }
+    const int cluster = CTAS == 2 ? 2 : j.cluster;
+    const long long ctas = CTAS == 2 ? 2 * std::min<long long>(tiles, sms / 2)
+                                     : j.cluster > 1 ? tiles : std::min<long long>(tiles, sms);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(j.cluster > 1 ? tiles : std::min<long long>(tiles, sms)), 1, 1);
+    cfg.gridDim = dim3(unsigned(ctas), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -665,46 +900,67 @@ void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long l
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = j.after_quantize;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = unsigned(j.cluster);
+    attr[1].val.clusterDim.x = unsigned(cluster);
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = j.cluster > 1 ? 2 : 1;
-    AEISU_CUDA(cudaLaunchKernelEx(&cfg, k_product<FP8, BN>, a, b, j));
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    AEISU_CUDA(cudaLaunchKernelEx(&cfg, k_product<FP8, BN, CTAS>, a, b, j));
 }
 
+// Tile of a product: columns, and CTAs that share it.
+struct TileShape {
+    int bn, ctas;
+    int rows() const { return kBM * ctas; }
+    int b_rows() const { return bn / ctas; }
+};
+
 template <bool FP8>
-void launch_width(int bn, const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long long tiles, int device,
+void launch_shape(TileShape s, const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long long tiles, int device,
                   cudaStream_t stream) {
-    switch (bn) {
-        case 16: return launch<FP8, 16>(a, b, j, tiles, device, stream);
-        case 32: return launch<FP8, 32>(a, b, j, tiles, device, stream);
-        case 64: return launch<FP8, 64>(a, b, j, tiles, device, stream);
-        case 128: return launch<FP8, 128>(a, b, j, tiles, device, stream);
-        default: return launch<FP8, 256>(a, b, j, tiles, device, stream);
+    if (s.ctas == 2) {
+        if (s.bn == 256) return launch<FP8, 256, 2>(a, b, j, tiles, device, stream);
+        return launch<FP8, 128, 2>(a, b, j, tiles, device, stream);
+    }
+    switch (s.bn) {
+        case 16: return launch<FP8, 16, 1>(a, b, j, tiles, device, stream);
+        case 32: return launch<FP8, 32, 1>(a, b, j, tiles, device, stream);
+        case 64: return launch<FP8, 64, 1>(a, b, j, tiles, device, stream);
+        default: return launch<FP8, 128, 1>(a, b, j, tiles, device, stream);
     }
 }
 
-uint32_t instruction(const MatrixRef& a, const MatrixRef& b, int bn) {
-    const uint32_t size = (uint32_t(bn >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// The tile for P x Q outputs, `count` of them: the one with the shortest time by waves of tiles over the
+// SMs.  A step's time goes by the operand bytes a CTA stages, A's 128 rows and its share of B's.
+TileShape choose_tile(long long row_tiles_of_128, int q, long long count, bool pairs, int least, int sms) {
+    TileShape best{least, 1};
+    double time = 0;
+    for (const TileShape s : {TileShape{16, 1}, TileShape{32, 1}, TileShape{64, 1}, TileShape{128, 1}, TileShape{128, 2},
+                              TileShape{256, 2}}) {
+        if (s.bn < least || (s.ctas == 2 && !pairs)) continue;
+        const long long tiles = ceil_div(row_tiles_of_128, s.ctas) * ceil_div(q, s.bn) * count;
+        const double t = double(ceil_div(tiles, sms / s.ctas)) * (kBM + s.b_rows());
+        if (time == 0 || t < time) best = s, time = t;
+    }
+    return best;
+}
+
+uint32_t instruction(const MatrixRef& a, const MatrixRef& b, TileShape s) {
+    const uint32_t size = (uint32_t(s.bn >> 3) << 17) | (uint32_t(s.rows() >> 4) << 24);
     if (is_code(a.type))
         return size | (uint32_t(a.type == kE5M2) << 7) | (uint32_t(b.type == kE5M2) << 10) | (1u << 23);
     const uint32_t f = a.type == kBF16 ? 1 : 0;
     return size | (1u << 4) | (f << 7) | (f << 10) | (uint32_t(a.trans) << 15) | (uint32_t(b.trans) << 16);
 }
 
-int width_for(int rows, bool trans) {
-    const int least = trans ? 64 : 16;
-    for (int w = least; w < 256; w *= 2)
-        if (rows <= w) return w;
-    return 256;
-}
-
-// How a dense product is cut: which side lies along the TMEM lanes, the tile width and the parts of
-// the contraction.
+// How a dense product is cut: which side lies along the TMEM lanes, the tile and the parts of the
+// contraction.
 struct Plan {
     bool swap;
-    int bn, split, steps;   // steps of the contraction per part
-    int cluster;
+    TileShape tile;
+    int split, steps;   // steps of the contraction per part
+    int cluster;        // parts of a cluster (split), or 1: parts joined by a kernel
 };
 
 Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
@@ -713,26 +969,34 @@ Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
     // Few rows: the weights take the 128 lanes, so that no lane idles, and the rows the columns.
     p.swap = m <= 64 && n > m;
     const int P = p.swap ? n : m, Q = p.swap ? m : n;
-    p.bn = width_for(Q, false);
-    auto tiles = [&](int bn) { return (long long)((P + kBM - 1) / kBM) * ((Q + bn - 1) / bn); };
-    while (p.bn > 64 && tiles(p.bn) < sms) p.bn /= 2;
+    p.tile = choose_tile(ceil_div(P, kBM), Q, 1, P > kBM, 16, sms);
     // While SMs are left over, the contraction is cut: into 2, 4 or 8 parts of at least two steps, the CTAs
     // of a cluster, which need no second kernel; where that fills less than half of the SMs and the
     // contraction is long, into as many parts as fill them, of at least eight steps, joined by a kernel.
-    const long long t = tiles(p.bn);
+    long long t = ceil_div(P, p.tile.rows()) * ceil_div(Q, p.tile.bn);
+    if (t * 2 <= sms && steps >= 4 && p.tile.ctas == 2) {
+        p.tile = {128, 1};
+        t = ceil_div(P, kBM) * ceil_div(Q, 128);
+    }
     p.cluster = p.split = 1;
     p.steps = steps;
-    while (p.cluster < 8 && t * p.cluster * 2 <= sms && steps >= 4 * p.cluster) p.cluster *= 2;
-    const long long wide = std::min<long long>(sms / t, steps / 8);
-    if (t < sms && wide >= 2 * p.cluster) {
-        p.cluster = 1;
-        p.split = int(wide);
-    } else {
-        p.split = p.cluster;
+    if (p.tile.ctas == 1) {
+        while (p.cluster < 8 && t * p.cluster * 2 <= sms && steps >= 4 * p.cluster) p.cluster *= 2;
+        const long long wide = std::min<long long>(sms / t, steps / 8);
+        if (t < sms && wide >= 2 * p.cluster) {
+            p.cluster = 1;
+            p.split = int(wide);
+        } else {
+            p.split = p.cluster;
+        }
+        p.steps = (steps + p.split - 1) / p.split;
+        if (p.cluster == 1) p.split = (steps + p.steps - 1) / p.steps;
     }
-    p.steps = (steps + p.split - 1) / p.split;
-    if (p.cluster == 1) p.split = (steps + p.steps - 1) / p.steps;
     return p;
+}
+
+bool whole_rows(const void* p, int type, long long ld, long long batch) {
+    return aligned(p, 16) && ld * elem_bytes(type) % 16 == 0 && batch * elem_bytes(type) % 16 == 0;
 }
 
 }  // namespace
@@ -762,7 +1026,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     j.K = A.cols;
     j.a_mn = A.trans;
     j.b_mn = B.trans;
-    j.idesc = instruction(A, B, pl.bn);
+    j.idesc = instruction(A, B, pl.tile);
     if (fp8) {
         j.sa = pl.swap ? *sb : *sa;
         j.sb = pl.swap ? *sa : *sb;
@@ -787,11 +1051,12 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
         j.bias = out.bias;
         j.bias_type = out.bias_type;
     }
-    const long long tiles = (long long)((j.P + kBM - 1) / kBM) * ((j.Q + pl.bn - 1) / pl.bn) * pl.split;
+    j.out_vec = whole_rows(j.out, j.out_type, j.out_ld, j.split_stride);
+    const long long tiles = ceil_div(j.P, pl.tile.rows()) * ceil_div(j.Q, pl.tile.bn) * pl.split;
     require(tiles < (1LL << 30), "matrix is too large");
-    const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM), mb = operand_map(B, B.trans ? 64 : pl.bn);
-    if (fp8) launch_width<true>(pl.bn, ma, mb, j, tiles, device, stream);
-    else launch_width<false>(pl.bn, ma, mb, j, tiles, device, stream);
+    const CUtensorMap ma = operand_map(A, kBM), mb = operand_map(B, pl.tile.b_rows());
+    if (fp8) launch_shape<true>(pl.tile, ma, mb, j, tiles, device, stream);
+    else launch_shape<false>(pl.tile, ma, mb, j, tiles, device, stream);
     if (pl.split > pl.cluster) {
         const long long n = (long long)a.rows * b.rows;
         k_join_parts<<<unsigned(std::min<long long>((n + 255) / 256, 148 * 8)), 256, 0, stream>>>(
@@ -817,11 +1082,11 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     ProdJob j{};
     const MatrixRef& A = swap ? b : x;
     const MatrixRef& B = swap ? x : b;
-    int bn = swap ? width_for(mean, false) : width_for(b.rows, b.trans);
-    if (!swap) {
-        const long long rows = (x.rows + kBM - 1) / kBM;
-        while (bn > 64 && rows * ((b.rows + bn - 1) / bn) < sm_count(device)) bn /= 2;
-    }
+    // Rows per group are known on the GPU only: full row tiles are counted as if groups were even, and a
+    // pair's 256 rows taken where groups have as many on average.
+    const TileShape tile = swap ? choose_tile(ceil_div(b.rows, kBM) * b.batch, mean, 1, false, 16, sm_count(device))
+                                : choose_tile(ceil_div(mean, kBM) * b.batch, b.rows, 1, mean >= 2 * kBM, b.trans ? 64 : 16,
+                                              sm_count(device));
     j.P = A.rows;
     j.Q = B.rows;
     j.K = A.cols;
@@ -830,7 +1095,7 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     j.off = off;
     j.a_mn = A.trans;
     j.b_mn = B.trans;
-    j.idesc = instruction(A, B, bn);
+    j.idesc = instruction(A, B, tile);
     if (fp8) {
         j.sa = swap ? *sb : *sx;
         j.sb = swap ? *sx : *sb;
@@ -846,14 +1111,14 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     j.after_quantize = after_quantize;
     j.zero_outside = zero_outside;
     j.zero_rows = x.rows;
-    const int high = swap ? bn : kBM, wide = swap ? kBM : bn;
+    j.out_vec = whole_rows(out.ptr, out.type, out.ld, 0);
     // Each group has at most one partly filled row tile.
-    const long long tiles = ((long long)(x.rows + high - 1) / high + std::min(b.batch, x.rows)) *
-                            ((b.rows + wide - 1) / wide);
+    const int high = swap ? tile.bn : tile.rows(), wide = swap ? tile.rows() : tile.bn;
+    const long long tiles = (ceil_div(x.rows, high) + std::min(b.batch, x.rows)) * ceil_div(b.rows, wide);
     require(tiles < (1LL << 30), "matrix is too large");
-    const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM), mb = operand_map(B, B.trans ? 64 : bn);
-    if (fp8) launch_width<true>(bn, ma, mb, j, tiles, device, stream);
-    else launch_width<false>(bn, ma, mb, j, tiles, device, stream);
+    const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM), mb = operand_map(B, B.trans ? 64 : tile.b_rows());
+    if (fp8) launch_shape<true>(tile, ma, mb, j, tiles, device, stream);
+    else launch_shape<false>(tile, ma, mb, j, tiles, device, stream);
 }
 
 void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* off, int groups, void* out,
@@ -866,9 +1131,7 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     require(out && out_type >= kF32 && out_type <= kBF16, "output is out of range");
     OnDevice on(device);
     ProdJob j{};
-    int bn = width_for(x.rows, true);
-    auto count = [&](int w) { return (long long)((g.rows + kBM - 1) / kBM) * ((x.rows + w - 1) / w) * groups; };
-    while (bn > 64 && count(bn) < sm_count(device)) bn /= 2;
+    const TileShape tile = choose_tile(ceil_div(g.rows, kBM), x.rows, groups, g.rows > kBM, 64, sm_count(device));
     j.P = g.rows;
     j.Q = x.rows;
     j.K = g.cols;
@@ -876,15 +1139,17 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     j.groups = groups;
     j.off = off;
     j.a_mn = j.b_mn = 1;
-    j.idesc = instruction(g, x, bn);
+    j.idesc = instruction(g, x, tile);
     j.out = out;
     j.out_type = out_type;
     j.out_ld = x.rows;
     j.out_batch = (long long)g.rows * x.rows;
     j.cols = x.rows;
     j.split = j.cluster = 1;
-    require(count(bn) < (1LL << 30), "matrix is too large");
-    launch_width<false>(bn, operand_map(g, 64), operand_map(x, 64), j, count(bn), device, stream);
+    j.out_vec = whole_rows(out, out_type, j.out_ld, j.out_batch);
+    const long long tiles = ceil_div(g.rows, tile.rows()) * ceil_div(x.rows, tile.bn) * groups;
+    require(tiles < (1LL << 30), "matrix is too large");
+    launch_shape<false>(tile, operand_map(g, 64), operand_map(x, 64), j, tiles, device, stream);
 }
 
 int product_status(int device) {
