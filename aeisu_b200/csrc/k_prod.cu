@@ -91,7 +91,7 @@ struct Shape {
                                  : kColsUsed <= 256 ? 256 : 512;
     // Writers: one warp per 32 lanes, two where each then has at least 32 columns.
     static constexpr int kHalves = BN >= 64 ? 2 : 1, kWide = BN / kHalves;
-    static constexpr int kBars = 3 * kStages + 2 * kScaleSlots + 2 * kAccs + 1;
+    static constexpr int kBars = 3 * kStages + 3 * kScaleSlots + 2 * kAccs + 1;
     static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kScaleSlots * kScaleBytes + kWriters * kTurn + kBars * 8;
     // Behind it the bias of each writer's columns (dense) or the groups' bounds and tiles.
     static constexpr size_t kBias = kWriters * kWide * sizeof(float);
@@ -207,37 +207,49 @@ __device__ __forceinline__ uint32_t address_in(uint32_t saddr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
     return a;
 }
-// Arrive on a barrier of the tile's first CTA.
+// Arrive on a barrier of the tile's first CTA, from the CTA of rank `rank`.
 template <int CTAS>
-__device__ __forceinline__ void arrive_first(uint64_t* bar) {
-    if constexpr (CTAS == 1)
+__device__ __forceinline__ void arrive_first(uint64_t* bar, int rank) {
+    if (CTAS == 1 || rank == 0)
         mbar_arrive(bar);
     else
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
                      :: "r"(address_in(smem_addr(bar), 0)) : "memory");
 }
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elected() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+    return e != 0;
+}
+
+// The clock is read only once a first try has failed: the MMA warp's waits are part of every step.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-    return mbar_wait_bounded(bar, parity, &g_product_error, kErrWait);
+    return mbar_try_wait(bar, parity) || mbar_wait_bounded(bar, parity, &g_product_error, kErrWait);
 }
 // As wait, for a phase that threads of the other CTA complete as well.  (An acquire on the barrier: a
 // fence of cluster scope here doubled the time of every step.)
 template <int CTAS>
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
     if constexpr (CTAS == 1) return wait(bar, parity);
-    const long long t0 = clock64();
-    for (;;) {
-        uint32_t done;
+    auto done = [&] {
+        uint32_t d;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
-        if (done) return true;
+            : "=r"(d) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+        return d != 0;
+    };
+    if (done()) return true;
+    const long long t0 = clock64();
+    while (!done()) {
         if (clock64() - t0 > 4000000000LL) {
             atomicCAS(&g_product_error, 0, kErrWait);
             return false;
         }
     }
+    return true;
 }
 
 // ---- tiles -------------------------------------------------------------------------------------
@@ -480,7 +492,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     uint64_t* fixed = empty + S::kStages;
     uint64_t* scales_full = fixed + S::kStages;
     uint64_t* scales_empty = scales_full + kScaleSlots;
-    uint64_t* acc_full = scales_empty + kScaleSlots;
+    uint64_t* scales_here = scales_empty + kScaleSlots;
+    uint64_t* acc_full = scales_here + kScaleSlots;
     uint64_t* acc_empty = acc_full + S::kAccs;
     uint64_t* drain = acc_empty + S::kAccs;
     int* bound = reinterpret_cast<int*>(drain + 1);
@@ -499,6 +512,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         for (int i = 0; i < kScaleSlots; ++i) {
             mbar_init(scales_full + i, CTAS);
             mbar_init(scales_empty + i, 1);
+            mbar_init(scales_here + i, 1);
         }
         for (int i = 0; i < S::kAccs; ++i) {
             mbar_init(acc_full + i, 1);
@@ -535,23 +549,26 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     const int stride = CTAS == 2 ? int(gridDim.x) / 2 : j.cluster > 1 ? tiles : int(gridDim.x);
     const int a_off = CTAS == 2 ? rank * kBM : 0, b_off = CTAS == 2 ? rank * S::kBRows : 0;
 
+    // Warps 0 and 1 run their loops as whole warps and elect a lane for the copies and MMAs only: addresses
+    // and descriptors then stay in uniform registers.  With one lane running the loop an MMA step took
+    // 700 cycles to issue, against the 512 that it takes to execute.
     if (warp == 0) {
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            long long issued = 0;
-            if (j.after_quantize) grid_dep_wait();
-            for (int t = first_tile; ok && t < tiles; t += stride) {
-                const Tile x = tile_at<BM, BN>(j, g, t, kStep);
-                const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
-                for (int k = x.k0; k < x.k1; k += kStep) {
-                    if (!(ok = wait(empty + stage, phase ^ 1))) break;
-                    const uint32_t a = smem_addr(ring + stage * S::kStage), b = a + S::kATile;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        long long issued = 0;
+        if (j.after_quantize) grid_dep_wait();
+        for (int t = first_tile; ok && t < tiles; t += stride) {
+            const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+            const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
+            for (int k = x.k0; k < x.k1; k += kStep) {
+                if (!(ok = __all_sync(~0u, wait(empty + stage, phase ^ 1)))) break;
+                // A pair's copies all count on its first CTA's barrier; where rows have to be zeroed first,
+                // each CTA's on its own.
+                const bool own = CTAS == 1 || (j.grouping == kContraction && k + kStep > x.k1);
+                if (elected()) {
+                    const uint32_t a = smem_addr(ring) + stage * S::kStage, b = a + S::kATile;
                     const uint32_t local = smem_addr(full + stage);
-                    // A pair's copies all count on its first CTA's barrier; where rows have to be zeroed first,
-                    // each CTA's on its own.
-                    const bool own = CTAS == 1 || (j.grouping == kContraction && k + kStep > x.k1);
                     const uint32_t bar = CTAS == 1 ? local : address_in(local, own ? rank : 0);
                     if (own || rank == 0) mbar_arrive_expect_tx(full + stage, own ? S::kStage : S::kStage * CTAS);
                     if (j.a_mn) {
@@ -565,76 +582,97 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     } else {
                         tma_3d<CTAS>(b, &mb, k, x.q0 + b_off, eb, bar);
                     }
-                    ++issued;
-                    if (++stage == S::kStages) stage = 0, phase ^= 1;
                 }
-            }
-            // Every copy has landed before the CTA may end: those that no MMA waited for are waited for here
-            // (a pair's by its first CTA; the other one cannot end before it).
-            for (int i = 0; !ok && (CTAS == 1 || rank == 0) && i < S::kStages && issued - i > 0; ++i) {
-                const long long n = issued - 1 - i;
-                wait(full + n % S::kStages, uint32_t(n / S::kStages) & 1);
+                __syncwarp();
+                ++issued;
+                if (++stage == S::kStages) stage = 0, phase ^= 1;
             }
         }
+        // Every copy has landed before the CTA may end: those that no MMA waited for are waited for here
+        // (a pair's by its first CTA; the other one cannot end before it).
+        for (int i = 0; !ok && (CTAS == 1 || rank == 0) && i < S::kStages && issued - i > 0; ++i) {
+            const long long n = issued - 1 - i;
+            wait(full + n % S::kStages, uint32_t(n / S::kStages) & 1);
+        }
     } else if (warp == 1) {
-        if (lane == 0 && (CTAS == 1 || rank == 0)) {
-            int stage = 0, acc = 0;
+        if (CTAS == 1 || rank == 0) {
+            int stage = 0, acc = 0, slot = 0;
             uint32_t phase = 0, acc_phase = 0, fixed_phase = 0, slot_phase = 0;
-            int slot = 0;
             bool ok = true;
             const uint32_t a_k = (j.a_mn ? 2048 : 32) >> 4, b_k = (j.b_mn ? 2048 : 32) >> 4;
+            const uint32_t first_a = smem_addr(ring), first_b = first_a + S::kATile;
+            const uint64_t desc_a = j.a_mn ? desc_mnmajor(first_a) : desc_kmajor(first_a);
+            const uint64_t desc_b = j.b_mn ? desc_mnmajor(first_b) : desc_kmajor(first_b);
             for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BM, BN>(j, g, t, kStep);
-                if (!(ok = wait_all<CTAS>(acc_empty + acc, acc_phase ^ 1))) break;
-                fence_after_sync();
+                if (!(ok = __all_sync(~0u, wait_all<CTAS>(acc_empty + acc, acc_phase ^ 1)))) break;
                 const uint32_t d = tmem + acc * BN;
-                uint32_t first = 0;
-                int step = 0;
-                for (int k = x.k0; k < x.k1; k += kStep, ++step) {
+                uint32_t byte = 0;
+                for (int k = x.k0; k < x.k1; k += kStep) {
                     if (j.grouping == kContraction && k + kStep > x.k1) {
-                        if (!(ok = wait_all<CTAS>(fixed + stage, (fixed_phase >> stage) & 1))) break;
+                        ok = wait_all<CTAS>(fixed + stage, (fixed_phase >> stage) & 1);
                         fixed_phase ^= 1u << stage;
                     } else {
-                        if (!(ok = wait(full + stage, phase))) break;
+                        ok = wait(full + stage, phase);
                     }
-                    if (FP8 && step % kGroupSteps == 0 && !(ok = wait_all<CTAS>(scales_full + slot, slot_phase))) break;
+                    if (FP8 && byte == 0) ok = ok && wait_all<CTAS>(scales_full + slot, slot_phase);
+                    if (!(ok = __all_sync(~0u, ok))) break;
                     fence_after_sync();
-                    const uint32_t sa = smem_addr(ring + stage * S::kStage), sb = sa + S::kATile;
-                    const uint64_t da = j.a_mn ? desc_mnmajor(sa) : desc_kmajor(sa);
-                    const uint64_t db = j.b_mn ? desc_mnmajor(sb) : desc_kmajor(sb);
-                    if constexpr (FP8) {
-                        const uint32_t sf = tmem + S::kAccs * BN + slot * S::kScaleCols, byte = step % kGroupSteps;
-                        if (byte == 0) {
-                            const uint32_t src = smem_addr(scales + slot * S::kScaleBytes);
+                    const bool group_ends = FP8 && (byte == kGroupSteps - 1 || k + kStep >= x.k1);
+                    if (elected()) {
+                        const uint64_t da = desc_a + uint32_t(stage * (S::kStage >> 4));
+                        const uint64_t db = desc_b + uint32_t(stage * (S::kStage >> 4));
+                        const uint32_t more = k > x.k0;
+                        if constexpr (FP8) {
+                            const uint32_t sf = tmem + S::kAccs * BN + slot * S::kScaleCols;
+                            if (byte == 0) {
+                                const uint32_t src = smem_addr(scales) + slot * S::kScaleBytes;
 #pragma unroll
-                            for (int i = 0; i <= S::kAtomsB; ++i) scales_to_tmem<CTAS>(sf + 4 * i, src + i * kAtom);
-                        }
-                        const uint32_t id = j.idesc | (byte << 4) | (byte << 29);
+                                for (int i = 0; i <= S::kAtomsB; ++i) scales_to_tmem<CTAS>(sf + 4 * i, src + i * kAtom);
+                            }
+                            const uint32_t id = j.idesc | (byte << 4) | (byte << 29);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            mma_block_scaled<CTAS>(d, da + i * 2, db + i * 2, id, sf, sf + 4, first);
-                            first = 1;
-                        }
-                    } else {
+                            for (int i = 0; i < 4; ++i)
+                                mma_block_scaled<CTAS>(d, da + i * 2, db + i * 2, id, sf, sf + 4, i ? 1 : more);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            mma_half<CTAS>(d, da + i * a_k, db + i * b_k, j.idesc, first);
-                            first = 1;
+                            for (int i = 0; i < 4; ++i) mma_half<CTAS>(d, da + i * a_k, db + i * b_k, j.idesc, i ? 1 : more);
                         }
+                        commit_all<CTAS>(empty + stage);
+                        if (group_ends) commit_all<CTAS>(scales_empty + slot);
                     }
-                    commit_all<CTAS>(empty + stage);
+                    __syncwarp();
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
-                    if (FP8 && (step % kGroupSteps == kGroupSteps - 1 || k + kStep >= x.k1)) {
-                        commit_all<CTAS>(scales_empty + slot);
-                        if (++slot == kScaleSlots) slot = 0, slot_phase ^= 1;
+                    if (FP8) {
+                        byte = group_ends ? 0 : byte + 1;
+                        if (group_ends && ++slot == kScaleSlots) slot = 0, slot_phase ^= 1;
                     }
                 }
-                commit_all<CTAS>(acc_full + acc);
+                if (elected()) commit_all<CTAS>(acc_full + acc);
+                __syncwarp();
                 if (++acc == S::kAccs) acc = 0, acc_phase ^= 1;
             }
             if (!ok) {   // let the MMAs in flight land before TMEM goes
-                commit_all<CTAS>(drain);
+                if (elected()) commit_all<CTAS>(drain);
+                __syncwarp();
                 wait(drain, 0);
+            }
+        }
+        if constexpr (FP8 && CTAS == 2) {
+            // The second CTA tells the first that its scales are in place.  Its release of cluster scope takes
+            // about as long as a step, and here it holds up no load.
+            if (lane == 0 && rank == 1) {
+                int slot = 0;
+                uint32_t phase = 0;
+                bool ok = true;
+                for (int t = first_tile; ok && t < tiles; t += stride) {
+                    const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+                    for (int k = x.k0; k < x.k1; k += kGroupSteps * kStep) {
+                        if (!(ok = wait(scales_here + slot, phase))) break;
+                        arrive_first<CTAS>(scales_full + slot, rank);
+                        if (++slot == kScaleSlots) slot = 0, phase ^= 1;
+                    }
+                }
             }
         }
     } else if (warp == 2) {
@@ -676,8 +714,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 for (int i = 0; i < S::kAtomsB; ++i) store_scales(raw_b[i], way_b, dst + (1 + i) * kAtom);
                 fence_async_smem();
                 __syncwarp();
-                // (One release of cluster scope per group: one per step cost more than the step.)
-                if (lane == 0) arrive_first<CTAS>(scales_full + slot);
+                if (lane == 0) mbar_arrive((rank == 0 || CTAS == 1 ? scales_full : scales_here) + slot);
                 if (++slot == kScaleSlots) slot = 0, phase ^= 1;
                 k += kGroupSteps * kStep;
                 if (k >= x.k1) {
@@ -705,7 +742,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                                 make_uint4(0, 0, 0, 0);
                         fence_async_smem();
                         __syncwarp();
-                        if (lane == 0) arrive_first<CTAS>(fixed + stage);
+                        if (lane == 0) arrive_first<CTAS>(fixed + stage, rank);
                     }
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
                 }
@@ -739,7 +776,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             }
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) arrive_first<CTAS>(acc_empty + acc);
+            if (lane == 0) arrive_first<CTAS>(acc_empty + acc, rank);
             if (++acc == S::kAccs) acc = 0, acc_phase ^= 1;
 
             const int p0 = x.p0 + a_off + quad * 32, q0 = x.q0 + col;
