@@ -331,27 +331,29 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
     }
 }
 
-// Column sums: each CTA adds a run of rows of 64 columns (lanes: column pairs, warps: every eighth
-// row), then the runs are added in order.
-template <typename T>
+// Column sums: each CTA adds a run of rows of 64 columns (lanes: eight columns of every fourth row of a
+// warp's), then the runs are added in order.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_column_runs(const T* x, int rows, int cols, long long ld, int run,
                                                           float* partial) {
-    __shared__ float sh[8][64];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = int(blockIdx.x) * 64 + lane;
+    __shared__ float sh[32][65];
+    const int part = threadIdx.x >> 3, oct = threadIdx.x & 7, c = int(blockIdx.x) * 64 + oct * 8;
     const int r1 = min(rows, int(blockIdx.y + 1) * run);
-    float a = 0.f, b = 0.f;
+    float a[8] = {};
 #pragma unroll 4
-    for (int r = int(blockIdx.y) * run + warp; r < r1; r += 8) {
-        if (c < cols) a += to_f32(x[r * ld + c]);
-        if (c + 32 < cols) b += to_f32(x[r * ld + c + 32]);
+    for (int r = int(blockIdx.y) * run + part; r < r1; r += 32) {
+        Vals<T> v;
+        load8<T, VEC>(v, 0, x + r * ld, c, cols);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] += v.get(i);
     }
-    sh[warp][lane] = a;
-    sh[warp][lane + 32] = b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sh[part][oct * 8 + i] = a[i];
     __syncthreads();
     if (threadIdx.x < 64 && int(blockIdx.x) * 64 + int(threadIdx.x) < cols) {
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) s += sh[w][threadIdx.x];
+        for (int w = 0; w < 32; ++w) s += sh[w][threadIdx.x];
         partial[size_t(blockIdx.y) * cols + blockIdx.x * 64 + threadIdx.x] = s;
     }
 }
@@ -453,7 +455,12 @@ void column_sum(const MatrixRef& x, void* out, int out_type, float* partial, int
     const dim3 grid(unsigned((x.cols + 63) / 64), unsigned(runs), 1);
     auto in = [&](auto t) {
         using T = decltype(t);
-        k_column_runs<T><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(x.ptr), x.rows, x.cols, x.ld, run, partial);
+        const T* p = static_cast<const T*>(x.ptr);
+        constexpr int n = Vals<T>::n;
+        if (aligned(p, 16) && x.ld % n == 0 && x.cols % n == 0)
+            k_column_runs<T, true><<<grid, kThreads, 0, stream>>>(p, x.rows, x.cols, x.ld, run, partial);
+        else
+            k_column_runs<T, false><<<grid, kThreads, 0, stream>>>(p, x.rows, x.cols, x.ld, run, partial);
     };
     auto join = [&](auto t) {
         using T = decltype(t);

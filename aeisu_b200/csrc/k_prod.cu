@@ -6,12 +6,12 @@
 // half of B's rows, so that a pair reads and stages B once.  Per step of 128 bytes of the contraction,
 // warp 0 copies the operands' tiles by TMA into a ring of 128-byte swizzled stages, warp 1 (of the
 // pair's first CTA) issues four MMAs into FP32 accumulators in TMEM, warps 4..11 write the finished tile
-// out (TMEM lane = row of A).  Warp 2 serves the form of the product:
+// out (TMEM lane = row of A).  Warps 2 and 3 serve the form of the product:
 //   * FP8: kind::mxf8f6f4.block_scale applies a power-of-two scale per row and 32 values inside the
 //     tensor core; a block of 128 is four such steps with the same scale.  The scales of 128 rows and
 //     four blocks form the 512-byte atom that tcgen05.cp spreads over the TMEM lanes (row r, block j at
-//     (r % 32) * 16 + (r / 32) * 4 + j); warp 2 gathers it from global memory once per four steps, one
-//     atom ahead, and the MMA names the byte j.  The accumulator never leaves TMEM before the tile is done.
+//     (r % 32) * 16 + (r / 32) * 4 + j); warps 2 and 3 gather it from global memory once per four
+//     steps, in turn and ahead of time, and the MMA names the byte j.  The accumulator never leaves TMEM before the tile is done.
 //   * contraction grouped by expert: a group's last step may reach into the next group's rows; warp 2
 //     zeroes those rows of both operands in shared memory before the MMA sees the stage.
 // The writers take a whole tile into registers and hand TMEM back before they store, because 256 columns
@@ -42,14 +42,25 @@ constexpr int kTurn = 2048;           // shared memory of a writer: 32 rows of 6
 constexpr int kErrWait = 1;           // error code: a wait ran out
 constexpr int kAtom = 512;            // scales of 128 rows and four block columns
 constexpr int kGroupSteps = 4;        // steps that share an atom
-constexpr int kScaleSlots = 4;        // groups of steps whose scales are staged
+constexpr int kScaleSlots = 4;        // groups of steps whose scales are staged (even: two warps fill them)
 
 // What is grouped by the offsets.
 enum Grouping { kDense = 0, kRowsA = 1, kRowsB = 2, kContraction = 3 };
 
 __device__ int g_product_error;
 
+// Division of 0 <= t < 2^31 by a constant of the launch: floor(t / d) = hi(t * mul) >> shift with
+// mul = ceil(2^(32 + shift) / d), 2^shift < d <= 2^(shift + 1).
+struct Divider {
+    uint32_t mul, shift, d;
+    __device__ __forceinline__ int quotient(int t) const {
+        return d == 1 ? t : int(__umulhi(uint32_t(t), mul) >> shift);
+    }
+};
+
 struct ProdJob {
+    Divider by_tiles, by_band, by_tp, by_rest;   // tiles of one part or group, of 16 row tiles; row tiles, of the last band
+    int tp, tq;                  // row tiles of A and B
     int P, Q, K;                 // rows of A, rows of B, contraction (whole sides; per batch entry)
     int grouping, groups;
     const int* off;
@@ -91,8 +102,9 @@ struct Shape {
                                  : kColsUsed <= 256 ? 256 : 512;
     // Writers: one warp per 32 lanes, two where each then has at least 32 columns.
     static constexpr int kHalves = BN >= 64 ? 2 : 1, kWide = BN / kHalves;
-    static constexpr int kBars = 3 * kStages + 3 * kScaleSlots + 2 * kAccs + 1;
-    static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kScaleSlots * kScaleBytes + kWriters * kTurn + kBars * 8;
+    static constexpr int kBars = 3 * kStages + 4 * kScaleSlots + 2 * kAccs + 1;
+    static constexpr int kBarBytes = (kBars * 8 + 15) / 16 * 16;   // what lies behind is read in 16-byte words
+    static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kScaleSlots * kScaleBytes + kWriters * kTurn + kBarBytes;
     // Behind it the bias of each writer's columns (dense) or the groups' bounds and tiles.
     static constexpr size_t kBias = kWriters * kWide * sizeof(float);
 };
@@ -207,13 +219,18 @@ __device__ __forceinline__ uint32_t address_in(uint32_t saddr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
     return a;
 }
-// Arrive on a barrier of the tile's first CTA, from the CTA of rank `rank`.
+// Arrive on a barrier of the tile's first CTA, from the CTA of rank `rank`.  Without `data` nothing in
+// memory is handed over (TMEM columns that have been read), and the arrival need not wait for this
+// thread's stores.
 template <int CTAS>
-__device__ __forceinline__ void arrive_first(uint64_t* bar, int rank) {
+__device__ __forceinline__ void arrive_first(uint64_t* bar, int rank, bool data) {
     if (CTAS == 1 || rank == 0)
         mbar_arrive(bar);
-    else
+    else if (data)
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+                     :: "r"(address_in(smem_addr(bar), 0)) : "memory");
+    else
+        asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];"
                      :: "r"(address_in(smem_addr(bar), 0)) : "memory");
 }
 
@@ -266,40 +283,49 @@ struct Tile {
 // no smaller than the one before, so that no value of theirs leads out of the tensors.
 struct Groups {
     const int* bound;    // [groups + 1]
-    const int* cum;      // [groups + 1] row tiles before each group
+    const int* cum;      // [groups + 1] row tiles before each group, or the groups by falling size
+    __device__ __forceinline__ int order(int i) const { return cum[i]; }
 };
 
-template <int BM, int BN>
+constexpr int kBand = 16;   // row tiles of a band
+
 __device__ __forceinline__ int tile_count(const ProdJob& j, const Groups& g) {
-    const int tp = (j.P + BM - 1) / BM, tq = (j.Q + BN - 1) / BN;
-    if (j.grouping == kDense) return tp * tq * j.split;
-    if (j.grouping == kContraction) return tp * tq * j.groups;
-    return g.cum[j.groups] * (j.grouping == kRowsA ? tq : tp);
+    if (j.grouping == kDense) return j.tp * j.tq * j.split;
+    if (j.grouping == kContraction) return j.tp * j.tq * j.groups;
+    return g.cum[j.groups] * (j.grouping == kRowsA ? j.tq : j.tp);
 }
 
 template <int BM, int BN>
 __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t, int step) {
-    const int tp = (j.P + BM - 1) / BM, tq = (j.Q + BN - 1) / BN;
     Tile x{0, 0, 0, j.P, j.Q, 0, j.K, 0};
     if (j.grouping == kDense) {
         // Bands of 16 row tiles, walked column by column: CTAs that run at the same time share both
         // operands' tiles in L2.
-        x.part = t / (tp * tq);
-        t -= x.part * tp * tq;
-        const int band = t / (16 * tq), first = band * 16, high = min(16, tp - first), in = t - band * 16 * tq;
-        x.p0 = (first + in % high) * BM;
-        x.q0 = (in / high) * BN;
+        x.part = j.by_tiles.quotient(t);
+        t -= x.part * int(j.by_tiles.d);
+        const int band = j.by_band.quotient(t), first = band * kBand;
+        t -= band * int(j.by_band.d);
+        const bool last = j.tp - first < kBand;
+        const int col = last ? j.by_rest.quotient(t) : t / kBand;
+        x.p0 = (first + t - col * (last ? int(j.by_rest.d) : kBand)) * BM;
+        x.q0 = col * BN;
         x.k0 = x.part * j.steps_per_split * step;
         x.k1 = min(j.K, x.k0 + j.steps_per_split * step);
     } else if (j.grouping == kContraction) {
-        x.e = t / (tp * tq);
-        t -= x.e * tp * tq;
-        x.p0 = (t % tp) * BM;
-        x.q0 = (t / tp) * BN;
+        // Groups from the longest to the shortest, in turns that run to and fro over the CTAs: the time of a
+        // tile goes by the rows of its group.
+        const int lanes = int(gridDim.x) * kBM / BM, turn = t / lanes;
+        if ((turn & 1) && j.tp * j.tq * j.groups - turn * lanes >= lanes) t = turn * lanes + lanes - 1 - (t - turn * lanes);
+        const int i = j.by_tiles.quotient(t);
+        x.e = g.order(i);
+        t -= i * int(j.by_tiles.d);
+        const int col = j.by_tp.quotient(t);
+        x.p0 = (t - col * j.tp) * BM;
+        x.q0 = col * BN;
         x.k0 = g.bound[x.e];
         x.k1 = g.bound[x.e + 1];
     } else {
-        const int other = j.grouping == kRowsA ? tq : tp;
+        const int other = j.grouping == kRowsA ? j.tq : j.tp;
         int lo = 0, hi = j.groups - 1;       // last group whose tiles start at or before t
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -308,14 +334,15 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
         }
         x.e = lo;
         const int own = g.cum[lo + 1] - g.cum[lo], in = t - g.cum[lo] * other;
+        const int col = own == 1 ? in : in / own, row = in - col * own;
         if (j.grouping == kRowsA) {
-            x.p0 = g.bound[lo] + (in % own) * BM;
+            x.p0 = g.bound[lo] + row * BM;
             x.p1 = g.bound[lo + 1];
-            x.q0 = (in / own) * BN;
+            x.q0 = col * BN;
         } else {
-            x.q0 = g.bound[lo] + (in % own) * BN;
+            x.q0 = g.bound[lo] + row * BN;
             x.q1 = g.bound[lo + 1];
-            x.p0 = (in / own) * BM;
+            x.p0 = col * BM;
         }
     }
     return x;
@@ -418,46 +445,78 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
     }
 }
 
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // The warp's 32 rows by W columns to out[p][q]: runs of 64 bytes turn through shared memory, so that
 // four lanes store one row's run.  Its 16-byte pieces are exclusive-or'ed with the row pair: no bank
 // conflicts either way.  Where rows do not start on 16-byte boundaries, or columns end, elements are
-// stored one by one, neighbouring lanes at neighbouring addresses.
+// stored one by one, neighbouring lanes at neighbouring addresses.  (Straight-line code with few
+// instructions per run: with element-wise conversions and addresses a run of 32 columns took 1,350 cycles.)
 template <typename T, int W>
-__device__ __forceinline__ void write_rows(const ProdJob& j, const uint32_t* v, const float* bias, uint8_t* turn,
+__device__ __forceinline__ void write_rows(const ProdJob& j, uint32_t* v, const float* bias, uint8_t* turn,
                                            long long base, int p0, int p1, int q0, int q1) {
     constexpr int kRun = 64 / sizeof(T) < W ? 64 / sizeof(T) : W, kPieces = kRun * sizeof(T) / 16;
+    constexpr int kWords = kRun * sizeof(T) / 4;      // of a row's run
     const int lane = threadIdx.x & 31;
+    if (j.bias) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + i);
+            v[i] = __float_as_uint(__uint_as_float(v[i]) + b.x);
+            v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) + b.y);
+            v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) + b.z);
+            v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) + b.w);
+        }
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+    }
+    uint8_t* put = turn + lane * 64;
+    const int turned = (lane >> 1) & (kPieces - 1);
+    const int row = lane / kPieces, piece = lane % kPieces;
+    const uint8_t* take = turn + row * 64 + ((piece ^ ((row >> 1) & (kPieces - 1))) << 4);
     T* out = static_cast<T*>(j.out) + base;
+    T* dst = out + (p0 + row) * j.out_ld + q0 + piece * int(16 / sizeof(T));
+    const long long down = j.out_ld * (32 / kPieces);
+    const int rows = p1 - p0 - row;                   // this lane stores rows row + i * 32 / kPieces
     const bool whole = j.out_vec && base % (16 / sizeof(T)) == 0;
 #pragma unroll
-    for (int c = 0; c < W; c += kRun) {
-        if (q0 + c >= q1) break;
-        uint4 piece[kPieces];
-        T* e = reinterpret_cast<T*>(piece);
+    for (int c = 0; c < W / kRun; ++c) {
+        if (q0 + c * kRun < q1) {
 #pragma unroll
-        for (int i = 0; i < kRun; ++i)
-            e[i] = rounded<T>(__uint_as_float(v[c + i]) + (j.bias ? bias[c + i] : 0.f));
+            for (int i = 0; i < kPieces; ++i)
+                *reinterpret_cast<uint4*>(put + ((i ^ turned) << 4)) =
+                    make_uint4(v[c * kWords + 4 * i], v[c * kWords + 4 * i + 1], v[c * kWords + 4 * i + 2],
+                               v[c * kWords + 4 * i + 3]);
+            __syncwarp();
+            if (whole && q0 + (c + 1) * kRun <= q1) {
+                uint4 q[kPieces];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-            *reinterpret_cast<uint4*>(turn + lane * 64 + ((i ^ ((lane >> 1) & (kPieces - 1))) << 4)) = piece[i];
-        __syncwarp();
-        if (whole && q0 + c + kRun <= q1) {
+                for (int i = 0; i < kPieces; ++i)
+                    q[i] = *reinterpret_cast<const uint4*>(take + i * (32 / kPieces) * 64);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int at = i * 32 + lane, r = at / kPieces, k = at % kPieces;
-                const uint4 q = *reinterpret_cast<const uint4*>(turn + r * 64 + ((k ^ ((r >> 1) & (kPieces - 1))) << 4));
-                if (p0 + r < p1)
-                    *reinterpret_cast<uint4*>(out + (p0 + r) * j.out_ld + q0 + c + k * (16 / sizeof(T))) = q;
+                for (int i = 0; i < kPieces; ++i)
+                    if (i * (32 / kPieces) < rows) *reinterpret_cast<uint4*>(dst + i * down + c * kRun) = q[i];
+            } else {
+#pragma unroll 1
+                for (int at = lane; at < 32 * kRun; at += 32) {
+                    const int r = at / kRun, k = at % kRun, b = k * int(sizeof(T));
+                    if (p0 + r < p1 && q0 + c * kRun + k < q1)
+                        out[(p0 + r) * j.out_ld + q0 + c * kRun + k] = *reinterpret_cast<const T*>(
+                            turn + r * 64 + (((b >> 4) ^ ((r >> 1) & (kPieces - 1))) << 4) + (b & 15));
+                }
             }
-        } else {
-            for (int at = lane; at < 32 * kRun; at += 32) {
-                const int r = at / kRun, k = at % kRun, b = k * int(sizeof(T));
-                if (p0 + r < p1 && q0 + c + k < q1)
-                    out[(p0 + r) * j.out_ld + q0 + c + k] = *reinterpret_cast<const T*>(
-                        turn + r * 64 + (((b >> 4) ^ ((r >> 1) & (kPieces - 1))) << 4) + (b & 15));
-            }
+            __syncwarp();
         }
-        __syncwarp();
     }
 }
 
@@ -493,10 +552,11 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     uint64_t* scales_full = fixed + S::kStages;
     uint64_t* scales_empty = scales_full + kScaleSlots;
     uint64_t* scales_here = scales_empty + kScaleSlots;
-    uint64_t* acc_full = scales_here + kScaleSlots;
+    uint64_t* scales_there = scales_here + kScaleSlots;
+    uint64_t* acc_full = scales_there + kScaleSlots;
     uint64_t* acc_empty = acc_full + S::kAccs;
     uint64_t* drain = acc_empty + S::kAccs;
-    int* bound = reinterpret_cast<int*>(drain + 1);
+    int* bound = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + S::kBarBytes);
     int* cum = bound + j.groups + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // A pair takes a tile; otherwise a cluster takes one tile, each of its CTAs a part of the contraction.
@@ -510,7 +570,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             mbar_init(fixed + i, CTAS);
         }
         for (int i = 0; i < kScaleSlots; ++i) {
-            mbar_init(scales_full + i, CTAS);
+            mbar_init(scales_full + i, 1);
+            mbar_init(scales_there + i, 1);
             mbar_init(scales_empty + i, 1);
             mbar_init(scales_here + i, 1);
         }
@@ -536,13 +597,25 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 cum[i + 1] = tiles;
             }
         }
+        if (j.grouping == kContraction) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < j.groups; i += kThreads) {
+                const int size = bound[i + 1] - bound[i];
+                int at = 0;
+                for (int o = 0; o < j.groups; ++o) {
+                    const int other = bound[o + 1] - bound[o];
+                    at += other > size || (other == size && o < i);
+                }
+                cum[at] = i;
+            }
+        }
     }
     fence_before_sync();
     __syncthreads();
     if constexpr (CTAS == 2) cluster_sync();
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
-    const int tiles = tile_count<BM, BN>(j, g);
+    const int tiles = tile_count(j, g);
     const int first_tile = CTAS == 2       ? int(blockIdx.x) / 2
                            : j.cluster > 1 ? rank * (tiles / j.split) + int(blockIdx.x) / j.cluster
                                            : int(blockIdx.x);
@@ -605,7 +678,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             const uint64_t desc_b = j.b_mn ? desc_mnmajor(first_b) : desc_kmajor(first_b);
             for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BM, BN>(j, g, t, kStep);
-                if (!(ok = __all_sync(~0u, wait_all<CTAS>(acc_empty + acc, acc_phase ^ 1)))) break;
+                if (!(ok = __all_sync(~0u, wait(acc_empty + acc, acc_phase ^ 1)))) break;
                 const uint32_t d = tmem + acc * BN;
                 uint32_t byte = 0;
                 for (int k = x.k0; k < x.k1; k += kStep) {
@@ -615,7 +688,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     } else {
                         ok = wait(full + stage, phase);
                     }
-                    if (FP8 && byte == 0) ok = ok && wait_all<CTAS>(scales_full + slot, slot_phase);
+                    if (FP8 && byte == 0) ok = ok && wait(scales_full + slot, slot_phase);
                     if (!(ok = __all_sync(~0u, ok))) break;
                     fence_after_sync();
                     const bool group_ends = FP8 && (byte == kGroupSteps - 1 || k + kStep >= x.k1);
@@ -669,13 +742,13 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     const Tile x = tile_at<BM, BN>(j, g, t, kStep);
                     for (int k = x.k0; k < x.k1; k += kGroupSteps * kStep) {
                         if (!(ok = wait(scales_here + slot, phase))) break;
-                        arrive_first<CTAS>(scales_full + slot, rank);
+                        arrive_first<CTAS>(scales_there + slot, rank, true);
                         if (++slot == kScaleSlots) slot = 0, phase ^= 1;
                     }
                 }
             }
         }
-    } else if (warp == 2) {
+    } else if (warp == 2 || (FP8 && warp == 3)) {
         [[maybe_unused]] int stage = 0;
         uint32_t phase = 0;
         [[maybe_unused]] bool ok = true;
@@ -692,9 +765,10 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 for (int i = 0; i < S::kAtomsB; ++i)
                     load_scales(raw_b[i], j.sb, way_b, eb, x.q0 + 128 * i, j.b_rows, k / kBlock, blocks);
             };
+            // The two warps take every other group each.
             int t = first_tile, k = 0;
             Tile x{};
-            // To the first step of a tile that has one.
+            // To the first step of a tile that has one, and from group to group.
             auto settle = [&] {
                 while (t < tiles) {
                     x = tile_at<BM, BN>(j, g, t, kStep);
@@ -703,9 +777,17 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     t += stride;
                 }
             };
+            auto advance = [&] {
+                k += kGroupSteps * kStep;
+                if (k >= x.k1) {
+                    t += stride;
+                    settle();
+                }
+            };
             settle();
+            if (warp == 3 && t < tiles) advance();
             if (t < tiles) load(x, k);
-            int slot = 0;
+            int slot = warp - 2;
             for (bool more = t < tiles; more;) {
                 if (!wait(scales_empty + slot, phase ^ 1)) break;
                 uint8_t* dst = scales + slot * S::kScaleBytes;
@@ -714,13 +796,13 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 for (int i = 0; i < S::kAtomsB; ++i) store_scales(raw_b[i], way_b, dst + (1 + i) * kAtom);
                 fence_async_smem();
                 __syncwarp();
+                // The first CTA's warp also takes in the other one's word, an acquire of cluster scope that would
+                // cost the MMA warp 480 cycles per group.
+                if (CTAS == 2 && rank == 0 && !wait_all<CTAS>(scales_there + slot, phase)) break;
                 if (lane == 0) mbar_arrive((rank == 0 || CTAS == 1 ? scales_full : scales_here) + slot);
-                if (++slot == kScaleSlots) slot = 0, phase ^= 1;
-                k += kGroupSteps * kStep;
-                if (k >= x.k1) {
-                    t += stride;
-                    settle();
-                }
+                if ((slot += 2) >= kScaleSlots) slot -= kScaleSlots, phase ^= 1;
+                advance();
+                if (t < tiles) advance();
                 more = t < tiles;
                 if (more) load(x, k);
             }
@@ -742,7 +824,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                                 make_uint4(0, 0, 0, 0);
                         fence_async_smem();
                         __syncwarp();
-                        if (lane == 0) arrive_first<CTAS>(fixed + stage, rank);
+                        if (lane == 0) arrive_first<CTAS>(fixed + stage, rank, true);
                     }
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
                 }
@@ -776,7 +858,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             }
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) arrive_first<CTAS>(acc_empty + acc, rank);
+            if (lane == 0) arrive_first<CTAS>(acc_empty + acc, rank, false);
             if (++acc == S::kAccs) acc = 0, acc_phase ^= 1;
 
             const int p0 = x.p0 + a_off + quad * 32, q0 = x.q0 + col;
@@ -969,15 +1051,19 @@ void launch_shape(TileShape s, const CUtensorMap& a, const CUtensorMap& b, const
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // The tile for P x Q outputs, `count` of them: the one with the shortest time by waves of tiles over the
-// SMs.  A step's time goes by the operand bytes a CTA stages, A's 128 rows and its share of B's.
-TileShape choose_tile(long long row_tiles_of_128, int q, long long count, bool pairs, int least, int sms) {
+// SMs.  A step takes as long as the operand bytes that a CTA stages, A's 128 rows and its share of B's
+// (256 rows: 512 cycles); starting and ending a tile, as long as 250 rows, 750 for a pair, whose CTAs
+// signal each other.
+TileShape choose_tile(long long row_tiles_of_128, int q, long long count, long long steps, bool pairs, int least,
+                      int sms) {
     TileShape best{least, 1};
     double time = 0;
     for (const TileShape s : {TileShape{16, 1}, TileShape{32, 1}, TileShape{64, 1}, TileShape{128, 1}, TileShape{128, 2},
                               TileShape{256, 2}}) {
         if (s.bn < least || (s.ctas == 2 && !pairs)) continue;
         const long long tiles = ceil_div(row_tiles_of_128, s.ctas) * ceil_div(q, s.bn) * count;
-        const double t = double(ceil_div(tiles, sms / s.ctas)) * (kBM + s.b_rows());
+        const double t = double(ceil_div(tiles, sms / s.ctas)) *
+                         (double(steps) * (kBM + s.b_rows()) + (s.ctas == 2 ? 750 : 250));
         if (time == 0 || t < time) best = s, time = t;
     }
     return best;
@@ -1006,18 +1092,19 @@ Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
     // Few rows: the weights take the 128 lanes, so that no lane idles, and the rows the columns.
     p.swap = m <= 64 && n > m;
     const int P = p.swap ? n : m, Q = p.swap ? m : n;
-    p.tile = choose_tile(ceil_div(P, kBM), Q, 1, P > kBM, 16, sms);
-    // While SMs are left over, the contraction is cut: into 2, 4 or 8 parts of at least two steps, the CTAs
-    // of a cluster, which need no second kernel; where that fills less than half of the SMs and the
-    // contraction is long, into as many parts as fill them, of at least eight steps, joined by a kernel.
-    long long t = ceil_div(P, p.tile.rows()) * ceil_div(Q, p.tile.bn);
-    if (t * 2 <= sms && steps >= 4 && p.tile.ctas == 2) {
-        p.tile = {128, 1};
-        t = ceil_div(P, kBM) * ceil_div(Q, 128);
-    }
+    p.tile = choose_tile(ceil_div(P, kBM), Q, 1, steps, P > kBM, 16, sms);
+    // Where one CTA per 128 rows and up to 128 columns leaves half of the SMs over, each takes as many columns
+    // as there are, so that A is staged once, and the contraction is cut instead: into 2, 4 or 8 parts of at
+    // least two steps, the CTAs of a cluster, which need no second kernel; where that fills less than half of
+    // the SMs and the contraction is long, into as many parts as fill them, of at least eight steps, joined
+    // by a kernel.
+    TileShape widest{16, 1};
+    while (widest.bn < std::min(Q, 128)) widest.bn *= 2;
+    const long long t = ceil_div(P, kBM) * ceil_div(Q, widest.bn);
+    if (t * 2 <= sms && steps >= 4) p.tile = widest;
     p.cluster = p.split = 1;
     p.steps = steps;
-    if (p.tile.ctas == 1) {
+    if (t * 2 <= sms && steps >= 4) {
         while (p.cluster < 8 && t * p.cluster * 2 <= sms && steps >= 4 * p.cluster) p.cluster *= 2;
         const long long wide = std::min<long long>(sms / t, steps / 8);
         if (t < sms && wide >= 2 * p.cluster) {
@@ -1030,6 +1117,24 @@ Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
         if (p.cluster == 1) p.split = (steps + p.steps - 1) / p.steps;
     }
     return p;
+}
+
+Divider divider(long long d) {
+    Divider v{0, 0, uint32_t(d)};
+    while ((2ull << v.shift) < uint64_t(d)) ++v.shift;
+    v.mul = uint32_t(((1ull << (32 + v.shift)) + uint64_t(d) - 1) / uint64_t(d));
+    return v;
+}
+// Tiles of the job, and the divisions that number them.
+void lay_tiles(ProdJob& j, TileShape s) {
+    j.tp = int(ceil_div(j.P, s.rows()));
+    j.tq = int(ceil_div(j.Q, s.bn));
+    const long long all = (long long)j.tp * j.tq;
+    require(all < (1LL << 28), "matrix is too large");
+    j.by_tiles = divider(all);
+    j.by_band = divider(kBand * (long long)j.tq);
+    j.by_tp = divider(j.tp);
+    j.by_rest = divider(std::max(1, j.tp % kBand));
 }
 
 bool whole_rows(const void* p, int type, long long ld, long long batch) {
@@ -1072,6 +1177,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     j.b_rows = B.rows;
     j.swapped = pl.swap;
     j.cols = b.rows;
+    lay_tiles(j, pl.tile);
     j.split = pl.split;
     j.steps_per_split = pl.steps;
     j.cluster = pl.cluster;
@@ -1121,9 +1227,11 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     const MatrixRef& B = swap ? x : b;
     // Rows per group are known on the GPU only: full row tiles are counted as if groups were even, and a
     // pair's 256 rows taken where groups have as many on average.
-    const TileShape tile = swap ? choose_tile(ceil_div(b.rows, kBM) * b.batch, mean, 1, false, 16, sm_count(device))
-                                : choose_tile(ceil_div(mean, kBM) * b.batch, b.rows, 1, mean >= 2 * kBM, b.trans ? 64 : 16,
-                                              sm_count(device));
+    const int steps = int(ceil_div((long long)x.cols * elem_bytes(x.type), kStepBytes));
+    const TileShape tile =
+        swap ? choose_tile(ceil_div(b.rows, kBM) * b.batch, mean, 1, steps, false, 16, sm_count(device))
+             : choose_tile(ceil_div(mean, kBM) * b.batch, b.rows, 1, steps, mean >= 2 * kBM, b.trans ? 64 : 16,
+                           sm_count(device));
     j.P = A.rows;
     j.Q = B.rows;
     j.K = A.cols;
@@ -1144,6 +1252,7 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     j.out_ld = out.ld;
     j.swapped = swap;
     j.cols = b.rows;
+    lay_tiles(j, tile);
     j.split = j.cluster = 1;
     j.after_quantize = after_quantize;
     j.zero_outside = zero_outside;
@@ -1168,7 +1277,8 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     require(out && out_type >= kF32 && out_type <= kBF16, "output is out of range");
     OnDevice on(device);
     ProdJob j{};
-    const TileShape tile = choose_tile(ceil_div(g.rows, kBM), x.rows, groups, g.rows > kBM, 64, sm_count(device));
+    const TileShape tile = choose_tile(ceil_div(g.rows, kBM), x.rows, groups, ceil_div(ceil_div(g.cols, groups), kStepBytes / 2),
+                                       g.rows > kBM, 64, sm_count(device));
     j.P = g.rows;
     j.Q = x.rows;
     j.K = g.cols;
@@ -1182,6 +1292,7 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     j.out_ld = x.rows;
     j.out_batch = (long long)g.rows * x.rows;
     j.cols = x.rows;
+    lay_tiles(j, tile);
     j.split = j.cluster = 1;
     j.out_vec = whole_rows(out, out_type, j.out_ld, j.out_batch);
     const long long tiles = ceil_div(g.rows, tile.rows()) * ceil_div(x.rows, tile.bn) * groups;
