@@ -93,5 +93,10 @@ def linear_bytes(m, n, k, train, index):
     return _lib.lib().aeisu_linear_workspace(m, n, k, train, index)
 
 
+@functools.lru_cache(maxsize=4096)
+def kept_bytes(rows, cols, block_rows):
+    return _lib.lib().aeisu_linear_kept_bytes(rows, cols, block_rows)
+
+
 def scratch(size, device):
     return torch.empty(size, dtype=torch.uint8, device=device)

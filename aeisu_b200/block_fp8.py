@@ -177,16 +177,15 @@ def _rows(x):
 
 
 def _forward(x, weight, bias, kept_x, kept_w, index):
-    """The layer on float x and weight, leaving the transposed codes in the kept buffers."""
+    """The layer on float x and weight, leaving the transposed codes at the addresses kept_x and kept_w."""
     (m, k), n, device = x.shape, weight.shape[0], x.device
-    out = torch.empty((m, n), dtype=x.dtype, device=device)
+    out = x.new_empty((m, n))
     size = mx.linear_bytes(m, n, k, 1, index)
     ws = mx.scratch(size, device)
     (x, mat), (weight, mw) = _rows(x), _rows(weight)
     _lib.check(_lib.lib().aeisu_linear_forward(
         mat, mw, None if bias is None else bias.data_ptr(), 0 if bias is None else mx.TYPES[bias.dtype],
-        mx.matrix(out, n), None if kept_x is None else kept_x.data_ptr(), None if kept_w is None else kept_w.data_ptr(),
-        ws.data_ptr(), size, index, mx.stream(index)))
+        mx.matrix(out, n), kept_x, kept_w, ws.data_ptr(), size, index, mx.stream(index)))
     return out
 
 
@@ -197,16 +196,15 @@ class _Linear(torch.autograd.Function):
         ctx.sizes = m, n, k
         ctx.types = (x.dtype, weight.dtype, None if bias is None else bias.dtype, grad_dtype)
         need_x, need_w = ctx.needs_input_grad[:2]
-        kept_x = kept_w = None
         if m == 0:
             return x.new_empty(0, n)
-        lib = _lib.lib()
-        if need_w:
-            kept_x = mx.scratch(lib.aeisu_linear_kept_bytes(m, k, 1), device)
-        if need_x:
-            kept_w = mx.scratch(lib.aeisu_linear_kept_bytes(n, k, mx.BLOCK), device)
-        ctx.save_for_backward(kept_x, kept_w)
-        return _forward(x, weight, bias, kept_x, kept_w, device.index)
+        size_x = mx.kept_bytes(m, k, 1) if need_w else 0
+        size_w = mx.kept_bytes(n, k, mx.BLOCK) if need_x else 0
+        kept = mx.scratch(size_x + size_w, device)
+        ctx.save_for_backward(kept)
+        ctx.places = (0 if need_w else None, size_x if need_x else None)
+        at = kept.data_ptr()
+        return _forward(x, weight, bias, at if need_w else None, at + size_x if need_x else None, device.index)
 
     @staticmethod
     @once_differentiable
@@ -219,12 +217,14 @@ class _Linear(torch.autograd.Function):
         gb = new((n,), dtype=b_type, device=device) if need_b else None
         if m == 0:
             return gx, gw, gb, None
-        kept_x, kept_w = ctx.saved_tensors
+        (kept,) = ctx.saved_tensors
+        at = kept.data_ptr()
+        kept_x, kept_w = (None if p is None else at + p for p in ctx.places)
         grad, mg = _rows(grad)
         size = mx.linear_bytes(m, n, k, 2, device.index)
         ws = mx.scratch(size, device)
         _lib.check(_lib.lib().aeisu_linear_backward(
-            mg, k, mx.TYPES[grad_dtype], *(v for t in (kept_x, kept_w) for v in (None if t is None else t.data_ptr(),)),
+            mg, k, mx.TYPES[grad_dtype], kept_x, kept_w,
             *(v for t in (gx, gw, gb) for v in ((None, 0) if t is None else (t.data_ptr(), mx.TYPES[t.dtype]))),
             ws.data_ptr(), size, device.index, mx.stream(device.index)))
         return gx, gw, gb, None
@@ -262,7 +262,7 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
         y = _forward(flat, weight, ready, None, None, index)
     else:
         m, device = flat.shape[0], flat.device
-        y = torch.empty((m, n), dtype=x.dtype, device=device)
+        y = flat.new_empty((m, n))
         size = mx.linear_bytes(m, n, k, 0, index)
         ws = mx.scratch(size, device)
         (flat, mat), (codes, mw) = _rows(flat), weight.matrix()

@@ -35,12 +35,14 @@ struct ScaleRef {
     long long batch_stride;
 };
 
+// `sums` (null, or with t_codes and single rows): the column sums of every 128 rows, [row blocks][cols].
 void block_quantize(const MatrixRef& x, int block_rows, int code_type, void* codes, long long ld,
                     long long batch_stride, uint8_t* scales, void* t_codes, long long t_ld, long long t_batch_stride,
-                    uint8_t* t_scales, int device, cudaStream_t stream);
+                    uint8_t* t_scales, float* sums, int device, cudaStream_t stream);
 
 // out[c] = sum over rows of x[r][c], added in 32 bits in a fixed order; `partial` holds
 // column_sum_partials(rows, cols) floats.
+void join_sums(const float* partial, int runs, int cols, void* out, int out_type, cudaStream_t stream);
 size_t column_sum_partials(int rows, int cols);
 void column_sum(const MatrixRef& x, void* out, int out_type, float* partial, int device, cudaStream_t stream);
 

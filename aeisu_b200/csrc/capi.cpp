@@ -311,7 +311,7 @@ int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, const aeisu_matr
                               codes->batch_stride, const_cast<uint8_t*>(codes->scales),
                               t_codes ? const_cast<void*>(t_codes->data) : nullptr, t_codes ? t_codes->ld : 0,
                               t_codes ? t_codes->batch_stride : 0,
-                              t_codes ? const_cast<uint8_t*>(t_codes->scales) : nullptr, device,
+                              t_codes ? const_cast<uint8_t*>(t_codes->scales) : nullptr, nullptr, device,
                               static_cast<cudaStream_t>(stream));
     });
 }

@@ -155,7 +155,7 @@ struct QuantJob {
     uint8_t* t_codes;          // codes of the transpose [batch][cols][rows], or null
     long long t_ld, t_batch;
     uint8_t* t_scales;         // [batch][row blocks of 128][col blocks or cols]
-    int tiles;
+    float* sums;               // column sums of each 128 rows [row blocks][cols], or null
 };
 
 // The product that reads the codes may start its set-up now; it waits for this kernel's end.
@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
     __shared__ P col_max[8][kBlock / kPer];
     __shared__ __align__(16) float col_inv[kBlock];
     __shared__ uint8_t row_s[kBlock];
+    __shared__ float col_sum[TILE_SCALE || !BOTH ? 1 : 8][kBlock];
     __shared__ float tile_max[8];
     __shared__ __align__(16) uint32_t turn[BOTH ? kBlock * 32 : 4];
     let_dependents_start();
@@ -240,6 +241,17 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
         if (r < j.rows) {
             load8<T, VEC>(v[i], 0, x + r * j.ld, c0 + oct * 8, j.cols);
             load8<T, VEC>(v[i], 1, x + r * j.ld, c0 + 64 + oct * 8, j.cols);
+        }
+    }
+    if constexpr (!TILE_SCALE && BOTH) {
+        if (j.sums) {   // of the values as they are, infinities too
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                float s = (v[0].get(k) + v[1].get(k)) + (v[2].get(k) + v[3].get(k));
+                s += __shfl_xor_sync(~0u, s, 8);
+                s += __shfl_xor_sync(~0u, s, 16);
+                if (sub == 0) col_sum[warp][(k >> 3) * 64 + oct * 8 + (k & 7)] = s;
+            }
         }
     }
     float amax[4];
@@ -289,7 +301,15 @@ __global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
             for (int w = 1; w < 8; ++w) m = larger<T>(m, col_max[w][c / kPer]);
             const uint32_t s = scale_of<E5M2>(kPer == 2 && (c & 1) ? second_of<T>(m) : first_of<T>(larger<T>(m, m)));
             col_inv[c] = inverse_scale(s);
-            if (c0 + c < j.cols) j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * j.cols + c0 + c] = uint8_t(s);
+            if (c0 + c < j.cols) {
+                j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * j.cols + c0 + c] = uint8_t(s);
+                if (j.sums) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 8; ++w) t += col_sum[w][c];
+                    j.sums[size_t(rb) * j.cols + c0 + c] = t;
+                }
+            }
         }
     }
     uint8_t* codes = j.codes + blockIdx.y * j.codes_batch;
@@ -368,8 +388,10 @@ __global__ void __launch_bounds__(1024) k_column_join(const float* partial, int 
     __shared__ float sh[32][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = int(blockIdx.x) * 32 + lane;
     float a = 0.f;
-    if (c < cols)
+    if (c < cols) {
+#pragma unroll 8
         for (int r = warp; r < runs; r += 32) a += partial[size_t(r) * cols + c];
+    }
     sh[warp][lane] = a;
     __syncthreads();
     if (warp == 0 && c < cols) {
@@ -402,10 +424,10 @@ void launch_quant(const QuantJob<T>& j, int block_rows, int batch, cudaStream_t 
 
 template <typename T>
 void quantize_as(const MatrixRef& x, int block_rows, int code_type, void* codes, long long ld, long long batch_stride,
-                 uint8_t* scales, void* t_codes, long long t_ld, long long t_batch, uint8_t* t_scales,
+                 uint8_t* scales, void* t_codes, long long t_ld, long long t_batch, uint8_t* t_scales, float* sums,
                  cudaStream_t stream) {
     QuantJob<T> j{static_cast<const T*>(x.ptr), x.rows, x.cols, x.ld, x.batch_stride, static_cast<uint8_t*>(codes), ld,
-                  batch_stride, scales, static_cast<uint8_t*>(t_codes), t_ld, t_batch, t_scales, 0};
+                  batch_stride, scales, static_cast<uint8_t*>(t_codes), t_ld, t_batch, t_scales, sums};
     constexpr int n = Vals<T>::n;
     const bool vec = aligned(x.ptr, 16) && x.ld % n == 0 && x.cols % n == 0 && (x.batch == 1 || x.batch_stride % n == 0);
     if (code_type == kE5M2) {
@@ -421,7 +443,8 @@ void quantize_as(const MatrixRef& x, int block_rows, int code_type, void* codes,
 
 void block_quantize(const MatrixRef& x, int block_rows, int code_type, void* codes, long long ld,
                     long long batch_stride, uint8_t* scales, void* t_codes, long long t_ld, long long t_batch_stride,
-                    uint8_t* t_scales, int device, cudaStream_t stream) {
+                    uint8_t* t_scales, float* sums, int device, cudaStream_t stream) {
+    require(!sums || (t_codes && block_rows == 1 && x.batch == 1), "column sums come with the codes of the transpose");
     require(x.ptr && codes && scales && (!t_codes || t_scales), "tensor pointer is null");
     require(x.rows >= 1 && x.cols >= 1 && x.batch >= 1 && x.batch <= 65535 && x.ld >= x.cols && !x.trans,
             "matrix sizes are out of range");
@@ -434,12 +457,24 @@ void block_quantize(const MatrixRef& x, int block_rows, int code_type, void* cod
     OnDevice on(device);
     auto go = [&](auto t) {
         quantize_as<decltype(t)>(x, block_rows, code_type, codes, ld, batch_stride, scales, t_codes, t_ld,
-                                 t_batch_stride, t_scales, stream);
+                                 t_batch_stride, t_scales, sums, stream);
     };
     if (x.type == kF32) go(float{});
     else if (x.type == kF16) go(__half{});
     else if (x.type == kBF16) go(__nv_bfloat16{});
     else fail(AEISU_ERR_INVALID_ARG, "values must be float32, float16 or bfloat16");
+}
+
+void join_sums(const float* partial, int runs, int cols, void* out, int out_type, cudaStream_t stream) {
+    auto join = [&](auto t) {
+        using T = decltype(t);
+        k_column_join<T><<<unsigned((cols + 31) / 32), 1024, 0, stream>>>(partial, runs, cols, static_cast<T*>(out));
+    };
+    if (out_type == kF32) join(float{});
+    else if (out_type == kF16) join(__half{});
+    else if (out_type == kBF16) join(__nv_bfloat16{});
+    else fail(AEISU_ERR_INVALID_ARG, "sums must be float32, float16 or bfloat16");
+    AEISU_CUDA(cudaGetLastError());
 }
 
 size_t column_sum_partials(int rows, int cols) {
@@ -462,20 +497,12 @@ void column_sum(const MatrixRef& x, void* out, int out_type, float* partial, int
         else
             k_column_runs<T, false><<<grid, kThreads, 0, stream>>>(p, x.rows, x.cols, x.ld, run, partial);
     };
-    auto join = [&](auto t) {
-        using T = decltype(t);
-        k_column_join<T><<<unsigned((x.cols + 31) / 32), 1024, 0, stream>>>(partial, runs, x.cols, static_cast<T*>(out));
-    };
     if (x.type == kF32) in(float{});
     else if (x.type == kF16) in(__half{});
     else if (x.type == kBF16) in(__nv_bfloat16{});
     else fail(AEISU_ERR_INVALID_ARG, "values must be float32, float16 or bfloat16");
     AEISU_CUDA(cudaGetLastError());
-    if (out_type == kF32) join(float{});
-    else if (out_type == kF16) join(__half{});
-    else if (out_type == kBF16) join(__nv_bfloat16{});
-    else fail(AEISU_ERR_INVALID_ARG, "sums must be float32, float16 or bfloat16");
-    AEISU_CUDA(cudaGetLastError());
+    join_sums(partial, runs, x.cols, out, out_type, stream);
 }
 
 }  // namespace aeisu

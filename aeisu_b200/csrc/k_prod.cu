@@ -78,8 +78,9 @@ struct ProdJob {
     int split, steps_per_split;  // the contraction in `split` parts:
     int cluster;                 //   of the CTAs of a cluster, joined in its shared memory (split > 1), or (1)
     long long split_stride;      //   each to its own partial output
-    int out_vec;                 // rows of out start on 16-byte boundaries
+    int out_vec;                 // rows of out start on 32-byte boundaries
     int zero_outside, zero_rows;
+    int early_a;                 // A is older than the kernel before (see after_quantize)
     int after_quantize;          // starts while the quantiser of its float operand still runs; the other
                                  // operand and the offsets are older
 };
@@ -455,16 +456,15 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The warp's 32 rows by W columns to out[p][q]: runs of 64 bytes turn through shared memory, so that
-// four lanes store one row's run.  Its 16-byte pieces are exclusive-or'ed with the row pair: no bank
-// conflicts either way.  Where rows do not start on 16-byte boundaries, or columns end, elements are
-// stored one by one, neighbouring lanes at neighbouring addresses.  (Straight-line code with few
-// instructions per run: with element-wise conversions and addresses a run of 32 columns took 1,350 cycles.)
+// The warp's 32 rows by W columns to out[p][q].  Each lane stores its row, 32 bytes at a time: whole
+// sectors, no exchange between lanes.  (Turned through shared memory, so that four lanes store a run of 64
+// bytes, each run of 32 columns took a chain of 800 cycles.)  Where rows do not start on 32-byte
+// boundaries, or columns end, runs of 64 bytes do turn through shared memory, and elements are stored one
+// by one, neighbouring lanes at neighbouring addresses.
 template <typename T, int W>
 __device__ __forceinline__ void write_rows(const ProdJob& j, uint32_t* v, const float* bias, uint8_t* turn,
                                            long long base, int p0, int p1, int q0, int q1) {
-    constexpr int kRun = 64 / sizeof(T) < W ? 64 / sizeof(T) : W, kPieces = kRun * sizeof(T) / 16;
-    constexpr int kWords = kRun * sizeof(T) / 4;      // of a row's run
+    constexpr int kRun = 64 / sizeof(T) < W ? 64 / sizeof(T) : W, kWords = kRun * sizeof(T) / 4;
     const int lane = threadIdx.x & 31;
     if (j.bias) {
 #pragma unroll
@@ -480,40 +480,36 @@ __device__ __forceinline__ void write_rows(const ProdJob& j, uint32_t* v, const 
 #pragma unroll
         for (int i = 0; i < W / 2; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
     }
-    uint8_t* put = turn + lane * 64;
-    const int turned = (lane >> 1) & (kPieces - 1);
-    const int row = lane / kPieces, piece = lane % kPieces;
-    const uint8_t* take = turn + row * 64 + ((piece ^ ((row >> 1) & (kPieces - 1))) << 4);
     T* out = static_cast<T*>(j.out) + base;
-    T* dst = out + (p0 + row) * j.out_ld + q0 + piece * int(16 / sizeof(T));
-    const long long down = j.out_ld * (32 / kPieces);
-    const int rows = p1 - p0 - row;                   // this lane stores rows row + i * 32 / kPieces
-    const bool whole = j.out_vec && base % (16 / sizeof(T)) == 0;
+    if (j.out_vec && q0 + W <= q1) {
+        if (p0 + lane < p1) {
+            T* dst = out + (p0 + lane) * j.out_ld + q0;
+#pragma unroll
+            for (int i = 0; i < W * int(sizeof(T)) / 4; i += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                             :: "l"(reinterpret_cast<uint32_t*>(dst) + i), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]),
+                                "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+                             : "memory");
+        }
+        return;
+    }
+    uint8_t* put = turn + lane * 64;
+    const int turned = (lane >> 1) & 3;     // 16-byte pieces exclusive-or'ed with the row pair: no bank conflicts
 #pragma unroll
     for (int c = 0; c < W / kRun; ++c) {
         if (q0 + c * kRun < q1) {
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i)
+            for (int i = 0; i < kWords / 4; ++i)
                 *reinterpret_cast<uint4*>(put + ((i ^ turned) << 4)) =
                     make_uint4(v[c * kWords + 4 * i], v[c * kWords + 4 * i + 1], v[c * kWords + 4 * i + 2],
                                v[c * kWords + 4 * i + 3]);
             __syncwarp();
-            if (whole && q0 + (c + 1) * kRun <= q1) {
-                uint4 q[kPieces];
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i)
-                    q[i] = *reinterpret_cast<const uint4*>(take + i * (32 / kPieces) * 64);
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i)
-                    if (i * (32 / kPieces) < rows) *reinterpret_cast<uint4*>(dst + i * down + c * kRun) = q[i];
-            } else {
-#pragma unroll 1
-                for (int at = lane; at < 32 * kRun; at += 32) {
-                    const int r = at / kRun, k = at % kRun, b = k * int(sizeof(T));
-                    if (p0 + r < p1 && q0 + c * kRun + k < q1)
-                        out[(p0 + r) * j.out_ld + q0 + c * kRun + k] = *reinterpret_cast<const T*>(
-                            turn + r * 64 + (((b >> 4) ^ ((r >> 1) & (kPieces - 1))) << 4) + (b & 15));
-                }
+#pragma unroll 4
+            for (int at = lane; at < 32 * kRun; at += 32) {
+                const int r = at / kRun, k = at % kRun, b = k * int(sizeof(T));
+                if (p0 + r < p1 && q0 + c * kRun + k < q1)
+                    out[(p0 + r) * j.out_ld + q0 + c * kRun + k] =
+                        *reinterpret_cast<const T*>(turn + r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15));
             }
             __syncwarp();
         }
@@ -630,6 +626,18 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         uint32_t phase = 0;
         bool ok = true;
         long long issued = 0;
+        // Weights are on their way before the quantiser has ended: A's copies of the first stages.
+        int early = 0;
+        if (CTAS == 1 && j.early_a && first_tile < tiles) {
+            const Tile x = tile_at<BM, BN>(j, g, first_tile, kStep);
+            if (elected())
+                for (int k = x.k0; k < x.k1 && early < S::kStages; k += kStep, ++early) {
+                    mbar_arrive_expect_tx(full + early, S::kStage);
+                    tma_3d<1>(smem_addr(ring) + early * S::kStage, &ma, k, x.p0, j.grouping == kRowsB ? x.e : 0,
+                              smem_addr(full + early));
+                }
+            early = __reduce_max_sync(~0u, early);
+        }
         if (j.after_quantize) grid_dep_wait();
         for (int t = first_tile; ok && t < tiles; t += stride) {
             const Tile x = tile_at<BM, BN>(j, g, t, kStep);
@@ -643,8 +651,11 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     const uint32_t a = smem_addr(ring) + stage * S::kStage, b = a + S::kATile;
                     const uint32_t local = smem_addr(full + stage);
                     const uint32_t bar = CTAS == 1 ? local : address_in(local, own ? rank : 0);
-                    if (own || rank == 0) mbar_arrive_expect_tx(full + stage, own ? S::kStage : S::kStage * CTAS);
-                    if (j.a_mn) {
+                    const bool begun = CTAS == 1 && issued < early;
+                    if (!begun && (own || rank == 0))
+                        mbar_arrive_expect_tx(full + stage, own ? S::kStage : S::kStage * CTAS);
+                    if (begun) {
+                    } else if (j.a_mn) {
                         for (int c = 0; c < kBM / 64; ++c) tma_3d<CTAS>(a + c * 8192, &ma, x.p0 + a_off + c * 64, k, ea, bar);
                     } else {
                         tma_3d<CTAS>(a, &ma, k, x.p0 + a_off, ea, bar);
@@ -1044,6 +1055,7 @@ void launch_shape(TileShape s, const CUtensorMap& a, const CUtensorMap& b, const
         case 16: return launch<FP8, 16, 1>(a, b, j, tiles, device, stream);
         case 32: return launch<FP8, 32, 1>(a, b, j, tiles, device, stream);
         case 64: return launch<FP8, 64, 1>(a, b, j, tiles, device, stream);
+        case 256: return launch<FP8, 256, 1>(a, b, j, tiles, device, stream);
         default: return launch<FP8, 128, 1>(a, b, j, tiles, device, stream);
     }
 }
@@ -1058,8 +1070,8 @@ TileShape choose_tile(long long row_tiles_of_128, int q, long long count, long l
                       int sms) {
     TileShape best{least, 1};
     double time = 0;
-    for (const TileShape s : {TileShape{16, 1}, TileShape{32, 1}, TileShape{64, 1}, TileShape{128, 1}, TileShape{128, 2},
-                              TileShape{256, 2}}) {
+    for (const TileShape s : {TileShape{16, 1}, TileShape{32, 1}, TileShape{64, 1}, TileShape{128, 1}, TileShape{256, 1},
+                              TileShape{128, 2}, TileShape{256, 2}}) {
         if (s.bn < least || (s.ctas == 2 && !pairs)) continue;
         const long long tiles = ceil_div(row_tiles_of_128, s.ctas) * ceil_div(q, s.bn) * count;
         const double t = double(ceil_div(tiles, sms / s.ctas)) *
@@ -1138,7 +1150,7 @@ void lay_tiles(ProdJob& j, TileShape s) {
 }
 
 bool whole_rows(const void* p, int type, long long ld, long long batch) {
-    return aligned(p, 16) && ld * elem_bytes(type) % 16 == 0 && batch * elem_bytes(type) % 16 == 0;
+    return aligned(p, 32) && ld * elem_bytes(type) % 32 == 0 && batch * elem_bytes(type) % 32 == 0;
 }
 
 }  // namespace
@@ -1182,6 +1194,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     j.steps_per_split = pl.steps;
     j.cluster = pl.cluster;
     j.after_quantize = after_quantize;
+    j.early_a = after_quantize && pl.swap && fp8;
     if (pl.split > pl.cluster) {
         j.out = workspace;
         j.out_type = kF32;
@@ -1255,6 +1268,7 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     lay_tiles(j, tile);
     j.split = j.cluster = 1;
     j.after_quantize = after_quantize;
+    j.early_a = after_quantize && swap && fp8;
     j.zero_outside = zero_outside;
     j.zero_rows = x.rows;
     j.out_vec = whole_rows(out.ptr, out.type, out.ld, 0);

@@ -32,10 +32,10 @@ void* codes_of(const Operand& o) { return const_cast<void*>(o.m.ptr); }
 uint8_t* scales_of(const Operand& o) { return const_cast<uint8_t*>(o.s.ptr); }
 
 // Quantises x into `o` and its transpose into `t` (null: not wanted).
-void quantize_into(const MatrixRef& x, int block_rows, const Operand& o, const Operand* t, int device,
+void quantize_into(const MatrixRef& x, int block_rows, const Operand& o, const Operand* t, float* sums, int device,
                    cudaStream_t stream) {
     block_quantize(x, block_rows, o.m.type, codes_of(o), o.m.ld, 0, scales_of(o), t ? codes_of(*t) : nullptr,
-                   t ? t->m.ld : 0, 0, t ? scales_of(*t) : nullptr, device, stream);
+                   t ? t->m.ld : 0, 0, t ? scales_of(*t) : nullptr, sums, device, stream);
 }
 
 void check_workspace(const void* workspace, size_t have, size_t need) {
@@ -52,7 +52,7 @@ size_t linear_workspace(int m, int n, int k, int pass, int device) {
         return operand_bytes(m, k, 1) + operand_bytes(n, k, kBlock) + product_workspace(m, n, k, true, device);
     return operand_bytes(m, n, 1) + operand_bytes(n, m, 1) +
            std::max({product_workspace(m, k, n, true, device), product_workspace(n, k, m, true, device),
-                     column_sum_partials(m, n) * sizeof(float)});
+                     std::max(column_sum_partials(m, n), size_t((m + kBlock - 1) / kBlock) * n) * sizeof(float)});
 }
 
 void linear_serve(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, const ProductOut& out, void* workspace,
@@ -60,7 +60,7 @@ void linear_serve(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, co
     check_workspace(workspace, workspace_bytes, linear_workspace(x.rows, w.rows, x.cols, kServe, device));
     const Operand q = operand_at(workspace, kE4M3, x.rows, x.cols, 1);
     const size_t used = operand_bytes(x.rows, x.cols, 1);
-    quantize_into(x, 1, q, nullptr, device, stream);
+    quantize_into(x, 1, q, nullptr, nullptr, device, stream);
     product(q.m, &q.s, w, &sw, out, static_cast<uint8_t*>(workspace) + used, workspace_bytes - used, true, device, stream);
 }
 
@@ -73,8 +73,8 @@ void linear_train_forward(const MatrixRef& x, const MatrixRef& w, const ProductO
     const Operand r = operand_at(ws, kE4M3, w.rows, w.cols, kBlock);
     ws += operand_bytes(w.rows, w.cols, kBlock);
     const Operand qt = operand_at(kept_x, kE4M3, x.cols, x.rows, 1), rt = operand_at(kept_w, kE4M3, w.cols, w.rows, kBlock);
-    quantize_into(w, kBlock, r, kept_w ? &rt : nullptr, device, stream);
-    quantize_into(x, 1, q, kept_x ? &qt : nullptr, device, stream);
+    quantize_into(w, kBlock, r, kept_w ? &rt : nullptr, nullptr, device, stream);
+    quantize_into(x, 1, q, kept_x ? &qt : nullptr, nullptr, device, stream);
     product(q.m, &q.s, r.m, &r.s, out, ws, workspace_bytes - size_t(ws - static_cast<uint8_t*>(workspace)), true, device,
             stream);
 }
@@ -92,15 +92,22 @@ void linear_train_backward(const MatrixRef& grad, int k, int code_type, const vo
     const Operand gt = operand_at(ws, code_type, n, m, 1);
     ws += operand_bytes(n, m, 1);
     const size_t left = workspace_bytes - size_t(ws - static_cast<uint8_t*>(workspace));
-    if (gb) column_sum(grad, gb, gb_type, reinterpret_cast<float*>(ws), device, stream);
-    if (gx || gw) quantize_into(grad, 1, g, gw ? &gt : nullptr, device, stream);
+    // The bias gradient comes out of the pass that quantises both ways, or has one of its own.
+    float* sums = reinterpret_cast<float*>(ws);
+    if (gb && !gw) column_sum(grad, gb, gb_type, sums, device, stream);
+    if (gx || gw) quantize_into(grad, 1, g, gw ? &gt : nullptr, gb && gw ? sums : nullptr, device, stream);
+    if (gb && gw) {
+        OnDevice on(device);
+        join_sums(sums, (m + kBlock - 1) / kBlock, n, gb, gb_type, stream);
+    }
+    const bool after = !(gb && gw);   // the kernel before the next product is the quantiser
     if (gx) {
         const Operand wt = operand_at(kept_w, kE4M3, k, n, kBlock);
-        product(g.m, &g.s, wt.m, &wt.s, {gx, gx_type, k, nullptr, 0}, ws, left, true, device, stream);
+        product(g.m, &g.s, wt.m, &wt.s, {gx, gx_type, k, nullptr, 0}, ws, left, after, device, stream);
     }
     if (gw) {
         const Operand xt = operand_at(kept_x, kE4M3, k, m, 1);
-        product(gt.m, &gt.s, xt.m, &xt.s, {gw, gw_type, k, nullptr, 0}, ws, left, !gx, device, stream);
+        product(gt.m, &gt.s, xt.m, &xt.s, {gw, gw_type, k, nullptr, 0}, ws, left, after && !gx, device, stream);
     }
 }
 
@@ -110,7 +117,7 @@ void grouped_linear(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, 
                     bool zero_outside, void* workspace, size_t workspace_bytes, int device, cudaStream_t stream) {
     check_workspace(workspace, workspace_bytes, grouped_linear_workspace(x.rows, x.cols));
     const Operand q = operand_at(workspace, kE4M3, x.rows, x.cols, 1);
-    quantize_into(x, 1, q, nullptr, device, stream);
+    quantize_into(x, 1, q, nullptr, nullptr, device, stream);
     grouped_product(q.m, &q.s, w, &sw, off, out, zero_outside, true, device, stream);
 }
 
