@@ -6,13 +6,14 @@
 
 namespace aeisu {
 
-// Makes `dev` current for the scope.
+// Makes `dev` current for the scope.  Set even where it already is: that is what gives a thread that
+// has not used the GPU yet (one of autograd's) the device's context, which tensor maps need.
 struct OnDevice {
     int prev = -1;
     explicit OnDevice(int dev) {
         AEISU_CUDA(cudaGetDevice(&prev));
-        if (prev != dev) AEISU_CUDA(cudaSetDevice(dev));
-        else prev = -1;
+        AEISU_CUDA(cudaSetDevice(dev));
+        if (prev == dev) prev = -1;
     }
     ~OnDevice() {
         if (prev >= 0) cudaSetDevice(prev);

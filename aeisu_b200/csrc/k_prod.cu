@@ -60,6 +60,7 @@ struct Divider {
 
 struct ProdJob {
     Divider by_tiles, by_band, by_tp, by_rest;   // tiles of one part or group, of 16 row tiles; row tiles, of the last band
+    Divider by_lanes;            // CTAs, or pairs of them
     int tp, tq;                  // row tiles of A and B
     int P, Q, K;                 // rows of A, rows of B, contraction (whole sides; per batch entry)
     int grouping, groups;
@@ -78,6 +79,7 @@ struct ProdJob {
     int split, steps_per_split;  // the contraction in `split` parts:
     int cluster;                 //   of the CTAs of a cluster, joined in its shared memory (split > 1), or (1)
     long long split_stride;      //   each to its own partial output
+    int balance;                 // tiles of the groups of a contraction are dealt to the least loaded CTAs
     int out_vec;                 // rows of out start on 32-byte boundaries
     int zero_outside, zero_rows;
     int early_a;                 // A is older than the kernel before (see after_quantize)
@@ -103,7 +105,7 @@ struct Shape {
                                  : kColsUsed <= 256 ? 256 : 512;
     // Writers: one warp per 32 lanes, two where each then has at least 32 columns.
     static constexpr int kHalves = BN >= 64 ? 2 : 1, kWide = BN / kHalves;
-    static constexpr int kBars = 3 * kStages + 4 * kScaleSlots + 2 * kAccs + 1;
+    static constexpr int kBars = 4 * kStages + 4 * kScaleSlots + 2 * kAccs + 1;
     static constexpr int kBarBytes = (kBars * 8 + 15) / 16 * 16;   // what lies behind is read in 16-byte words
     static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kScaleSlots * kScaleBytes + kWriters * kTurn + kBarBytes;
     // Behind it the bias of each writer's columns (dense) or the groups' bounds and tiles.
@@ -274,7 +276,7 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
 
 struct Tile {
     int e;               // batch entry of the grouped operand or output
-    int p0, q0;          // first rows of A and B (absolute)
+    int p0, q0;          // first rows of A and B (absolute); p0 < 0: no tile
     int p1, q1;          // ends of the rows that are stored
     int k0, k1;          // contraction range (absolute)
     int part;            // part of a split contraction
@@ -284,15 +286,17 @@ struct Tile {
 // no smaller than the one before, so that no value of theirs leads out of the tensors.
 struct Groups {
     const int* bound;    // [groups + 1]
-    const int* cum;      // [groups + 1] row tiles before each group, or the groups by falling size
-    __device__ __forceinline__ int order(int i) const { return cum[i]; }
+    const int* cum;      // [groups + 1] row tiles before each group; of a contraction the groups by falling size
+    const int* dealt;    // [groups] tile of each group (in that order) dealt to this CTA beside full rounds, or -1
+    int lane;            // this CTA or pair among all
 };
 
 constexpr int kBand = 16;   // row tiles of a band
 
 __device__ __forceinline__ int tile_count(const ProdJob& j, const Groups& g) {
     if (j.grouping == kDense) return j.tp * j.tq * j.split;
-    if (j.grouping == kContraction) return j.tp * j.tq * j.groups;
+    if (j.grouping == kContraction)
+        return j.balance ? (j.by_lanes.quotient(int(j.by_tiles.d)) + 1) * j.groups : j.tp * j.tq * j.groups;
     return g.cum[j.groups] * (j.grouping == kRowsA ? j.tq : j.tp);
 }
 
@@ -313,13 +317,23 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
         x.k0 = x.part * j.steps_per_split * step;
         x.k1 = min(j.K, x.k0 + j.steps_per_split * step);
     } else if (j.grouping == kContraction) {
-        // Groups from the longest to the shortest, in turns that run to and fro over the CTAs: the time of a
-        // tile goes by the rows of its group.
-        const int lanes = int(gridDim.x) * kBM / BM, turn = t / lanes;
-        if ((turn & 1) && j.tp * j.tq * j.groups - turn * lanes >= lanes) t = turn * lanes + lanes - 1 - (t - turn * lanes);
-        const int i = j.by_tiles.quotient(t);
-        x.e = g.order(i);
-        t -= i * int(j.by_tiles.d);
+        // Groups from the longest to the shortest: the time of a tile goes by the rows of its group.
+        int i;
+        if (j.balance) {
+            // Entry t of this CTA (or pair): full rounds of a group's tiles, then the one dealt to it, if any.
+            const int per = j.by_lanes.quotient(int(j.by_tiles.d)) + 1;
+            i = t / per;
+            const int round = t - i * per;
+            t = round < per - 1 ? round * int(j.by_lanes.d) + g.lane : g.dealt[i];
+            if (t < 0) {
+                x.p0 = -1;
+                return x;
+            }
+        } else {
+            i = j.by_tiles.quotient(t);
+            t -= i * int(j.by_tiles.d);
+        }
+        x.e = g.cum[i];
         const int col = j.by_tp.quotient(t);
         x.p0 = (t - col * j.tp) * BM;
         x.q0 = col * BN;
@@ -545,7 +559,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     uint64_t* full = reinterpret_cast<uint64_t*>(turns + kWriters * kTurn);
     uint64_t* empty = full + S::kStages;
     uint64_t* fixed = empty + S::kStages;
-    uint64_t* scales_full = fixed + S::kStages;
+    uint64_t* landed = fixed + S::kStages;
+    uint64_t* scales_full = landed + S::kStages;
     uint64_t* scales_empty = scales_full + kScaleSlots;
     uint64_t* scales_here = scales_empty + kScaleSlots;
     uint64_t* scales_there = scales_here + kScaleSlots;
@@ -564,6 +579,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
             mbar_init(fixed + i, CTAS);
+            mbar_init(landed + i, 1);
         }
         for (int i = 0; i < kScaleSlots; ++i) {
             mbar_init(scales_full + i, 1);
@@ -578,31 +594,77 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         mbar_init(drain, 1);
         fence_mbar_init();
     }
-    const Groups g{bound, cum};
+    int* dealt = cum + j.groups + 1;
+    const Groups g{bound, cum, dealt, int(blockIdx.x) / CTAS};
     if (j.grouping != kDense) {
         const int rows = j.grouping == kContraction ? j.K : j.grouping == kRowsA ? j.P : j.Q;
         const int high = j.grouping == kRowsB ? BN : BM;
-        for (int i = threadIdx.x; i <= j.groups; i += kThreads) bound[i] = min(max(j.off[i], 0), rows);
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int tiles = 0;
-            cum[0] = 0;
-            for (int i = 0; i < j.groups; ++i) {
-                bound[i + 1] = max(bound[i + 1], bound[i]);
-                tiles += (bound[i + 1] - bound[i] + high - 1) / high;
-                cum[i + 1] = tiles;
+        if (warp == 0) {
+            // Bounds made rising and tiles added up, 32 groups at a time.
+            int low = 0, tiles = 0;
+            for (int i = 0; i <= j.groups; i += 32) {
+                int b = i + lane <= j.groups ? min(max(j.off[i + lane], 0), rows) : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(~0u, b, d);
+                    if (lane >= d) b = max(b, o);
+                }
+                b = max(b, low);
+                const int before = __shfl_up_sync(~0u, b, 1);
+                // tiles of the group that ends at this bound
+                int n = i + lane == 0 ? 0 : (b - (lane ? before : low) + high - 1) / high;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(~0u, n, d);
+                    if (lane >= d) n += o;
+                }
+                if (i + lane <= j.groups) {
+                    bound[i + lane] = b;
+                    cum[i + lane] = tiles + n;
+                }
+                low = __shfl_sync(~0u, b, 31);
+                tiles += __shfl_sync(~0u, n, 31);
             }
         }
         if (j.grouping == kContraction) {
             __syncthreads();
             for (int i = threadIdx.x; i < j.groups; i += kThreads) {
-                const int size = bound[i + 1] - bound[i];
-                int at = 0;
-                for (int o = 0; o < j.groups; ++o) {
-                    const int other = bound[o + 1] - bound[o];
-                    at += other > size || (other == size && o < i);
+                int at = i;
+                if (j.balance) {
+                    const int size = bound[i + 1] - bound[i];
+                    at = 0;
+                    for (int o = 0; o < j.groups; ++o) {
+                        const int other = bound[o + 1] - bound[o];
+                        at += other > size || (other == size && o < i);
+                    }
                 }
                 cum[at] = i;
+            }
+            if (j.balance) {
+                // The tiles of a group that do not make a full round go to the CTAs with the least to do so far,
+                // longest groups first.  (With groups of 100 to 5,000 rows the longest CTA had 1.5 times the mean.)
+                // A CTA's load and number make one key, so that a rank is a count of smaller keys.
+                const int lanes = int(j.by_lanes.d), left = int(j.by_tiles.d) % lanes, padded = (lanes + 3) / 4;
+                int* load = reinterpret_cast<int*>((reinterpret_cast<uintptr_t>(dealt + j.groups) + 15) & ~uintptr_t(15));
+                for (int i = threadIdx.x; i < 4 * padded; i += kThreads) load[i] = i < lanes ? i : 0x7fffffff;
+                for (int i = 0; i < j.groups; ++i) {
+                    __syncthreads();
+                    int mine = 0, at = 0;
+                    if (int(threadIdx.x) < lanes) {
+                        mine = load[threadIdx.x];
+#pragma unroll 8
+                        for (int o = 0; o < padded; ++o) {
+                            const int4 k = reinterpret_cast<const int4*>(load)[o];
+                            at += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+                        }
+                        if (int(threadIdx.x) == g.lane)
+                            dealt[i] = at < left ? int(j.by_tiles.d) - left + at : -1;
+                    }
+                    __syncthreads();
+                    // a tile costs its steps, and starting and ending it about as much as four
+                    if (int(threadIdx.x) < lanes && at < left)
+                        load[threadIdx.x] = mine + (((bound[cum[i] + 1] - bound[cum[i]]) / kStep + 4) << 9);
+                }
             }
         }
     }
@@ -612,10 +674,11 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
     const int tiles = tile_count(j, g);
-    const int first_tile = CTAS == 2       ? int(blockIdx.x) / 2
+    const int first_tile = j.balance       ? 0
+                           : CTAS == 2     ? int(blockIdx.x) / 2
                            : j.cluster > 1 ? rank * (tiles / j.split) + int(blockIdx.x) / j.cluster
                                            : int(blockIdx.x);
-    const int stride = CTAS == 2 ? int(gridDim.x) / 2 : j.cluster > 1 ? tiles : int(gridDim.x);
+    const int stride = j.balance ? 1 : CTAS == 2 ? int(gridDim.x) / 2 : j.cluster > 1 ? tiles : int(gridDim.x);
     const int a_off = CTAS == 2 ? rank * kBM : 0, b_off = CTAS == 2 ? rank * S::kBRows : 0;
 
     // Warps 0 and 1 run their loops as whole warps and elect a lane for the copies and MMAs only: addresses
@@ -641,19 +704,24 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         if (j.after_quantize) grid_dep_wait();
         for (int t = first_tile; ok && t < tiles; t += stride) {
             const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+            if (x.p0 < 0) continue;
             const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
             for (int k = x.k0; k < x.k1; k += kStep) {
                 if (!(ok = __all_sync(~0u, wait(empty + stage, phase ^ 1)))) break;
-                // A pair's copies all count on its first CTA's barrier; where rows have to be zeroed first,
-                // each CTA's on its own.
-                const bool own = CTAS == 1 || (j.grouping == kContraction && k + kStep > x.k1);
+                // A pair's copies all count on its first CTA's barrier.  Where rows have to be zeroed first, each
+                // CTA's count on a barrier of its own, and the stage's barrier passes at once.
+                const bool tail = j.grouping == kContraction && k + kStep > x.k1;
                 if (elected()) {
                     const uint32_t a = smem_addr(ring) + stage * S::kStage, b = a + S::kATile;
-                    const uint32_t local = smem_addr(full + stage);
-                    const uint32_t bar = CTAS == 1 ? local : address_in(local, own ? rank : 0);
+                    uint64_t* counted = (tail ? landed : full) + stage;
+                    const uint32_t bar = CTAS == 1 ? smem_addr(counted) : address_in(smem_addr(counted), tail ? rank : 0);
                     const bool begun = CTAS == 1 && issued < early;
-                    if (!begun && (own || rank == 0))
-                        mbar_arrive_expect_tx(full + stage, own ? S::kStage : S::kStage * CTAS);
+                    if (tail) {
+                        mbar_arrive_expect_tx(landed + stage, S::kStage);
+                        if (CTAS == 1 || rank == 0) mbar_arrive(full + stage);
+                    } else if (!begun && (CTAS == 1 || rank == 0)) {
+                        mbar_arrive_expect_tx(full + stage, S::kStage * CTAS);
+                    }
                     if (begun) {
                     } else if (j.a_mn) {
                         for (int c = 0; c < kBM / 64; ++c) tma_3d<CTAS>(a + c * 8192, &ma, x.p0 + a_off + c * 64, k, ea, bar);
@@ -689,6 +757,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             const uint64_t desc_b = j.b_mn ? desc_mnmajor(first_b) : desc_kmajor(first_b);
             for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+                if (x.p0 < 0) continue;
                 if (!(ok = __all_sync(~0u, wait(acc_empty + acc, acc_phase ^ 1)))) break;
                 const uint32_t d = tmem + acc * BN;
                 uint32_t byte = 0;
@@ -800,7 +869,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             if (t < tiles) load(x, k);
             int slot = warp - 2;
             for (bool more = t < tiles; more;) {
-                if (!wait(scales_empty + slot, phase ^ 1)) break;
+                if (!__all_sync(~0u, wait(scales_empty + slot, phase ^ 1))) break;
                 uint8_t* dst = scales + slot * S::kScaleBytes;
                 store_scales(raw_a, way_a, dst);
 #pragma unroll
@@ -809,7 +878,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 __syncwarp();
                 // The first CTA's warp also takes in the other one's word, an acquire of cluster scope that would
                 // cost the MMA warp 480 cycles per group.
-                if (CTAS == 2 && rank == 0 && !wait_all<CTAS>(scales_there + slot, phase)) break;
+                if (CTAS == 2 && rank == 0 && !__all_sync(~0u, wait_all<CTAS>(scales_there + slot, phase))) break;
                 if (lane == 0) mbar_arrive((rank == 0 || CTAS == 1 ? scales_full : scales_here) + slot);
                 if ((slot += 2) >= kScaleSlots) slot -= kScaleSlots, phase ^= 1;
                 advance();
@@ -818,16 +887,17 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 if (more) load(x, k);
             }
         } else if (j.grouping == kContraction) {
-            uint32_t own_phase = 0;   // of the barriers of a pair's second CTA, which only these steps use
+            // (This warp waits on barriers that only these steps use: it is no part of the ring's flow, so a
+            // barrier that every step passes could run two phases ahead of it.)
+            uint32_t landed_phase = 0;
             for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+                if (x.p0 < 0) continue;
                 for (int k = x.k0; k < x.k1; k += kStep) {
                     const int rows = x.k1 - k;
-                    // (A phase may be waited for only in turn: the first CTA's barriers see every step.)
-                    if (rank == 0 && !(ok = wait(full + stage, phase))) break;
                     if (rows < kStep) {
-                        if (rank == 1 && !(ok = wait(full + stage, (own_phase >> stage) & 1))) break;
-                        own_phase ^= 1u << stage;
+                        if (!(ok = __all_sync(~0u, wait(landed + stage, (landed_phase >> stage) & 1)))) break;
+                        landed_phase ^= 1u << stage;
                         uint8_t* base = ring + stage * S::kStage;
                         const int tail = (kStep - rows) * 8;   // 16-byte pieces per chunk
                         for (int i = lane; i < tail * (S::kStage / 8192); i += 32)
@@ -837,7 +907,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                         __syncwarp();
                         if (lane == 0) arrive_first<CTAS>(fixed + stage, rank, true);
                     }
-                    if (++stage == S::kStages) stage = 0, phase ^= 1;
+                    if (++stage == S::kStages) stage = 0;
                 }
             }
         }
@@ -849,13 +919,14 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         uint32_t acc_phase = 0;
         for (int t = first_tile; t < tiles; t += stride) {
             const Tile x = tile_at<BM, BN>(j, g, t, kStep);
+            if (x.p0 < 0) continue;
             if (j.bias && !j.swapped && bias_q != x.q0) {
                 for (int i = lane; i < S::kWide; i += 32)
                     bias[i] = x.q0 + col + i < j.Q ? load_elem(j.bias, j.bias_type, x.q0 + col + i) : 0.f;
                 __syncwarp();
                 bias_q = x.q0;
             }
-            if (!wait(acc_full + acc, acc_phase)) break;
+            if (!__all_sync(~0u, wait(acc_full + acc, acc_phase))) break;
             fence_after_sync();
             uint32_t v[S::kWide];
             if (x.k0 < x.k1) {
@@ -1006,7 +1077,9 @@ void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long l
     using S = Shape<FP8, BN, CTAS>;
     constexpr size_t most = S::kSmem + std::max(S::kBias, 2 * (kMaxGroups + 1) * sizeof(int));
     static_assert(most <= 227 * 1024, "shared memory of a CTA");
-    const size_t smem = S::kSmem + (j.grouping == kDense ? S::kBias : 2 * size_t(j.groups + 1) * sizeof(int));
+    const size_t lists = j.balance ? size_t(j.groups + j.by_lanes.d + 8) : 0;
+    const size_t smem = S::kSmem + (j.grouping == kDense ? S::kBias : (2 * size_t(j.groups + 1) + lists) * sizeof(int));
+    require(smem <= most, "too many groups");
     static std::mutex mu;
     static bool ready[64] = {};
     const int sms = sm_count(device);
@@ -1310,6 +1383,11 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     j.split = j.cluster = 1;
     j.out_vec = whole_rows(out, out_type, j.out_ld, j.out_batch);
     const long long tiles = ceil_div(g.rows, tile.rows()) * ceil_div(x.rows, tile.bn) * groups;
+    // Dealing takes about 300 cycles per group; it is left out where groups are many (and short) or all tiles run
+    // at once.
+    const int lanes = sm_count(device) / tile.ctas;
+    j.by_lanes = divider(lanes);
+    j.balance = groups <= 64 && tiles > lanes && lanes <= kThreads;
     require(tiles < (1LL << 30), "matrix is too large");
     launch_shape<false>(tile, operand_map(g, 64), operand_map(x, 64), j, tiles, device, stream);
 }

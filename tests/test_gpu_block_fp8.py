@@ -1,13 +1,24 @@
 """Block-scaled FP8 quantisation, products and the linear layer (aeisu_b200.block_fp8) against the
 plain 64-bit forms of tests/block_oracle.py.  Codes and scales are compared bit for bit; products
 within the bounds derived there."""
+import ctypes as C
+
 import pytest
 import torch
 
 import block_oracle as O
-from aeisu_b200 import block_fp8 as B
+from aeisu_b200 import _lib, block_fp8 as B
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    code = C.c_int(-1)
+    _lib.check(_lib.lib().aeisu_product_status(0, C.byref(code)))
+    assert code.value == 0
+
 E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
 HALVES = [torch.bfloat16, torch.float16]
 

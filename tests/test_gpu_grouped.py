@@ -1,12 +1,23 @@
 """Products grouped by expert (aeisu_b200.grouped) against plain 64-bit loops over the groups."""
+import ctypes as C
+
 import pytest
 import torch
 
 import block_oracle as O
-from aeisu_b200 import block_fp8 as B
+from aeisu_b200 import _lib, block_fp8 as B
 from aeisu_b200.grouped import grouped_matmul
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    code = C.c_int(-1)
+    _lib.check(_lib.lib().aeisu_product_status(0, C.byref(code)))
+    assert code.value == 0
+
 HALVES = [torch.bfloat16, torch.float16]
 
 
@@ -194,6 +205,34 @@ def test_graph_replays_with_other_bounds():
         graph.replay()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("sizes", [[2048] * 8, [512] * 32, [0, 4992, 512, 1472, 9408], [4992, 517, 1472, 9403]], ids=str)
+def test_weight_gradient_of_long_groups(sizes):
+    # hundreds of steps without a partial one, and between partial ones
+    t, off = sum(sizes), bounds(sizes)
+    x, g = randn(t, 1024), randn(t, 512, seed=1)
+    w = torch.zeros(len(sizes), 512, 1024, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    first = None
+    for _ in range(10):
+        (dw,) = torch.autograd.grad(grouped_matmul(x, w, off), w, g)
+        first = dw if first is None else first
+        assert torch.equal(dw, first)
+    for i, (lo, hi) in enumerate(spans(off)):
+        a, b = g[lo:hi].double().t(), x[lo:hi].double()
+        terms, want = (a.abs() @ b.abs()).cpu(), (a @ b).cpu()
+        acc = (hi - lo + 1) * 2.0 ** -23 * terms
+        O.check(first[i], want, acc + O.half_step(want.abs() + acc, torch.bfloat16))
+
+
+def test_first_call_in_a_new_thread():
+    # a thread without a CUDA context of its own, as autograd's
+    from concurrent.futures import ThreadPoolExecutor
+    x, w, off = randn(8, 64), randn(2, 32, 64), bounds([3, 5])
+    with ThreadPoolExecutor(1) as pool:
+        y = pool.submit(grouped_matmul, x, w, off).result()
+    torch.cuda.synchronize()
+    assert torch.equal(y, grouped_matmul(x, w, off))
 
 
 def test_refusals_on_the_gpu():
