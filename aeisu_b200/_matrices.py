@@ -25,15 +25,14 @@ def stream(index):
 
 def need_cuda(name, *tensors):
     """All tensors on one CUDA device; its index."""
-    first = tensors[0].device
-    if first.type != "cuda":
-        raise ValueError(f"{name} needs CUDA tensors (there is no CPU path)")
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError(f"{name} needs CUDA tensors (there is no CPU path)")
+    index = tensors[0].get_device()
     for t in tensors[1:]:
-        if t.device != first:
-            if not t.is_cuda:
-                raise ValueError(f"{name} needs CUDA tensors (there is no CPU path)")
+        if t.get_device() != index:
             raise ValueError(f"{name}: the tensors must be on one device")
-    return first.index
+    return index
 
 
 def row_stride(t):
@@ -98,5 +97,5 @@ def kept_bytes(rows, cols, block_rows):
     return _lib.lib().aeisu_linear_kept_bytes(rows, cols, block_rows)
 
 
-def scratch(size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device)
+def scratch(size, like):
+    return like.new_empty(size, dtype=torch.uint8)

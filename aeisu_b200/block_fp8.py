@@ -26,6 +26,8 @@ captured into a CUDA graph.  float64 is refused rather than computed at a lower 
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -33,6 +35,8 @@ from . import _lib
 from . import _matrices as mx
 
 _E8M0 = torch.float8_e8m0fnu
+_call = _lib.lib
+_new = object.__new__
 
 
 class BlockFP8:
@@ -85,20 +89,28 @@ class BlockFP8:
         return f"BlockFP8({list(self.codes.shape)}, {self.codes.dtype}, rows={self.rows}, {self.codes.device})"
 
 
-def _empty(shape, rows, dtype, device):
-    codes = mx.empty_rows(shape, dtype, device)
-    scales = torch.empty((*shape[:-2], mx.blocks(shape[-1]), -(-shape[-2] // rows)), dtype=_E8M0, device=device)
-    q = BlockFP8.__new__(BlockFP8)
-    q.codes, q.scales, q.rows = codes, scales, rows
-    return q
+@functools.lru_cache(maxsize=4096)
+def _sizes(shape, rows, dtype):
+    """(row stride of the codes, shape of the codes' storage, shape of the scales)."""
+    *lead, r, c = shape
+    ld = -(-c // 16) * 16
+    return ld, (*lead, r, ld), (*lead, mx.blocks(c), -(-r // rows))
 
 
-def _out(q):
-    return mx.matrix(q.codes, -(-q.codes.shape[-1] // 16) * 16, q.scales, q.rows)
+def _empty(x, shape, rows, dtype):
+    """(uninitialised BlockFP8 beside x, its aeisu_matrix)."""
+    ld, stored, scaled = _sizes(shape, rows, dtype)
+    q = _new(BlockFP8)
+    codes = x.new_empty(stored, dtype=dtype)
+    q.codes = codes if ld == shape[-1] else codes[..., :shape[-1]]
+    q.scales = x.new_empty(scaled, dtype=_E8M0)
+    q.rows = rows
+    return q, mx.matrix(q.codes, ld, q.scales, rows)
 
 
 def _quantize(x, rows, dtype, both):
-    if x.dim() not in (2, 3) or x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) not in (2, 3) or shape[-1] == 0:
         raise ValueError("Expected values [R, C] or [E, R, C]")
     if rows not in (1, mx.BLOCK):
         raise ValueError("blocks have 1 or 128 rows")
@@ -107,18 +119,18 @@ def _quantize(x, rows, dtype, both):
     if x.dtype not in mx.FLOATS:
         raise TypeError(f"quantize takes float32, float16 or bfloat16; got {x.dtype}")
     index = mx.need_cuda("quantize", x)
-    if both and x.shape[-2] == 0:
-        raise ValueError("Expected values with at least one row")
     ld = mx.row_stride(x)
     if ld is None:
         x = x.detach().contiguous()
-        ld = x.shape[-1]
-    device = x.device
-    q = _empty(x.shape, rows, dtype, device)
-    t = _empty((*x.shape[:-2], x.shape[-1], x.shape[-2]), rows, dtype, device) if both else None
+        ld = shape[-1]
+    q, mq = _empty(x, tuple(shape), rows, dtype)
+    t = mt = None
+    if both:
+        if shape[-2] == 0:
+            raise ValueError("Expected values with at least one row")
+        t, mt = _empty(x, (*shape[:-2], shape[-1], shape[-2]), rows, dtype)
     if x.numel():
-        _lib.check(_lib.lib().aeisu_block_quantize(mx.matrix(x, ld), rows, _out(q), None if t is None else _out(t), index,
-                                                   mx.stream(index)))
+        _lib.check(_call().aeisu_block_quantize(mx.matrix(x, ld), rows, mq, mt, index, mx.stream(index)))
     return q, t
 
 
@@ -154,14 +166,13 @@ def matmul(a, b, *, bias=None, dtype=torch.bfloat16):
     (m, k), n = a.shape, b.shape[0]
     bias = _bias(bias, n)
     index = mx.need_cuda("matmul", a.codes, b.codes, *(() if bias is None else (bias,)))
-    device = a.codes.device
-    out = torch.empty((m, n), dtype=dtype, device=device)
+    out = a.codes.new_empty((m, n), dtype=dtype)
     if m == 0 or n == 0:
         return out
     (ka, ma), (kb, mb) = a.matrix(), b.matrix()
     size = mx.product_bytes(m, n, k, 1, index)
-    ws = mx.scratch(size, device) if size else None
-    _lib.check(_lib.lib().aeisu_product(ma, mb, None if bias is None else bias.data_ptr(),
+    ws = mx.scratch(size, out) if size else None
+    _lib.check(_call().aeisu_product(ma, mb, None if bias is None else bias.data_ptr(),
                                         0 if bias is None else mx.TYPES[bias.dtype], mx.matrix(out, n),
                                         None if ws is None else ws.data_ptr(), size, index, mx.stream(index)))
     return out
@@ -178,12 +189,12 @@ def _rows(x):
 
 def _forward(x, weight, bias, kept_x, kept_w, index):
     """The layer on float x and weight, leaving the transposed codes at the addresses kept_x and kept_w."""
-    (m, k), n, device = x.shape, weight.shape[0], x.device
+    (m, k), n = x.shape, weight.shape[0]
     out = x.new_empty((m, n))
     size = mx.linear_bytes(m, n, k, 1, index)
-    ws = mx.scratch(size, device)
+    ws = mx.scratch(size, out)
     (x, mat), (weight, mw) = _rows(x), _rows(weight)
-    _lib.check(_lib.lib().aeisu_linear_forward(
+    _lib.check(_call().aeisu_linear_forward(
         mat, mw, None if bias is None else bias.data_ptr(), 0 if bias is None else mx.TYPES[bias.dtype],
         mx.matrix(out, n), kept_x, kept_w, ws.data_ptr(), size, index, mx.stream(index)))
     return out
@@ -192,7 +203,7 @@ def _forward(x, weight, bias, kept_x, kept_w, index):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, grad_dtype):
-        (m, k), n, device = x.shape, weight.shape[0], x.device
+        (m, k), n = x.shape, weight.shape[0]
         ctx.sizes = m, n, k
         ctx.types = (x.dtype, weight.dtype, None if bias is None else bias.dtype, grad_dtype)
         need_x, need_w = ctx.needs_input_grad[:2]
@@ -200,33 +211,33 @@ class _Linear(torch.autograd.Function):
             return x.new_empty(0, n)
         size_x = mx.kept_bytes(m, k, 1) if need_w else 0
         size_w = mx.kept_bytes(n, k, mx.BLOCK) if need_x else 0
-        kept = mx.scratch(size_x + size_w, device)
+        kept = mx.scratch(size_x + size_w, x)
         ctx.save_for_backward(kept)
         ctx.places = (0 if need_w else None, size_x if need_x else None)
         at = kept.data_ptr()
-        return _forward(x, weight, bias, at if need_w else None, at + size_x if need_x else None, device.index)
+        return _forward(x, weight, bias, at if need_w else None, at + size_x if need_x else None, x.get_device())
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         x_type, w_type, b_type, grad_dtype = ctx.types
-        (m, n, k), (need_x, need_w, need_b, _), device = ctx.sizes, ctx.needs_input_grad, grad.device
-        new = torch.zeros if m == 0 else torch.empty
-        gx = new((m, k), dtype=x_type, device=device) if need_x else None
-        gw = new((n, k), dtype=w_type, device=device) if need_w else None
-        gb = new((n,), dtype=b_type, device=device) if need_b else None
+        (m, n, k), (need_x, need_w, need_b, _), index = ctx.sizes, ctx.needs_input_grad, grad.get_device()
+        new = grad.new_zeros if m == 0 else grad.new_empty
+        gx = new((m, k), dtype=x_type) if need_x else None
+        gw = new((n, k), dtype=w_type) if need_w else None
+        gb = new((n,), dtype=b_type) if need_b else None
         if m == 0:
             return gx, gw, gb, None
         (kept,) = ctx.saved_tensors
         at = kept.data_ptr()
         kept_x, kept_w = (None if p is None else at + p for p in ctx.places)
         grad, mg = _rows(grad)
-        size = mx.linear_bytes(m, n, k, 2, device.index)
-        ws = mx.scratch(size, device)
-        _lib.check(_lib.lib().aeisu_linear_backward(
+        size = mx.linear_bytes(m, n, k, 2, index)
+        ws = mx.scratch(size, grad)
+        _lib.check(_call().aeisu_linear_backward(
             mg, k, mx.TYPES[grad_dtype], kept_x, kept_w,
             *(v for t in (gx, gw, gb) for v in ((None, 0) if t is None else (t.data_ptr(), mx.TYPES[t.dtype]))),
-            ws.data_ptr(), size, device.index, mx.stream(device.index)))
+            ws.data_ptr(), size, index, mx.stream(index)))
         return gx, gw, gb, None
 
 
@@ -261,12 +272,12 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
     elif not serving:
         y = _forward(flat, weight, ready, None, None, index)
     else:
-        m, device = flat.shape[0], flat.device
+        m = flat.shape[0]
         y = flat.new_empty((m, n))
         size = mx.linear_bytes(m, n, k, 0, index)
-        ws = mx.scratch(size, device)
+        ws = mx.scratch(size, flat)
         (flat, mat), (codes, mw) = _rows(flat), weight.matrix()
-        _lib.check(_lib.lib().aeisu_linear(mat, mw, None if ready is None else ready.data_ptr(),
+        _lib.check(_call().aeisu_linear(mat, mw, None if ready is None else ready.data_ptr(),
                                            0 if ready is None else mx.TYPES[ready.dtype], mx.matrix(y, n), ws.data_ptr(),
                                            size, index, mx.stream(index)))
     return y if len(shape) == 2 else y.reshape(*shape[:-1], n)

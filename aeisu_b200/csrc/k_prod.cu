@@ -79,7 +79,7 @@ struct ProdJob {
     int split, steps_per_split;  // the contraction in `split` parts:
     int cluster;                 //   of the CTAs of a cluster, joined in its shared memory (split > 1), or (1)
     long long split_stride;      //   each to its own partial output
-    int balance;                 // tiles of the groups of a contraction are dealt to the least loaded CTAs
+    int balance;                 // tiles of unequal groups of a contraction are dealt to the least loaded CTAs
     int out_vec;                 // rows of out start on 32-byte boundaries
     int zero_outside, zero_rows;
     int early_a;                 // A is older than the kernel before (see after_quantize)
@@ -289,14 +289,16 @@ struct Groups {
     const int* cum;      // [groups + 1] row tiles before each group; of a contraction the groups by falling size
     const int* dealt;    // [groups] tile of each group (in that order) dealt to this CTA beside full rounds, or -1
     int lane;            // this CTA or pair among all
+    bool deal;           // tiles go by `dealt`
 };
 
+constexpr int kDealGroups = 64;   // groups that are sorted and dealt at most
 constexpr int kBand = 16;   // row tiles of a band
 
 __device__ __forceinline__ int tile_count(const ProdJob& j, const Groups& g) {
     if (j.grouping == kDense) return j.tp * j.tq * j.split;
     if (j.grouping == kContraction)
-        return j.balance ? (j.by_lanes.quotient(int(j.by_tiles.d)) + 1) * j.groups : j.tp * j.tq * j.groups;
+        return g.deal ? (j.by_lanes.quotient(int(j.by_tiles.d)) + 1) * j.groups : j.tp * j.tq * j.groups;
     return g.cum[j.groups] * (j.grouping == kRowsA ? j.tq : j.tp);
 }
 
@@ -319,7 +321,7 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
     } else if (j.grouping == kContraction) {
         // Groups from the longest to the shortest: the time of a tile goes by the rows of its group.
         int i;
-        if (j.balance) {
+        if (g.deal) {
             // Entry t of this CTA (or pair): full rounds of a group's tiles, then the one dealt to it, if any.
             const int per = j.by_lanes.quotient(int(j.by_tiles.d)) + 1;
             i = t / per;
@@ -553,7 +555,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     constexpr int BM = kBM * CTAS;
     extern __shared__ uint8_t raw[];
     __shared__ uint32_t tmem_slot;
-    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    // (Aligned by an offset, not by a cast of the address, which would turn every access generic.)
+    uint8_t* ring = raw + (-smem_addr(raw) & 1023u);
     uint8_t* scales = ring + S::kStages * S::kStage;
     uint8_t* turns = scales + kScaleSlots * S::kScaleBytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(turns + kWriters * kTurn);
@@ -595,7 +598,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         fence_mbar_init();
     }
     int* dealt = cum + j.groups + 1;
-    const Groups g{bound, cum, dealt, int(blockIdx.x) / CTAS};
+    Groups g{bound, cum, dealt, int(blockIdx.x) / CTAS, false};
     if (j.grouping != kDense) {
         const int rows = j.grouping == kContraction ? j.K : j.grouping == kRowsA ? j.P : j.Q;
         const int high = j.grouping == kRowsB ? BN : BM;
@@ -630,7 +633,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             __syncthreads();
             for (int i = threadIdx.x; i < j.groups; i += kThreads) {
                 int at = i;
-                if (j.balance) {
+                if (j.groups <= kDealGroups) {
                     const int size = bound[i + 1] - bound[i];
                     at = 0;
                     for (int o = 0; o < j.groups; ++o) {
@@ -640,30 +643,40 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 }
                 cum[at] = i;
             }
-            if (j.balance) {
-                // The tiles of a group that do not make a full round go to the CTAs with the least to do so far,
-                // longest groups first.  (With groups of 100 to 5,000 rows the longest CTA had 1.5 times the mean.)
+            __syncthreads();
+            // The tiles of a group that do not make a full round go to the CTAs with the least to do so far,
+            // longest groups first.  That takes about 1,300 cycles per group, and pays where the longest
+            // group is far above the mean: 16 groups of 0 to 5,000 of 16,384 rows, 1,024 x 2,048, 85 -> 78 us; 16
+            // equal groups, 55 -> 64 us.
+            const int longest = bound[cum[0] + 1] - bound[cum[0]];
+            g.deal = j.balance && 2LL * longest * j.groups > 3LL * (bound[j.groups] - bound[0]);
+            if (g.deal) {
                 // A CTA's load and number make one key, so that a rank is a count of smaller keys.
                 const int lanes = int(j.by_lanes.d), left = int(j.by_tiles.d) % lanes, padded = (lanes + 3) / 4;
-                int* load = reinterpret_cast<int*>((reinterpret_cast<uintptr_t>(dealt + j.groups) + 15) & ~uintptr_t(15));
-                for (int i = threadIdx.x; i < 4 * padded; i += kThreads) load[i] = i < lanes ? i : 0x7fffffff;
+                const int share = lanes <= kThreads / 4 ? 4 : 2;        // threads that count for one key
+                const int own = int(threadIdx.x) / share, sub = int(threadIdx.x) % share;
+                int* load = dealt + j.groups + (-smem_addr(dealt + j.groups) & 15u) / 4;
+                for (int i = threadIdx.x; i < 8 * padded; i += kThreads)
+                    load[i] = i % (4 * padded) < lanes ? i % (4 * padded) : 0x7fffffff;
                 for (int i = 0; i < j.groups; ++i) {
                     __syncthreads();
-                    int mine = 0, at = 0;
-                    if (int(threadIdx.x) < lanes) {
-                        mine = load[threadIdx.x];
-#pragma unroll 8
-                        for (int o = 0; o < padded; ++o) {
-                            const int4 k = reinterpret_cast<const int4*>(load)[o];
-                            at += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
-                        }
-                        if (int(threadIdx.x) == g.lane)
-                            dealt[i] = at < left ? int(j.by_tiles.d) - left + at : -1;
-                    }
-                    __syncthreads();
+                    const int* now = load + (i & 1) * 4 * padded;
+                    int* then = load + (~i & 1) * 4 * padded;
                     // a tile costs its steps, and starting and ending it about as much as four
-                    if (int(threadIdx.x) < lanes && at < left)
-                        load[threadIdx.x] = mine + (((bound[cum[i] + 1] - bound[cum[i]]) / kStep + 4) << 9);
+                    const int cost = ((bound[cum[i] + 1] - bound[cum[i]]) / kStep + 4) << 9;
+                    const int mine = own < lanes ? now[own] : 0;
+                    int at = 0;
+#pragma unroll 5
+                    for (int o = sub; o < padded; o += share) {
+                        const int4 k = reinterpret_cast<const int4*>(now)[o];
+                        at += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+                    }
+                    at += __shfl_xor_sync(~0u, at, 1);
+                    if (share == 4) at += __shfl_xor_sync(~0u, at, 2);
+                    if (own < lanes && sub == 0) {
+                        then[own] = mine + (at < left ? cost : 0);
+                        if (own == g.lane) dealt[i] = at < left ? int(j.by_tiles.d) - left + at : -1;
+                    }
                 }
             }
         }
@@ -674,11 +687,11 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
     const int tiles = tile_count(j, g);
-    const int first_tile = j.balance       ? 0
+    const int first_tile = g.deal          ? 0
                            : CTAS == 2     ? int(blockIdx.x) / 2
                            : j.cluster > 1 ? rank * (tiles / j.split) + int(blockIdx.x) / j.cluster
                                            : int(blockIdx.x);
-    const int stride = j.balance ? 1 : CTAS == 2 ? int(gridDim.x) / 2 : j.cluster > 1 ? tiles : int(gridDim.x);
+    const int stride = g.deal ? 1 : CTAS == 2 ? int(gridDim.x) / 2 : j.cluster > 1 ? tiles : int(gridDim.x);
     const int a_off = CTAS == 2 ? rank * kBM : 0, b_off = CTAS == 2 ? rank * S::kBRows : 0;
 
     // Warps 0 and 1 run their loops as whole warps and elect a lane for the copies and MMAs only: addresses
@@ -898,11 +911,12 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     if (rows < kStep) {
                         if (!(ok = __all_sync(~0u, wait(landed + stage, (landed_phase >> stage) & 1)))) break;
                         landed_phase ^= 1u << stage;
-                        uint8_t* base = ring + stage * S::kStage;
-                        const int tail = (kStep - rows) * 8;   // 16-byte pieces per chunk
-                        for (int i = lane; i < tail * (S::kStage / 8192); i += 32)
-                            *reinterpret_cast<uint4*>(base + (i / tail) * 8192 + rows * 128 + (i % tail) * 16) =
-                                make_uint4(0, 0, 0, 0);
+                        // eight lanes to a row of 128 bytes
+                        uint8_t* at = ring + stage * S::kStage + (lane & 7) * 16;
+#pragma unroll
+                        for (int c = 0; c < S::kStage / 8192; ++c)
+                            for (int r = rows + (lane >> 3); r < kStep; r += 4)
+                                *reinterpret_cast<uint4*>(at + c * 8192 + r * 128) = make_uint4(0, 0, 0, 0);
                         fence_async_smem();
                         __syncwarp();
                         if (lane == 0) arrive_first<CTAS>(fixed + stage, rank, true);
@@ -1077,7 +1091,7 @@ void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long l
     using S = Shape<FP8, BN, CTAS>;
     constexpr size_t most = S::kSmem + std::max(S::kBias, 2 * (kMaxGroups + 1) * sizeof(int));
     static_assert(most <= 227 * 1024, "shared memory of a CTA");
-    const size_t lists = j.balance ? size_t(j.groups + j.by_lanes.d + 8) : 0;
+    const size_t lists = j.balance ? size_t(j.groups + 2 * j.by_lanes.d + 16) : 0;
     const size_t smem = S::kSmem + (j.grouping == kDense ? S::kBias : (2 * size_t(j.groups + 1) + lists) * sizeof(int));
     require(smem <= most, "too many groups");
     static std::mutex mu;
@@ -1383,11 +1397,9 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     j.split = j.cluster = 1;
     j.out_vec = whole_rows(out, out_type, j.out_ld, j.out_batch);
     const long long tiles = ceil_div(g.rows, tile.rows()) * ceil_div(x.rows, tile.bn) * groups;
-    // Dealing takes about 300 cycles per group; it is left out where groups are many (and short) or all tiles run
-    // at once.
     const int lanes = sm_count(device) / tile.ctas;
     j.by_lanes = divider(lanes);
-    j.balance = groups <= 64 && tiles > lanes && lanes <= kThreads;
+    j.balance = groups <= kDealGroups && tiles > lanes && lanes <= kThreads / 2;
     require(tiles < (1LL << 30), "matrix is too large");
     launch_shape<false>(tile, operand_map(g, 64), operand_map(x, 64), j, tiles, device, stream);
 }

@@ -37,7 +37,7 @@ def _weights(weight):
 
 def _product(x, weight, offsets, out, zero_outside):
     """x, weight: (tensors kept, aeisu_matrix)."""
-    index = out.device.index
+    index = out.get_device()
     _lib.check(_lib.lib().aeisu_grouped_product(x[1], weight[1], offsets.data_ptr(), zero_outside,
                                                 mx.matrix(out, mx.row_stride(out)), index, mx.stream(index)))
     return out
@@ -52,7 +52,7 @@ class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
         ctx.save_for_backward(x, weight, offsets)
-        out = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=x.device)
+        out = x.new_empty((x.shape[0], weight.shape[1]))
         if x.shape[0] == 0:
             return out
         return _product(_rows(x), _weights(weight), offsets, out, True)
@@ -66,12 +66,12 @@ class _Grouped(torch.autograd.Function):
         g = _rows(grad)
         gx = gw = None
         if ctx.needs_input_grad[0]:
-            gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            gx = x.new_empty(x.shape)
             _product(g, _weights(weight.transpose(1, 2)), offsets, gx, True)
         if ctx.needs_input_grad[1]:
-            gw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+            gw = weight.new_empty(weight.shape)
             kept = _rows(x)
-            index = gw.device.index
+            index = gw.get_device()
             _lib.check(_lib.lib().aeisu_grouped_weight_gradient(g[1], kept[1], offsets.data_ptr(), weight.shape[0],
                                                                 gw.data_ptr(), mx.TYPES[gw.dtype], index,
                                                                 mx.stream(index)))
@@ -114,10 +114,9 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
         if fp8 or out is not None:
             raise ValueError("FP8 weights and out serve without gradients")
         return _Grouped.apply(x, weight, offsets.contiguous())
-    device = offsets.device
     new = out is None
     if new:
-        out = torch.empty((t, n), dtype=dtype, device=device)
+        out = offsets.new_empty((t, n), dtype=dtype)
     if t == 0:
         return out
     offsets = offsets.contiguous()
@@ -131,7 +130,7 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
         x = x.detach().contiguous()
         ld = k
     size = _lib.lib().aeisu_grouped_linear_workspace(t, k)
-    ws, (codes, mw) = mx.scratch(size, device), weight.matrix()
+    ws, (codes, mw) = mx.scratch(size, x), weight.matrix()
     _lib.check(_lib.lib().aeisu_grouped_linear(mx.matrix(x, ld), mw, offsets.data_ptr(), new,
                                                mx.matrix(out, mx.row_stride(out)), ws.data_ptr(), size, index,
                                                mx.stream(index)))
