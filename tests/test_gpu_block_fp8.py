@@ -261,6 +261,75 @@ def test_graph_capture_replays_with_new_inputs():
             assert torch.equal(a, b)
 
 
+def test_linear_mixed_types_and_strides():
+    # activations in bfloat16 with a float32 master weight and a strided bias, everything a view
+    x = randn(70, 300, dtype=torch.bfloat16)[:, 3:203].requires_grad_()
+    w = randn(200, 130, seed=1).t().requires_grad_()
+    b = randn(260, seed=2)[::2].requires_grad_()
+    g = randn(130, 70, seed=3).bfloat16().t()
+    y = B.linear(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
+    assert y.dtype == gx.dtype == torch.bfloat16 and gw.dtype == gb.dtype == torch.float32
+    O.check_product(y, O.values(x.detach()), O.values(w.detach(), 128), b.detach())
+    O.check_product(gx, O.values(g), O.values(w.detach().t(), 128))
+    O.check_product(gw, O.values(g.t()), O.values(x.detach().t()))
+    assert torch.equal(gb, torch.autograd.grad(B.linear(x, w, b), b, g)[0])
+
+
+def test_linear_e5m2_gradients():
+    x, w = (randn(*s, seed=i).requires_grad_() for i, s in enumerate(((150, 96), (72, 96))))
+    g = randn(150, 72, seed=2) * torch.exp2(torch.randint(-20, 20, (150, 1), generator=torch.Generator().manual_seed(0))).cuda()
+    gx, gw = torch.autograd.grad(B.linear(x, w, grad_dtype=E5), (x, w), g)
+    O.check_product(gx, O.values(g, dtype=E5), O.values(w.detach().t(), 128))
+    O.check_product(gw, O.values(g.t(), dtype=E5), O.values(x.detach().t()))
+
+
+def test_infinite_gradients_reach_the_bias_as_they_are():
+    x, w, b = randn(200, 64), randn(32, 64, seed=1).requires_grad_(), randn(32, seed=2).requires_grad_()
+    g = randn(200, 32, seed=3)
+    g[7, 3], g[150, 4], g[1, 5], g[2, 5] = float("inf"), float("nan"), float("inf"), -float("inf")
+    gw, gb = torch.autograd.grad(B.linear(x, w, b), (w, b), g)
+    assert torch.equal(gb.isnan(), g.sum(0).isnan()) and torch.equal(gb.isinf(), g.sum(0).isinf())
+    assert torch.equal(gw.isnan().any(1), torch.isin(torch.arange(32), torch.tensor([3, 4, 5])).cuda())
+
+
+def test_more_than_two_to_the_31_elements():
+    rows, k = 270_000, 8192
+    x = torch.empty(rows, k, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w = B.quantize(randn(24, k, seed=2), rows=128)
+    q, t = B.quantize_both(x)
+    ends = (slice(0, 100), slice(rows - 100, rows))
+    for s in ends:
+        part = B.quantize(x[s])
+        assert torch.equal(q.codes[s].view(torch.uint8), part.codes.view(torch.uint8))
+        assert torch.equal(q.scales[:, s].view(torch.uint8), part.scales.view(torch.uint8))
+    last = x[rows // 128 * 128:]        # the last block of the transpose, which starts on a multiple of 128
+    lt = B.quantize(last.t())
+    assert torch.equal(t.codes[:, rows // 128 * 128:].view(torch.uint8), lt.codes.view(torch.uint8))
+    assert torch.equal(t.scales[-1].view(torch.uint8), lt.scales[0].view(torch.uint8))
+    y = B.matmul(q, w, dtype=torch.float32)
+    for s in ends:
+        O.check_product(y[s], q.codes[s].double().cpu() * q.scales[:, s].float().t().repeat_interleave(128, 1).double().cpu(),
+                        w.dequantize())
+
+
+def test_two_streams_at_once():
+    a, b = randn(1500, 1024, dtype=torch.bfloat16), randn(900, 2048, seed=1, dtype=torch.bfloat16)
+    wa, wb = randn(700, 1024, seed=2, dtype=torch.bfloat16), randn(512, 2048, seed=3, dtype=torch.bfloat16)
+    want = B.linear(a, wa), B.linear(b, wb)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for s, x, w, o in ((streams[0], a, wa, got[0]), (streams[1], b, wb, got[1])):
+            with torch.cuda.stream(s):
+                o.append(B.linear(x, w))
+    torch.cuda.synchronize()
+    for o, w in zip(got, want):
+        assert all(torch.equal(v, w) for v in o)
+
+
 def test_refusals_on_the_gpu():
     x, w = randn(4, 64, dtype=torch.bfloat16), randn(32, 64, seed=1, dtype=torch.bfloat16)
     kept = B.quantize(w, rows=128)

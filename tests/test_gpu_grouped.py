@@ -235,6 +235,15 @@ def test_first_call_in_a_new_thread():
     assert torch.equal(y, grouped_matmul(x, w, off))
 
 
+def test_output_of_more_than_two_to_the_31_elements():
+    t, n, k = 140_000, 16384, 64
+    off = torch.tensor([0, 70_001, t], dtype=torch.int32).cuda()
+    x, w = randn(t, k), randn(2, n, k, seed=1)
+    y = grouped_matmul(x, w, off)
+    for lo, hi, e in ((0, 50, 0), (69_980, 70_001, 0), (70_001, 70_030, 1), (t - 50, t, 1)):
+        O.check_product(y[lo:hi], x[lo:hi], w[e])
+
+
 def test_refusals_on_the_gpu():
     x, w, off = randn(8, 64), randn(2, 32, 64), bounds([3, 5])
     with pytest.raises(ValueError, match="without gradients"):
