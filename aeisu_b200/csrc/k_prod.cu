@@ -210,13 +210,6 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float peer_float(uint32_t saddr, uint32_t rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}\n"
-                 : "=f"(v) : "r"(saddr), "r"(rank) : "memory");
-    return v;
-}
-
 __device__ __forceinline__ uint32_t address_in(uint32_t saddr, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
@@ -542,6 +535,43 @@ __device__ __forceinline__ void write_columns(const ProdJob& j, const uint32_t* 
 #pragma unroll
     for (int c = 0; c < W; ++c)
         if (q0 + c < q1) out[(q0 + c) * j.out_ld + p] = rounded<T>(__uint_as_float(v[c]) + b);
+}
+
+// The parts of a tile, one in the shared memory of each of the cluster's CTAs as [column][128 rows],
+// added in their order; each CTA takes its share of the columns, a thread four rows at a time, with the
+// loads of all parts and of two columns under way at once.
+template <int BN, int PARTS>
+__device__ __forceinline__ void join_cluster(const ProdJob& j, const Tile& x, int rank, uint32_t tile) {
+    constexpr int kShare = BN / PARTS, kAtOnce = 32 * kWriters / 32;   // columns; 32 threads for each
+    const int t = threadIdx.x - 128, r4 = (t & 31) * 4, p = x.p0 + r4;
+    uint32_t part[PARTS];
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) part[i] = address_in(tile, i);
+    float pb[4] = {};
+    if (j.bias && j.swapped)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p + i < x.p1) pb[i] = load_elem(j.bias, j.bias_type, p + i);
+#pragma unroll 2
+    for (int c = t >> 5; c < kShare; c += kAtOnce) {
+        const int col = rank * kShare + c, q = x.q0 + col;
+        if (q >= x.q1) continue;
+        float4 v[PARTS];
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[i].x), "=f"(v[i].y), "=f"(v[i].z), "=f"(v[i].w)
+                         : "r"(part[i] + uint32_t(col * kBM + r4) * 4) : "memory");
+        float4 s = v[0];
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) s.x += v[i].x, s.y += v[i].y, s.z += v[i].z, s.w += v[i].w;
+        const float qb = j.bias && !j.swapped ? load_elem(j.bias, j.bias_type, q) : 0.f;
+        const float o[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p + i < x.p1)
+                store_elem(j.out, j.out_type, j.swapped ? q * j.out_ld + p + i : (p + i) * j.out_ld + q, o[i] + qb + pb[i]);
+    }
 }
 
 // ---- the kernel --------------------------------------------------------------------------------
@@ -987,21 +1017,13 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         }
     }
     if (CTAS == 1 && j.cluster > 1) {
-        // The parts are added in their order, each CTA taking its share of the columns.
         __syncwarp();
         cluster_sync();
-        if (warp >= 4 && warp < 8 && first_tile < tiles) {
+        if (warp >= 4 && first_tile < tiles) {
             const Tile x = tile_at<BM, BN>(j, g, first_tile, kStep);
-            const int row = threadIdx.x - 128, p = x.p0 + row, share = BN / j.cluster;
-            const float pb = j.bias && j.swapped && p < x.p1 ? load_elem(j.bias, j.bias_type, p) : 0.f;
-            for (int c = rank * share; c < (rank + 1) * share; ++c) {
-                const int q = x.q0 + c;
-                if (p >= x.p1 || q >= x.q1) continue;
-                float v = 0.f;
-                for (int r = 0; r < j.cluster; ++r) v += peer_float(smem_addr(ring) + (c * kBM + row) * 4, r);
-                if (j.swapped) store_elem(j.out, j.out_type, q * j.out_ld + p, v + pb);
-                else store_elem(j.out, j.out_type, p * j.out_ld + q, v + (j.bias ? load_elem(j.bias, j.bias_type, q) : 0.f));
-            }
+            if (j.cluster == 2) join_cluster<BN, 2>(j, x, rank, smem_addr(ring));
+            else if (j.cluster == 4) join_cluster<BN, 4>(j, x, rank, smem_addr(ring));
+            else join_cluster<BN, 8>(j, x, rank, smem_addr(ring));
         }
     }
     fence_before_sync();
