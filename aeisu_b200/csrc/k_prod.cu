@@ -2,7 +2,7 @@
 // dense, with the rows of one side grouped by expert, or with the contraction grouped by expert.
 //
 // One persistent, warp-specialised kernel.  A tile is 128 x BN of the output, taken by one CTA, or
-// 256 x BN, taken by a pair of CTAs (cta_group::2): each holds 128 rows of A and of the accumulator and
+// 256 x 256, taken by a pair of CTAs (cta_group::2): each holds 128 rows of A and of the accumulator and
 // half of B's rows, so that a pair reads and stages B once.  Per step of 128 bytes of the contraction,
 // warp 0 copies the operands' tiles by TMA into a ring of 128-byte swizzled stages, warp 1 (of the
 // pair's first CTA) issues four MMAs into FP32 accumulators in TMEM, warps 4..11 write the finished tile
@@ -1156,10 +1156,7 @@ struct TileShape {
 template <bool FP8>
 void launch_shape(TileShape s, const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long long tiles, int device,
                   cudaStream_t stream) {
-    if (s.ctas == 2) {
-        if (s.bn == 256) return launch<FP8, 256, 2>(a, b, j, tiles, device, stream);
-        return launch<FP8, 128, 2>(a, b, j, tiles, device, stream);
-    }
+    if (s.ctas == 2) return launch<FP8, 256, 2>(a, b, j, tiles, device, stream);
     switch (s.bn) {
         case 16: return launch<FP8, 16, 1>(a, b, j, tiles, device, stream);
         case 32: return launch<FP8, 32, 1>(a, b, j, tiles, device, stream);
@@ -1180,7 +1177,7 @@ TileShape choose_tile(long long row_tiles_of_128, int q, long long count, long l
     TileShape best{least, 1};
     double time = 0;
     for (const TileShape s : {TileShape{16, 1}, TileShape{32, 1}, TileShape{64, 1}, TileShape{128, 1}, TileShape{256, 1},
-                              TileShape{128, 2}, TileShape{256, 2}}) {
+                              TileShape{256, 2}}) {
         if (s.bn < least || (s.ctas == 2 && !pairs)) continue;
         const long long tiles = ceil_div(row_tiles_of_128, s.ctas) * ceil_div(q, s.bn) * count;
         const double t = double(ceil_div(tiles, sms / s.ctas)) *
@@ -1347,12 +1344,13 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     ProdJob j{};
     const MatrixRef& A = swap ? b : x;
     const MatrixRef& B = swap ? x : b;
-    // Rows per group are known on the GPU only: full row tiles are counted as if groups were even, and a
-    // pair's 256 rows taken where groups have as many on average.
+    // Rows per group are known on the GPU only: full row tiles are counted as if groups were even.  Pairs, whose
+    // rows are twice as high, where groups have three of theirs on average (16-bit, 16 groups of 1,024 rows,
+    // 1,024 x 2,048: 58 us in pairs, 66 us without; FP8, 8 groups of about 512, 2,048 x 2,048: 30 and 25 us).
     const int steps = int(ceil_div((long long)x.cols * elem_bytes(x.type), kStepBytes));
     const TileShape tile =
         swap ? choose_tile(ceil_div(b.rows, kBM) * b.batch, mean, 1, steps, false, 16, sm_count(device))
-             : choose_tile(ceil_div(mean, kBM) * b.batch, b.rows, 1, steps, mean >= 2 * kBM, b.trans ? 64 : 16,
+             : choose_tile(ceil_div(mean, kBM) * b.batch, b.rows, 1, steps, mean >= 6 * kBM, b.trans ? 64 : 16,
                            sm_count(device));
     j.P = A.rows;
     j.Q = B.rows;
