@@ -64,10 +64,6 @@ template <> __device__ __forceinline__ float second_of<__nv_bfloat16>(uint32_t p
 template <> __device__ __forceinline__ float first_of<__half>(uint32_t p) { return number_or_zero(__low2float(*reinterpret_cast<const __half2*>(&p))); }
 template <> __device__ __forceinline__ float second_of<__half>(uint32_t p) { return number_or_zero(__high2float(*reinterpret_cast<const __half2*>(&p))); }
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-
 // Eight consecutive values of a row, to places 8 h .. of v; columns at or past `cols` read as zero.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(Vals<T>& v, int h, const T* row, int c, int cols) {
@@ -162,22 +158,26 @@ struct QuantJob {
 __device__ __forceinline__ void let_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // One scale per row and block column, no transpose.  Eight lanes share a block (two loads of eight
-// values each), a warp takes four neighbouring blocks of four rows, a CTA 32 rows of them; the
-// scales leave through shared memory as 32 contiguous bytes per block column.
-template <typename T, bool E5M2, bool VEC>
+// values each), a warp takes CB neighbouring blocks of 4 / CB rows at a time, four times, a CTA 128 of these
+// blocks; the scales leave through shared memory as contiguous bytes of a block column.  CB is 4 where
+// rows are long, so that a warp reads whole runs of them; fewer leave no lane idle on short rows (165,888 x 128
+// bfloat16: 29 us with 4).
+template <typename T, bool E5M2, bool VEC, int CB>
 __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
-    __shared__ uint8_t sh[4][32];
+    constexpr int kRows = kBlock / CB;
+    __shared__ uint8_t sh[CB][kRows];
     let_dependents_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col_groups = (j.cols + 4 * kBlock - 1) / (4 * kBlock);
-    const int r0 = int(blockIdx.x / col_groups) * 32, c0 = int(blockIdx.x % col_groups) * 4 * kBlock;
+    const int col_groups = (j.cols + CB * kBlock - 1) / (CB * kBlock);
+    const int r0 = int(blockIdx.x / col_groups) * kRows, c0 = int(blockIdx.x % col_groups) * CB * kBlock;
     const T* x = j.x + blockIdx.y * j.batch_stride;
     uint8_t* codes = j.codes + blockIdx.y * j.codes_batch;
-    const int c = c0 + (lane >> 3) * kBlock + (lane & 7) * 16;
+    const int b = (lane >> 3) % CB, c = c0 + b * kBlock + (lane & 7) * 16;
+    const int first = warp * (kRows / 8) + (lane >> 3) / CB;   // rows first + i * 4 / CB
     Vals<T> v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int r = r0 + warp * 4 + i;
+        const int r = r0 + first + i * (4 / CB);
         v[i] = {};
         if (r < j.rows) {
             load8<T, VEC>(v[i], 0, x + r * j.ld, c, j.cols);
@@ -186,13 +186,13 @@ __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int r = r0 + warp * 4 + i;
+        const int r = r0 + first + i * (4 / CB);
         float amax = finite_max(v[i]);
 #pragma unroll
         for (int d = 1; d < 8; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, d));
         const uint32_t s = scale_of<E5M2>(amax);
         const float inv = inverse_scale(s);
-        if ((lane & 7) == 0) sh[lane >> 3][warp * 4 + i] = uint8_t(s);
+        if ((lane & 7) == 0) sh[b][first + i * (4 / CB)] = uint8_t(s);
         if (r < j.rows && c < j.cols) {
             uint4 q;
             uint32_t* w = reinterpret_cast<uint32_t*>(&q);
@@ -204,10 +204,10 @@ __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
         }
     }
     __syncthreads();
-    if (threadIdx.x < 128) {
-        const int b = threadIdx.x >> 5, r = r0 + lane, col_blocks = (j.cols + kBlock - 1) / kBlock;
-        if (r < j.rows && c0 / kBlock + b < col_blocks)
-            j.scales[(size_t(blockIdx.y) * col_blocks + c0 / kBlock + b) * j.rows + r] = sh[b][lane];
+    if (threadIdx.x < kBlock) {
+        const int block = threadIdx.x / kRows, r = threadIdx.x % kRows, col_blocks = (j.cols + kBlock - 1) / kBlock;
+        if (r0 + r < j.rows && c0 / kBlock + block < col_blocks)
+            j.scales[(size_t(blockIdx.y) * col_blocks + c0 / kBlock + block) * j.rows + r0 + r] = sh[block][r];
     }
 }
 
@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
 // 16-byte chunk of a column is exclusive-or'ed with the column's octet, so that a warp's 32 words
 // fall in 32 banks.
 template <typename T, bool E5M2, bool VEC, bool TILE_SCALE, bool BOTH>
-__global__ void __launch_bounds__(kThreads) k_quant_tile(QuantJob<T> j) {
+__global__ void __launch_bounds__(kThreads, !BOTH ? (sizeof(T) == 2 ? 4 : 3) : sizeof(T) == 4 && !TILE_SCALE ? 2 : 3)
+k_quant_tile(QuantJob<T> j) {
     using P = typename Pair<T>::type;
     constexpr int kPairs = sizeof(Vals<T>) / 4, kPer = 16 / kPairs;   // pairs of a lane's row, values in one
     __shared__ P col_max[8][kBlock / kPer];
@@ -407,14 +408,18 @@ int column_run(int rows) { return std::max(64, (rows + 591) / 592); }
 
 template <typename T, bool E5M2, bool VEC>
 void launch_quant(const QuantJob<T>& j, int block_rows, int batch, cudaStream_t stream) {
-    const long long rows32 = (j.rows + 31) / 32, rows128 = (j.rows + 127) / 128;
-    const long long grid = block_rows == 1 && !j.t_codes ? rows32 * ((j.cols + 511) / 512)
-                                                         : rows128 * ((j.cols + 127) / 128);
+    const long long rows128 = (j.rows + 127) / 128, col_blocks = (j.cols + 127) / 128;
+    const int cb = col_blocks >= 3 ? 4 : int(col_blocks);
+    const long long grid = block_rows == 1 && !j.t_codes
+                               ? (j.rows * (long long)cb + 127) / 128 * ((col_blocks + cb - 1) / cb) : rows128 * col_blocks;
     require(grid < (1LL << 31), "matrix is too large");
     const dim3 g(unsigned(grid), unsigned(batch), 1);
-    if (block_rows == 1) {
-        if (!j.t_codes) k_quant_rows<T, E5M2, VEC><<<g, kThreads, 0, stream>>>(j);
-        else k_quant_tile<T, E5M2, VEC, false, true><<<g, kThreads, 0, stream>>>(j);
+    if (block_rows == 1 && !j.t_codes) {
+        if (cb == 4) k_quant_rows<T, E5M2, VEC, 4><<<g, kThreads, 0, stream>>>(j);
+        else if (cb == 2) k_quant_rows<T, E5M2, VEC, 2><<<g, kThreads, 0, stream>>>(j);
+        else k_quant_rows<T, E5M2, VEC, 1><<<g, kThreads, 0, stream>>>(j);
+    } else if (block_rows == 1) {
+        k_quant_tile<T, E5M2, VEC, false, true><<<g, kThreads, 0, stream>>>(j);
     } else {
         if (!j.t_codes) k_quant_tile<T, E5M2, VEC, true, false><<<g, kThreads, 0, stream>>>(j);
         else k_quant_tile<T, E5M2, VEC, true, true><<<g, kThreads, 0, stream>>>(j);
