@@ -93,7 +93,7 @@ _SIGNATURES = {
     "aeisu_block_quantize": (C.c_int, [_MATRIX, C.c_int, _MATRIX, _MATRIX, C.c_int, C.c_void_p]),
     "aeisu_column_sum_workspace": (C.c_uint64, [C.c_int, C.c_int]),
     "aeisu_column_sum": (C.c_int, [_MATRIX, C.c_void_p, C.c_int, C.c_void_p, C.c_uint64, C.c_int, C.c_void_p]),
-    "aeisu_product_workspace": (C.c_uint64, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "aeisu_product_workspace": (C.c_uint64, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "aeisu_product": (C.c_int, [_MATRIX, _MATRIX, C.c_void_p, C.c_int, _MATRIX, C.c_void_p, C.c_uint64, C.c_int,
                                 C.c_void_p]),
     "aeisu_linear_workspace": (C.c_uint64, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),

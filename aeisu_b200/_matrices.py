@@ -83,8 +83,8 @@ def operand(t):
 
 
 @functools.lru_cache(maxsize=4096)
-def product_bytes(m, n, k, fp8, index):
-    return _lib.lib().aeisu_product_workspace(m, n, k, fp8, index)
+def product_bytes(m, n, k, index):
+    return _lib.lib().aeisu_product_workspace(m, n, k, index)
 
 
 @functools.lru_cache(maxsize=4096)

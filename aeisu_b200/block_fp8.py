@@ -170,7 +170,7 @@ def matmul(a, b, *, bias=None, dtype=torch.bfloat16):
     if m == 0 or n == 0:
         return out
     (ka, ma), (kb, mb) = a.matrix(), b.matrix()
-    size = mx.product_bytes(m, n, k, 1, index)
+    size = mx.product_bytes(m, n, k, index)
     ws = mx.scratch(size, out) if size else None
     _lib.check(_call().aeisu_product(ma, mb, None if bias is None else bias.data_ptr(),
                                         0 if bias is None else mx.TYPES[bias.dtype], mx.matrix(out, n),

@@ -46,7 +46,7 @@ void join_sums(const float* partial, int runs, int cols, void* out, int out_type
 size_t column_sum_partials(int rows, int cols);
 void column_sum(const MatrixRef& x, void* out, int out_type, float* partial, int device, cudaStream_t stream);
 
-// out[m][n] = sum_k a[m][k] b[n][k] (+ bias[n]).
+// out[m][n] = sum_k a[m][k] b[n][k] (+ bias[n]) of FP8 operands.
 struct ProductOut {
     void* ptr;
     int type;
@@ -54,10 +54,10 @@ struct ProductOut {
     const void* bias;        // n values of bias_type, or null
     int bias_type;
 };
-size_t product_workspace(int m, int n, int k, bool fp8, int device);
+size_t product_workspace(int m, int n, int k, int device);
 // after_quantize: the kernel enqueued just before on `stream` is the quantiser of an operand, and the
 // product may start while it runs.
-void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const ScaleRef* sb, const ProductOut& out,
+void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
              void* workspace, size_t workspace_bytes, bool after_quantize, int device, cudaStream_t stream);
 
 // Rows t in [off[e], off[e + 1]) of x [rows][k] times b[e] [n][k]: out[t][n].  Rows outside every

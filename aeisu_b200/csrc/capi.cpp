@@ -329,11 +329,11 @@ int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* works
     });
 }
 
-uint64_t aeisu_product_workspace(int m, int n, int k, int fp8, int device) {
+uint64_t aeisu_product_workspace(int m, int n, int k, int device) {
     uint64_t r = 0;
     guarded([&] {
         aeisu::require(m >= 1 && n >= 1 && k >= 1, "matrix sizes are out of range");
-        r = aeisu::product_workspace(m, n, k, fp8 != 0, device);
+        r = aeisu::product_workspace(m, n, k, device);
     });
     return r;
 }
@@ -342,8 +342,8 @@ int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias
                   void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
         const aeisu::MatrixRef ma = matrix(a), mb = matrix(b);
-        const Scales sa(a), sb(b);
-        aeisu::product(ma, sa.ptr, mb, sb.ptr, product_out(out, bias, bias_type), workspace, size_t(workspace_bytes),
+        aeisu::require(a->scales && b->scales, "FP8 operands, and only they, come with scales");
+        aeisu::product(ma, scales_of(a), mb, scales_of(b), product_out(out, bias, bias_type), workspace, size_t(workspace_bytes),
                        false, device, static_cast<cudaStream_t>(stream));
     });
 }

@@ -11,7 +11,8 @@
 //     tensor core; a block of 128 is four such steps with the same scale.  The scales of 128 rows and
 //     four blocks form the 512-byte atom that tcgen05.cp spreads over the TMEM lanes (row r, block j at
 //     (r % 32) * 16 + (r / 32) * 4 + j); warps 2 and 3 gather it from global memory once per four
-//     steps, in turn and ahead of time, and the MMA names the byte j.  The accumulator never leaves TMEM before the tile is done.
+//     steps, in turn and ahead of time, and the MMA names the byte j.  The accumulator never leaves TMEM
+//     before the tile is done.
 //   * contraction grouped by expert: a group's last step may reach into the next group's rows; warp 2
 //     zeroes those rows of both operands in shared memory before the MMA sees the stage.
 // The writers take a whole tile into registers and hand TMEM back before they store, because 256 columns
@@ -388,7 +389,8 @@ __device__ __forceinline__ void load_scales(RawScales& r, const ScaleRef& s, Sca
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r.v[4 * b + i] = __ldg(col[b] + min(row0 + 32 * i + lane, rows - 1));
+            for (int i = 0; i < 4; ++i)
+                r.v[4 * b + i] = __ldg(col[b] + (min(row0 + 32 * i + lane, rows - 1) >> s.shift));
     }
 }
 // The atom into shared memory: row r, block j at (r % 32) * 16 + (r / 32) * 4 + j.
@@ -415,9 +417,10 @@ __device__ __forceinline__ void store_scales(const RawScales& r, ScaleWay way, u
         reinterpret_cast<uint4*>(atom)[lane] = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
-// Words of four rows where every tile starts at a multiple of four rows and the columns are as aligned.
+// Words of four rows where every tile starts at a multiple of four rows and the columns are as aligned; tiles
+// of ragged groups start anywhere.
 __device__ __forceinline__ ScaleWay scale_way(const ScaleRef& s, int rows, bool ragged) {
-    if (s.shift) return kPerBlock;
+    if (s.shift) return ragged ? kPerRow : kPerBlock;
     return !ragged && rows >= 4 && s.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(s.ptr) & 3) == 0 &&
                    s.batch_stride % 4 == 0 ? kPerRowWords : kPerRow;
 }
@@ -1006,13 +1009,14 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             __syncwarp();
         }
         if (j.zero_outside) {
-            const int before = bound[0], after = bound[j.groups], skip = after - before;
-            const long long todo = (long long)(j.zero_rows - skip) * j.cols;
-            constexpr int kLanes = 128 * S::kHalves;
-            for (long long i = (long long)blockIdx.x * kLanes + (threadIdx.x - 128); i < todo;
-                 i += (long long)gridDim.x * kLanes) {
-                const int r = int(i / j.cols), at = r < before ? r : r + skip;
-                store_elem(j.out, j.out_type, at * j.out_ld + i % j.cols, 0.f);
+            // A warp takes a row at a time: the rows before the first group, then those behind the last.
+            const int before = bound[0], skip = bound[j.groups] - before, size = j.out_type == kF32 ? 4 : 2;
+            constexpr int kWarps = 4 * S::kHalves;
+            for (int i = int(blockIdx.x) * kWarps + warp - 4; i < j.zero_rows - skip; i += int(gridDim.x) * kWarps) {
+                uint8_t* row = static_cast<uint8_t*>(j.out) + (i < before ? i : i + skip) * j.out_ld * size;
+                const int bytes = j.cols * size, whole = j.out_vec ? bytes / 16 * 16 : 0;
+                for (int c = lane * 16; c < whole; c += 32 * 16) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+                for (int c = whole + lane * 2; c < bytes; c += 32 * 2) *reinterpret_cast<uint16_t*>(row + c) = 0;
             }
         }
     }
@@ -1204,9 +1208,9 @@ struct Plan {
     int cluster;        // parts of a cluster (split), or 1: parts joined by a kernel
 };
 
-Plan plan_dense(int m, int n, int k, bool fp8, int sms) {
+Plan plan_dense(int m, int n, int k, int sms) {
     Plan p{};
-    const int step = fp8 ? kStepBytes : kStepBytes / 2, steps = (k + step - 1) / step;
+    const int steps = (k + kStepBytes - 1) / kStepBytes;
     // Few rows: the weights take the 128 lanes, so that no lane idles, and the rows the columns.
     p.swap = m <= 64 && n > m;
     const int P = p.swap ? n : m, Q = p.swap ? m : n;
@@ -1261,21 +1265,19 @@ bool whole_rows(const void* p, int type, long long ld, long long batch) {
 
 }  // namespace
 
-size_t product_workspace(int m, int n, int k, bool fp8, int device) {
-    const Plan p = plan_dense(m, n, k, fp8, sm_count(device));
+size_t product_workspace(int m, int n, int k, int device) {
+    const Plan p = plan_dense(m, n, k, sm_count(device));
     return p.split > p.cluster ? size_t(p.split) * m * n * sizeof(float) : 0;
 }
 
-void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const ScaleRef* sb, const ProductOut& out,
+void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
              void* workspace, size_t workspace_bytes, bool after_quantize, int device, cudaStream_t stream) {
-    check_operand(a, sa);
-    check_operand(b, sb);
-    require(a.batch == 1 && b.batch == 1 && !a.trans && !b.trans && a.cols == b.cols, "contraction sizes differ");
-    require((sa != nullptr) == (sb != nullptr) && (sa || a.type == b.type), "operand types do not go together");
+    check_operand(a, &sa);
+    check_operand(b, &sb);
+    require(a.batch == 1 && b.batch == 1 && a.cols == b.cols, "contraction sizes differ");
     require(out.ptr && out.type >= kF32 && out.type <= kBF16 && out.ld >= b.rows, "output is out of range");
     OnDevice on(device);
-    const bool fp8 = sa != nullptr;
-    const Plan pl = plan_dense(a.rows, b.rows, a.cols, fp8, sm_count(device));
+    const Plan pl = plan_dense(a.rows, b.rows, a.cols, sm_count(device));
     const size_t need = pl.split > pl.cluster ? size_t(pl.split) * a.rows * b.rows * sizeof(float) : 0;
     require(need == 0 || (workspace && workspace_bytes >= need), "workspace is too small");
     const MatrixRef& A = pl.swap ? b : a;
@@ -1284,13 +1286,9 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     j.P = A.rows;
     j.Q = B.rows;
     j.K = A.cols;
-    j.a_mn = A.trans;
-    j.b_mn = B.trans;
     j.idesc = instruction(A, B, pl.tile);
-    if (fp8) {
-        j.sa = pl.swap ? *sb : *sa;
-        j.sb = pl.swap ? *sa : *sb;
-    }
+    j.sa = pl.swap ? sb : sa;
+    j.sb = pl.swap ? sa : sb;
     j.a_rows = A.rows;
     j.b_rows = B.rows;
     j.swapped = pl.swap;
@@ -1300,7 +1298,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     j.steps_per_split = pl.steps;
     j.cluster = pl.cluster;
     j.after_quantize = after_quantize;
-    j.early_a = after_quantize && pl.swap && fp8;
+    j.early_a = after_quantize && pl.swap;
     if (pl.split > pl.cluster) {
         j.out = workspace;
         j.out_type = kF32;
@@ -1317,8 +1315,7 @@ void product(const MatrixRef& a, const ScaleRef* sa, const MatrixRef& b, const S
     const long long tiles = ceil_div(j.P, pl.tile.rows()) * ceil_div(j.Q, pl.tile.bn) * pl.split;
     require(tiles < (1LL << 30), "matrix is too large");
     const CUtensorMap ma = operand_map(A, kBM), mb = operand_map(B, pl.tile.b_rows());
-    if (fp8) launch_shape<true>(pl.tile, ma, mb, j, tiles, device, stream);
-    else launch_shape<false>(pl.tile, ma, mb, j, tiles, device, stream);
+    launch_shape<true>(pl.tile, ma, mb, j, tiles, device, stream);
     if (pl.split > pl.cluster) {
         const long long n = (long long)a.rows * b.rows;
         k_join_parts<<<unsigned(std::min<long long>((n + 255) / 256, 148 * 8)), 256, 0, stream>>>(
@@ -1419,7 +1416,8 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     const long long tiles = ceil_div(g.rows, tile.rows()) * ceil_div(x.rows, tile.bn) * groups;
     const int lanes = sm_count(device) / tile.ctas;
     j.by_lanes = divider(lanes);
-    j.balance = groups <= kDealGroups && tiles > lanes && lanes <= kThreads / 2;
+    j.balance = groups <= kDealGroups && tiles > lanes && lanes <= kThreads / 2 &&
+                g.cols < (1 << 27);   // a CTA's steps and number share an int
     require(tiles < (1LL << 30), "matrix is too large");
     launch_shape<false>(tile, operand_map(g, 64), operand_map(x, 64), j, tiles, device, stream);
 }

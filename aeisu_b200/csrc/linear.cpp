@@ -47,11 +47,11 @@ void check_workspace(const void* workspace, size_t have, size_t need) {
 size_t transposed_codes_bytes(int rows, int cols, int block_rows) { return operand_bytes(cols, rows, block_rows); }
 
 size_t linear_workspace(int m, int n, int k, int pass, int device) {
-    if (pass == kServe) return operand_bytes(m, k, 1) + product_workspace(m, n, k, true, device);
+    if (pass == kServe) return operand_bytes(m, k, 1) + product_workspace(m, n, k, device);
     if (pass == kTrainForward)
-        return operand_bytes(m, k, 1) + operand_bytes(n, k, kBlock) + product_workspace(m, n, k, true, device);
+        return operand_bytes(m, k, 1) + operand_bytes(n, k, kBlock) + product_workspace(m, n, k, device);
     return operand_bytes(m, n, 1) + operand_bytes(n, m, 1) +
-           std::max({product_workspace(m, k, n, true, device), product_workspace(n, k, m, true, device),
+           std::max({product_workspace(m, k, n, device), product_workspace(n, k, m, device),
                      std::max(column_sum_partials(m, n), size_t((m + kBlock - 1) / kBlock) * n) * sizeof(float)});
 }
 
@@ -61,7 +61,7 @@ void linear_serve(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, co
     const Operand q = operand_at(workspace, kE4M3, x.rows, x.cols, 1);
     const size_t used = operand_bytes(x.rows, x.cols, 1);
     quantize_into(x, 1, q, nullptr, nullptr, device, stream);
-    product(q.m, &q.s, w, &sw, out, static_cast<uint8_t*>(workspace) + used, workspace_bytes - used, true, device, stream);
+    product(q.m, q.s, w, sw, out, static_cast<uint8_t*>(workspace) + used, workspace_bytes - used, true, device, stream);
 }
 
 void linear_train_forward(const MatrixRef& x, const MatrixRef& w, const ProductOut& out, void* kept_x, void* kept_w,
@@ -75,7 +75,7 @@ void linear_train_forward(const MatrixRef& x, const MatrixRef& w, const ProductO
     const Operand qt = operand_at(kept_x, kE4M3, x.cols, x.rows, 1), rt = operand_at(kept_w, kE4M3, w.cols, w.rows, kBlock);
     quantize_into(w, kBlock, r, kept_w ? &rt : nullptr, nullptr, device, stream);
     quantize_into(x, 1, q, kept_x ? &qt : nullptr, nullptr, device, stream);
-    product(q.m, &q.s, r.m, &r.s, out, ws, workspace_bytes - size_t(ws - static_cast<uint8_t*>(workspace)), true, device,
+    product(q.m, q.s, r.m, r.s, out, ws, workspace_bytes - size_t(ws - static_cast<uint8_t*>(workspace)), true, device,
             stream);
 }
 
@@ -103,11 +103,11 @@ void linear_train_backward(const MatrixRef& grad, int k, int code_type, const vo
     const bool after = !(gb && gw);   // the kernel before the next product is the quantiser
     if (gx) {
         const Operand wt = operand_at(kept_w, kE4M3, k, n, kBlock);
-        product(g.m, &g.s, wt.m, &wt.s, {gx, gx_type, k, nullptr, 0}, ws, left, after, device, stream);
+        product(g.m, g.s, wt.m, wt.s, {gx, gx_type, k, nullptr, 0}, ws, left, after, device, stream);
     }
     if (gw) {
         const Operand xt = operand_at(kept_x, kE4M3, k, m, 1);
-        product(gt.m, &gt.s, xt.m, &xt.s, {gw, gw_type, k, nullptr, 0}, ws, left, after && !gx, device, stream);
+        product(gt.m, gt.s, xt.m, xt.s, {gw, gw_type, k, nullptr, 0}, ws, left, after && !gx, device, stream);
     }
 }
 

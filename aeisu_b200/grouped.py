@@ -84,7 +84,8 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
     ``x`` [T, K]; ``weight`` [E, N, K], E at most 1024, either of its last two dimensions contiguous;
     ``offsets`` int32 [E + 1], not decreasing, within [0, T] (values outside are moved to the nearest
     allowed one).  The result has x's type; ``dtype`` names it where x is BlockFP8 (default bfloat16).
-    ``out`` [T, N] takes the result instead of a new tensor; no gradients flow through it.
+    ``out`` [T, N] takes the result instead of a new tensor; it must not overlap x, and no gradients flow
+    through it.
     """
     fp8 = isinstance(weight, BlockFP8)
     coded = isinstance(x, BlockFP8)
@@ -106,8 +107,9 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
     if dtype not in mx.FLOATS:
         raise TypeError(f"the result is float32, float16 or bfloat16; got {dtype}")
     t, n = x.shape[0], weight.shape[1]
-    if out is not None and (tuple(out.shape) != (t, n) or out.dtype != dtype or (t and mx.row_stride(out) is None)):
-        raise ValueError(f"Expected out [{t}, {n}] of {dtype} with contiguous rows")
+    if out is not None and (tuple(out.shape) != (t, n) or out.dtype != dtype or (t and mx.row_stride(out) is None) or
+                            out.requires_grad):
+        raise ValueError(f"Expected out [{t}, {n}] of {dtype} with contiguous rows and without gradient")
     index = mx.need_cuda("grouped_matmul", x.codes if coded else x, weight.codes if fp8 else weight, offsets,
                          *(() if out is None else (out,)))
     if torch.is_grad_enabled() and ((not coded and x.requires_grad) or (not fp8 and weight.requires_grad)):

@@ -348,10 +348,10 @@ uint64_t aeisu_column_sum_workspace(int rows, int cols);
 int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* workspace, uint64_t workspace_bytes,
                      int device, void* stream);
 
-/* out[m][n] = sum_k a[m][k] b[n][k] + bias[n] (bias may be NULL): two FP8 operands with their
- * scales, or two of one 16-bit type; float32 accumulation, one rounding to out's type (float32,
- * float16 or bfloat16).  The order of the sum depends on the sizes alone. */
-uint64_t aeisu_product_workspace(int m, int n, int k, int fp8, int device);
+/* out[m][n] = sum_k a[m][k] b[n][k] + bias[n] (bias may be NULL) of two FP8 operands with their
+ * scales; float32 accumulation, one rounding to out's type (float32, float16 or bfloat16).  The
+ * order of the sum depends on the sizes alone. */
+uint64_t aeisu_product_workspace(int m, int n, int k, int device);
 int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias, int bias_type, const aeisu_matrix* out,
                   void* workspace, uint64_t workspace_bytes, int device, void* stream);
 
@@ -379,7 +379,8 @@ int aeisu_linear_backward(const aeisu_matrix* grad, int k, int code_type, const 
  * offsets[e + 1]); weight->batch groups (at most 1024), offsets int32 [groups + 1] in device
  * memory.  Rows in no group are set to zero when zero_outside is nonzero, otherwise left as they
  * were.  Offsets outside [0, x->rows] or below the one before are moved to the nearest allowed
- * value.  Types as for aeisu_product. */
+ * value.  x and weight are both FP8 with their scales, or both float16 or both bfloat16 (weight then
+ * transposed or not); accumulation and rounding as for aeisu_product.  out must not overlap x. */
 int aeisu_grouped_product(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
                           const aeisu_matrix* out, int device, void* stream);
 /* The same with x float, quantised to E4M3 in blocks of 1 x 128 into the workspace, and FP8 weights. */

@@ -132,7 +132,8 @@ def test_row_strides():
     assert mx.row_stride(b.transpose(0, 1)) is None      # rows of one matrix lie between those of the next
 
 
-MATRIX = dict(data=4096, scales=0, type=2, rows=8, cols=64, batch=1, ld=64, batch_stride=0, block_rows=0, transposed=0)
+MATRIX = dict(data=4096, scales=64, type=3, rows=8, cols=64, batch=1, ld=64, batch_stride=0, block_rows=1, transposed=0)
+HALF = dict(type=2, scales=0, block_rows=0)
 
 
 def packed(**kw):
@@ -140,42 +141,45 @@ def packed(**kw):
 
 
 @pytest.mark.parametrize("a, text", [
-    (dict(data=0), "null"), (dict(rows=0), "sizes"), (dict(ld=32), "overlap"), (dict(ld=68), "16-byte"),
-    (dict(data=4098), "16-byte"), (dict(type=0), "FP8, float16 or bfloat16"), (dict(type=9), "FP8, float16 or bfloat16"),
-    (dict(type=3), "come with scales"), (dict(scales=64, block_rows=1), "come with scales"),
-    (dict(type=3, scales=64, block_rows=5), "1 or 128"), (dict(type=1), "go together"), (dict(cols=128, ld=128), "contraction"),
-    (dict(transposed=1), "contraction"), (dict(batch=2, batch_stride=512), "contraction"),
+    (dict(data=0), "null"), (dict(rows=0), "sizes"), (dict(ld=32), "overlap"), (dict(ld=72), "16-byte"),
+    (dict(data=4098), "16-byte"), (dict(type=0), "come with scales"), (dict(type=2), "come with scales"),
+    (dict(type=9), "come with scales"), (dict(scales=0), "come with scales"), (HALF, "come with scales"),
+    (dict(block_rows=5), "1 or 128"), (dict(cols=128, ld=128), "contraction"), (dict(transposed=1), "row by row"),
+    (dict(batch=2, batch_stride=512), "contraction"),
 ])
 def test_c_product_refuses_bad_operands(lib, a, text):
-    out = packed(cols=8, ld=8)
+    out = packed(cols=8, ld=8, **HALF)
     status = lib.aeisu_product(packed(**a), packed(), None, 0, out, None, 0, 0, None)
     assert status == _lib.INVALID_ARG and text in _lib.last_error()
 
 
 def test_c_entries_refuse_bad_arguments(lib):
-    ok, out = packed(), packed(cols=8, ld=8)
-    f32 = packed(type=0)
-    codes = packed(type=3, scales=64, block_rows=1)
+    codes, half, out = packed(), packed(**HALF), packed(cols=8, ld=8, **HALF)
+    f32 = packed(**{**HALF, "type": 0})
     for call, text in (
-            (lambda: lib.aeisu_product(None, ok, None, 0, out, None, 0, 0, None), "null"),
-            (lambda: lib.aeisu_product(ok, ok, None, 0, None, None, 0, 0, None), "null"),
-            (lambda: lib.aeisu_product(ok, ok, 4096, 7, out, None, 0, 0, None), "bias"),
-            (lambda: lib.aeisu_product(ok, ok, None, 0, packed(cols=8, ld=4), None, 0, 0, None), "output"),
-            (lambda: lib.aeisu_product(ok, ok, None, 0, packed(type=3), None, 0, 0, None), "output"),
+            (lambda: lib.aeisu_product(None, codes, None, 0, out, None, 0, 0, None), "null"),
+            (lambda: lib.aeisu_product(codes, codes, None, 0, None, None, 0, 0, None), "null"),
+            (lambda: lib.aeisu_product(codes, codes, 4096, 7, out, None, 0, 0, None), "bias"),
+            (lambda: lib.aeisu_product(codes, codes, None, 0, packed(cols=8, ld=4, **HALF), None, 0, 0, None), "output"),
+            (lambda: lib.aeisu_product(codes, codes, None, 0, packed(), None, 0, 0, None), "output"),
             (lambda: lib.aeisu_block_quantize(f32, 64, codes, None, 0, None), "1 or 128"),
             (lambda: lib.aeisu_block_quantize(f32, 1, None, None, 0, None), "null"),
-            (lambda: lib.aeisu_block_quantize(f32, 1, packed(type=2, scales=64), None, 0, None), "E4M3"),
-            (lambda: lib.aeisu_block_quantize(f32, 1, packed(type=3, scales=64, ld=72), None, 0, None), "16-byte"),
-            (lambda: lib.aeisu_block_quantize(f32, 1, packed(type=3, scales=64, rows=9), None, 0, None), "sizes"),
+            (lambda: lib.aeisu_block_quantize(f32, 1, packed(type=2), None, 0, None), "E4M3"),
+            (lambda: lib.aeisu_block_quantize(f32, 1, packed(ld=72), None, 0, None), "16-byte"),
+            (lambda: lib.aeisu_block_quantize(f32, 1, packed(rows=9), None, 0, None), "sizes"),
             (lambda: lib.aeisu_block_quantize(f32, 1, codes, codes, 0, None), "transposed sizes"),
-            (lambda: lib.aeisu_linear(ok, ok, None, 0, out, 4096, 1 << 20, 0, None), "scales"),
-            (lambda: lib.aeisu_linear(packed(cols=32), codes, None, 0, out, 4096, 1 << 20, 0, None), "contraction"),
-            (lambda: lib.aeisu_grouped_product(ok, ok, None, 1, out, 0, None), "offsets"),
-            (lambda: lib.aeisu_grouped_product(ok, packed(batch=1025, batch_stride=512), 4096, 1, out, 0, None), "1024"),
-            (lambda: lib.aeisu_grouped_weight_gradient(ok, packed(rows=9), 4096, 2, 4096, 2, 0, None), "contraction"),
-            (lambda: lib.aeisu_grouped_weight_gradient(ok, ok, 4096, 0, 4096, 2, 0, None), "offsets"),
-            (lambda: lib.aeisu_grouped_weight_gradient(ok, ok, 4096, 2, None, 2, 0, None), "output"),
-            (lambda: lib.aeisu_column_sum(ok, 4096, 2, None, 0, 0, None), "workspace"),
+            (lambda: lib.aeisu_linear(half, half, None, 0, out, 4096, 1 << 20, 0, None), "scales"),
+            (lambda: lib.aeisu_linear(packed(cols=32, **HALF), codes, None, 0, out, 4096, 1 << 20, 0, None), "contraction"),
+            (lambda: lib.aeisu_grouped_product(half, half, None, 1, out, 0, None), "offsets"),
+            (lambda: lib.aeisu_grouped_product(half, packed(batch=1025, batch_stride=512, **HALF), 4096, 1, out, 0, None), "1024"),
+            (lambda: lib.aeisu_grouped_product(half, codes, 4096, 1, out, 0, None), "go together"),
+            (lambda: lib.aeisu_grouped_product(half, packed(**{**HALF, "type": 1}), 4096, 1, out, 0, None), "go together"),
+            (lambda: lib.aeisu_grouped_product(packed(transposed=1, **HALF), half, 4096, 1, out, 0, None), "contraction"),
+            (lambda: lib.aeisu_grouped_weight_gradient(codes, half, 4096, 2, 4096, 2, 0, None), "come with scales"),
+            (lambda: lib.aeisu_grouped_weight_gradient(half, packed(rows=9, **HALF), 4096, 2, 4096, 2, 0, None), "contraction"),
+            (lambda: lib.aeisu_grouped_weight_gradient(half, half, 4096, 0, 4096, 2, 0, None), "offsets"),
+            (lambda: lib.aeisu_grouped_weight_gradient(half, half, 4096, 2, None, 2, 0, None), "output"),
+            (lambda: lib.aeisu_column_sum(half, 4096, 2, None, 0, 0, None), "workspace"),
             (lambda: lib.aeisu_product_status(0, None), "null")):
         assert call() == _lib.INVALID_ARG and text in _lib.last_error(), _lib.last_error()
     assert lib.aeisu_linear_kept_bytes(0, 4, 1) == 0 and lib.aeisu_linear_kept_bytes(4, 4, 2) == 0

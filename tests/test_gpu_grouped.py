@@ -72,6 +72,20 @@ def test_fp8_weights(sizes, k, n):
         O.check_product(exact[lo:hi], xv[lo:hi], wv[i])
 
 
+@pytest.mark.parametrize("sizes", [[5, 0, 3], [37, 130, 60], [300, 201]], ids=str)
+@pytest.mark.parametrize("rows, weight_rows", [(128, 128), (128, 1), (1, 1)])
+def test_fp8_operands_of_either_block_height(sizes, rows, weight_rows):
+    # a group starts anywhere in a block of 128 rows of x, and its tiles reach into the next
+    t, off = sum(sizes) + 11, bounds(sizes, first=11)
+    x = B.quantize(randn(t, 300) * torch.exp2(torch.arange(t).float() // 64 - 4)[:, None].cuda(), rows=rows)
+    w = B.quantize(randn(len(sizes), 150, 300, seed=1), rows=weight_rows)
+    y = grouped_matmul(x, w, off, dtype=torch.float32)
+    xv, wv = x.dequantize(), w.dequantize()
+    for i, (lo, hi) in enumerate(spans(off)):
+        O.check_product(y[lo:hi], xv[lo:hi], wv[i])
+    assert not y[:11].any()
+
+
 def test_gradient_against_differences():
     # The product is linear: a whole step in one entry moves the weighted sum by the gradient exactly,
     # up to float16's rounding of the outputs and of the gradient (integers here: both exact).
@@ -115,6 +129,16 @@ def test_rows_outside_the_groups(fp8, sizes):
         g[21:int(off[-1])] = 1.0
         grouped_matmul(x, w, off).backward(g)
         assert not x.grad.cpu()[~inside].any() and bool(w.grad.isfinite().all())
+
+
+@pytest.mark.parametrize("n, dtype", [(37, torch.bfloat16), (64, torch.float16), (9, torch.float32), (264, torch.float32)])
+def test_long_padding_is_zeroed(n, dtype):
+    t, off = 20_000, bounds([3, 0, 70], first=9000)
+    x, w = randn(t, 32), B.quantize(randn(3, n, 32, seed=1), rows=128)
+    big = torch.full((t * n + 4096,), 3.0, device="cuda", dtype=dtype)      # what the allocator may hand out next
+    del big
+    y = grouped_matmul(B.quantize(x), w, off, dtype=dtype)
+    assert not y[:9000].any() and not y[9073:].any() and bool(y[9000:9073].any())
 
 
 def test_nan_stays_in_its_group():
