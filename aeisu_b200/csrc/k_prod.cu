@@ -1045,6 +1045,7 @@ __global__ void __launch_bounds__(256) k_join_parts(const float* part, int parts
     const long long n = (long long)rows * cols;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
         float s = 0.f;
+#pragma unroll 16
         for (int k = 0; k < parts; ++k) s += part[k * stride + i];
         const int r = int(i / cols), c = int(i % cols);
         if (bias) s += load_elem(bias, bias_type, c);
