@@ -37,6 +37,40 @@ from . import _matrices as mx
 _E8M0 = torch.float8_e8m0fnu
 _call = _lib.lib
 _new = object.__new__
+_pack = _lib.MATRIX.pack
+
+
+@functools.lru_cache(maxsize=4096)
+def _sizes(shape, rows):
+    """(row stride of the codes, shape of the codes' storage, shape of the scales)."""
+    *lead, r, c = shape
+    ld = -(-c // 16) * 16
+    return ld, (*lead, r, ld), (*lead, mx.blocks(c), -(-r // rows))
+
+
+def _form(codes, ld, rows):
+    """The fields of aeisu_matrix behind its pointers; None where a product has to take a copy."""
+    shape = codes.shape
+    batch, step = (shape[0], codes.stride(0)) if len(shape) == 3 else (1, 0)
+    r, c = shape[-2], shape[-1]
+    if ld is not None and r == 1:
+        ld = -(-ld // 16) * 16   # the stride of a single row is never taken
+    if ld is None or ld % 16 or (batch > 1 and step % 16):
+        return None
+    return mx.TYPES[codes.dtype], r, c, batch, ld, step, rows, 0
+
+
+def _empty(x, shape, rows, dtype):
+    """(uninitialised BlockFP8 beside x, its aeisu_matrix)."""
+    ld, stored, scaled = _sizes(shape, rows)
+    q = _new(BlockFP8)
+    codes = x.new_empty(stored, dtype=dtype)
+    at = codes.data_ptr()
+    q._codes = codes = codes if ld == shape[-1] else codes[..., :shape[-1]]
+    q._scales = scales = x.new_empty(scaled, dtype=_E8M0)
+    q._rows = rows
+    q._form = form = _form(codes, ld, rows)
+    return q, _pack(at, scales.data_ptr(), *form)
 
 
 class BlockFP8:
@@ -44,26 +78,40 @@ class BlockFP8:
 
     ``scales`` (``torch.float8_e8m0fnu``, contiguous) is ``[..., ceil(C / 128), ceil(R / rows)]``: the
     scales of one block column lie together.  ``rows`` is 1 or 128; the value of a code is
-    ``codes[r, c] * scales[c // 128, r // rows]``.
+    ``codes[r, c] * scales[c // 128, r // rows]``.  The tensors' values may change, their sizes and strides
+    may not.
     """
-    __slots__ = ("codes", "scales", "rows")
+    __slots__ = ("_codes", "_scales", "_rows", "_form")
 
     def __init__(self, codes, scales, rows=1):
-        if rows not in (1, mx.BLOCK):
+        if rows != 1 and rows != mx.BLOCK:
             raise ValueError("blocks have 1 or 128 rows")
         if codes.dtype not in mx.CODES:
             raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2; got {codes.dtype}")
         if scales.dtype != _E8M0:
             raise TypeError(f"scales must be float8_e8m0fnu; got {scales.dtype}")
-        if codes.dim() not in (2, 3):
+        shape = codes.shape
+        if len(shape) != 2 and len(shape) != 3:
             raise ValueError("Expected codes [R, C] or [E, R, C]")
-        r, c = codes.shape[-2:]
-        want = (*codes.shape[:-2], mx.blocks(c), -(-r // rows))
-        if tuple(scales.shape) != want or not scales.is_contiguous():
+        want = _sizes(shape, rows)[2]
+        if scales.shape != want or not scales.is_contiguous():
             raise ValueError(f"Expected contiguous scales {list(want)}; got {list(scales.shape)}")
-        if codes.device != scales.device:
+        if codes.get_device() != scales.get_device():
             raise ValueError("codes and scales must be on one device")
-        self.codes, self.scales, self.rows = codes, scales, rows
+        self._codes, self._scales, self._rows = codes, scales, rows
+        self._form = _form(codes, mx.row_stride(codes), rows)
+
+    @property
+    def codes(self):
+        return self._codes
+
+    @property
+    def scales(self):
+        return self._scales
+
+    @property
+    def rows(self):
+        return self._rows
 
     @property
     def shape(self):
@@ -81,31 +129,17 @@ class BlockFP8:
         return self.codes.to(torch.float32) * s
 
     def matrix(self):
-        """aeisu_matrix for a product; the tensors it points to have to be kept by the caller."""
-        codes, ld = mx.operand(self.codes)
-        return codes, mx.matrix(codes, ld, self.scales, self.rows)
+        """(codes, aeisu_matrix) for a product; the codes, a copy where theirs do not start rows on 16-byte
+        boundaries, have to be kept by the caller."""
+        codes, form = self._codes, self._form
+        at = codes.data_ptr()
+        if form is None or at % 16:
+            codes, ld = mx.operand(codes)
+            return codes, mx.matrix(codes, ld, self._scales, self._rows)
+        return codes, _pack(at, self._scales.data_ptr(), *form)
 
     def __repr__(self):
         return f"BlockFP8({list(self.codes.shape)}, {self.codes.dtype}, rows={self.rows}, {self.codes.device})"
-
-
-@functools.lru_cache(maxsize=4096)
-def _sizes(shape, rows, dtype):
-    """(row stride of the codes, shape of the codes' storage, shape of the scales)."""
-    *lead, r, c = shape
-    ld = -(-c // 16) * 16
-    return ld, (*lead, r, ld), (*lead, mx.blocks(c), -(-r // rows))
-
-
-def _empty(x, shape, rows, dtype):
-    """(uninitialised BlockFP8 beside x, its aeisu_matrix)."""
-    ld, stored, scaled = _sizes(shape, rows, dtype)
-    q = _new(BlockFP8)
-    codes = x.new_empty(stored, dtype=dtype)
-    q.codes = codes if ld == shape[-1] else codes[..., :shape[-1]]
-    q.scales = x.new_empty(scaled, dtype=_E8M0)
-    q.rows = rows
-    return q, mx.matrix(q.codes, ld, q.scales, rows)
 
 
 def _quantize(x, rows, dtype, both):
@@ -218,8 +252,11 @@ class _Linear(torch.autograd.Function):
         return _forward(x, weight, bias, at if need_w else None, at + size_x if need_x else None, x.get_device())
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
+        return _Linear.twice(ctx, grad) if torch.is_grad_enabled() else _Linear.once(ctx, grad)
+
+    @staticmethod
+    def once(ctx, grad):
         x_type, w_type, b_type, grad_dtype = ctx.types
         (m, n, k), (need_x, need_w, need_b, _), index = ctx.sizes, ctx.needs_input_grad, grad.get_device()
         new = grad.new_zeros if m == 0 else grad.new_empty
@@ -230,15 +267,20 @@ class _Linear(torch.autograd.Function):
             return gx, gw, gb, None
         (kept,) = ctx.saved_tensors
         at = kept.data_ptr()
-        kept_x, kept_w = (None if p is None else at + p for p in ctx.places)
+        kept_x, kept_w = ctx.places
+        kept_x = None if kept_x is None else at + kept_x
+        kept_w = None if kept_w is None else at + kept_w
         grad, mg = _rows(grad)
         size = mx.linear_bytes(m, n, k, 2, index)
         ws = mx.scratch(size, grad)
         _lib.check(_call().aeisu_linear_backward(
-            mg, k, mx.TYPES[grad_dtype], kept_x, kept_w,
-            *(v for t in (gx, gw, gb) for v in ((None, 0) if t is None else (t.data_ptr(), mx.TYPES[t.dtype]))),
+            mg, k, mx.TYPES[grad_dtype], kept_x, kept_w, gx.data_ptr() if need_x else None, mx.TYPES[x_type],
+            gw.data_ptr() if need_w else None, mx.TYPES[w_type], gb.data_ptr() if need_b else None,
+            mx.TYPES[b_type] if need_b else 0,
             ws.data_ptr(), size, index, mx.stream(index)))
         return gx, gw, gb, None
+
+    twice = staticmethod(once_differentiable(lambda ctx, grad: _Linear.once(ctx, grad)))
 
 
 def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
@@ -248,19 +290,24 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
     or a BlockFP8 kept from before, which serves without gradients.  The output has x's type; gradients
     have the types of their tensors.  ``grad_dtype`` is the FP8 type that the upstream gradient takes.
     """
-    serving = isinstance(weight, BlockFP8)
+    serving = type(weight) is BlockFP8
     if x.dtype not in mx.FLOATS:
         raise TypeError(f"linear takes float32, float16 or bfloat16; got {x.dtype}")
     if not serving and weight.dtype not in mx.FLOATS:
         raise TypeError(f"weight must be float32, float16, bfloat16 or BlockFP8; got {weight.dtype}")
     if grad_dtype not in mx.CODES:
         raise TypeError(f"grad_dtype must be float8_e4m3fn or float8_e5m2; got {grad_dtype}")
-    shape, wide = x.shape, weight.shape
+    values = weight.codes if serving else weight
+    shape, wide = x.shape, values.shape
     if len(shape) < 1 or len(wide) != 2 or shape[-1] != wide[1] or 0 in wide:
         raise ValueError("Expected x [..., K] and weight [N, K]")
     n, k = wide
-    ready = _bias(bias, n)
-    index = mx.need_cuda("linear", x, weight.codes if serving else weight, *(() if bias is None else (bias,)))
+    if bias is None:
+        ready = None
+        index = mx.need_cuda("linear", x, values)
+    else:
+        ready = _bias(bias, n)
+        index = mx.need_cuda("linear", x, values, bias)
     flat = x if len(shape) == 2 else x.reshape(shape[:-1].numel(), k)
     if torch.is_grad_enabled() and (x.requires_grad or (not serving and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):

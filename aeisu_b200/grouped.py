@@ -58,8 +58,11 @@ class _Grouped(torch.autograd.Function):
         return _product(_rows(x), _weights(weight), offsets, out, True)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
+        return _Grouped.twice(ctx, grad) if torch.is_grad_enabled() else _Grouped.once(ctx, grad)
+
+    @staticmethod
+    def once(ctx, grad):
         x, weight, offsets = ctx.saved_tensors
         if x.shape[0] == 0:
             return torch.empty_like(x), torch.zeros_like(weight), None
@@ -76,6 +79,8 @@ class _Grouped(torch.autograd.Function):
                                                                 gw.data_ptr(), mx.TYPES[gw.dtype], index,
                                                                 mx.stream(index)))
         return gx, gw, None
+
+    twice = staticmethod(once_differentiable(lambda ctx, grad: _Grouped.once(ctx, grad)))
 
 
 def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):

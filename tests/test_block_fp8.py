@@ -56,6 +56,10 @@ def test_block_fp8_refuses_what_is_no_operand():
         B.BlockFP8(codes, torch.ones(3, 10))
     with pytest.raises(ValueError, match="Expected codes"):
         B.BlockFP8(codes[0], scales(3, 10))
+    q = B.BlockFP8(codes, scales(3, 10))
+    for name, value in (("codes", codes[:5]), ("scales", scales(3, 5)), ("rows", 128)):
+        with pytest.raises(AttributeError):
+            setattr(q, name, value)
 
 
 def test_quantize_refusals():
