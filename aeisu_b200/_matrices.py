@@ -58,15 +58,6 @@ def matrix(t, ld, scales=None, rows=0, transposed=False):
                  transposed)
 
 
-def empty_rows(shape, dtype, device):
-    """An uninitialised tensor whose rows start on 16-byte boundaries."""
-    per = 16 // dtype.itemsize
-    c = shape[-1]
-    wide = -(-c // per) * per
-    t = torch.empty((*shape[:-1], wide), dtype=dtype, device=device)
-    return t if wide == c else t[..., :c]
-
-
 def operand(t):
     """(tensor, row stride) fit for a product: t itself where its rows are contiguous and start on 16-byte
     boundaries, else a copy."""
@@ -75,10 +66,11 @@ def operand(t):
     if ld is not None and t.shape[-2] == 1:
         ld = -(-ld * size // 16) * 16 // size   # the stride of a single row is never taken
     if ld is None or ld * size % 16 or t.data_ptr() % 16 or (t.dim() == 3 and t.shape[0] > 1 and t.stride(0) * size % 16):
-        copy = empty_rows(t.shape, t.dtype, t.device)
+        per = 16 // size
+        ld = -(-t.shape[-1] // per) * per
+        copy = t.new_empty_strided(t.shape, (t.shape[-2] * ld, ld, 1)[-t.dim():])
         copy.copy_(t)
         t = copy
-        ld = t.stride(-2)
     return t, ld
 
 
