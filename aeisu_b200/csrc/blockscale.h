@@ -60,10 +60,17 @@ size_t product_workspace(int m, int n, int k, int device);
 void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
              void* workspace, size_t workspace_bytes, bool after_quantize, int device, cudaStream_t stream);
 
+// The same with float rows x, which the product quantises to E4M3 in blocks of 1 x 128 itself; false, and
+// nothing done, where there are too many or their type or alignment does not allow it.
+bool product_of_values(const MatrixRef& x, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
+                       void* workspace, size_t workspace_bytes, int device, cudaStream_t stream);
+
 // Rows t in [off[e], off[e + 1]) of x [rows][k] times b[e] [n][k]: out[t][n].  Rows outside every
 // group are zeroed when zero_outside is set, otherwise left as they were.
 void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const ScaleRef* sb, const int* off,
                      const ProductOut& out, bool zero_outside, bool after_quantize, int device, cudaStream_t stream);
+bool grouped_product_of_values(const MatrixRef& x, const MatrixRef& b, const ScaleRef& sb, const int* off,
+                               const ProductOut& out, bool zero_outside, int device, cudaStream_t stream);
 // out[e][n][k] = sum over t in group e of g[t][n] x[t][k].
 void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* off, int groups, void* out,
                              int out_type, int device, cudaStream_t stream);

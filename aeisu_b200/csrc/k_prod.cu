@@ -26,6 +26,7 @@
 #include <mutex>
 #include <string>
 
+#include "blockscale_dev.cuh"
 #include "blockscale_host.h"
 #include "tc.cuh"
 
@@ -42,8 +43,7 @@ constexpr int kRing = 201 * 1024 + 512;   // shared memory of the operand ring
 constexpr int kTurn = 2048;           // shared memory of a writer: 32 rows of 64 bytes
 constexpr int kErrWait = 1;           // error code: a wait ran out
 constexpr int kAtom = 512;            // scales of 128 rows and four block columns
-constexpr int kGroupSteps = 4;        // steps that share an atom
-constexpr int kScaleSlots = 4;        // groups of steps whose scales are staged (even: two warps fill them)
+constexpr int kScaleSlots = 4;        // atoms that are staged at a time (even: two warps fill them)
 
 // What is grouped by the offsets.
 enum Grouping { kDense = 0, kRowsA = 1, kRowsB = 2, kContraction = 3 };
@@ -83,13 +83,18 @@ struct ProdJob {
     int balance;                 // tiles of unequal groups of a contraction are dealt to the least loaded CTAs
     int out_vec;                 // rows of out start on 32-byte boundaries
     int zero_outside, zero_rows;
+    const void* values;          // 16-bit rows of B that the kernel quantises itself, or null
+    int values_type;
+    long long values_ld;
     int early_a;                 // A is older than the kernel before (see after_quantize)
     int after_quantize;          // starts while the quantiser of its float operand still runs; the other
                                  // operand and the offsets are older
 };
 
-template <bool FP8, int BN, int CTAS>
+// OWN: the kernel quantises B's rows itself.
+template <bool FP8, int BN, int CTAS, bool OWN>
 struct Shape {
+    static constexpr int kGroup = OWN ? 1 : 4;               // steps that share an atom of scales
     static constexpr int kBRows = BN / CTAS;                 // rows of B that a CTA stages
     static constexpr int kATile = kBM * kStepBytes, kBTile = kBRows * kStepBytes;
     static constexpr int kAtomsB = (BN + 127) / 128;         // every CTA needs the scales of all BN
@@ -579,11 +584,51 @@ __device__ __forceinline__ void join_cluster(const ProdJob& j, const Tile& x, in
 
 // ---- the kernel --------------------------------------------------------------------------------
 
-template <bool FP8, int BN, int CTAS>
+// Few rows quantised on the spot (OWN): a warp's half, eight rows, of the rows q0 .. q0 + 15 of the 16-bit B by
+// 128 columns from k on, four lanes to a row.  Loaded a step ahead, turned into codes of the stage's swizzled
+// tile and scales of the atom's first block; the same arithmetic as the quantiser's, which these calls do
+// without.
+struct OwnRows {
+    blockq::Vals<__half> v[2];   // 32 values; the type only matters where they are read
+};
+__device__ __forceinline__ void load_own(OwnRows& o, const ProdJob& j, const Tile& x, int half, int k) {
+    const int lane = threadIdx.x & 31, q = x.q0 + half * 8 + (lane >> 2), c = k + (lane & 3) * 32;
+    const __half* row = static_cast<const __half*>(j.values) + q * j.values_ld;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (q < x.q1 && c + i * 8 < j.K) w = __ldg(reinterpret_cast<const uint4*>(row + c + i * 8));
+        reinterpret_cast<uint4*>(o.v[i >> 1].w)[i & 1] = w;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_own(OwnRows& o, int half, uint8_t* tile, uint8_t* atom) {
+    const int lane = threadIdx.x & 31, row = half * 8 + (lane >> 2);
+    auto& v = reinterpret_cast<blockq::Vals<T>(&)[2]>(o.v);
+    float amax = fmaxf(blockq::finite_max(v[0]), blockq::finite_max(v[1]));
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+    const uint32_t s = blockq::scale_of<false>(amax);
+    const float inv = blockq::inverse_scale(s);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint4 q;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            w[c] = blockq::codes4<false>(v[i].get(4 * c) * inv, v[i].get(4 * c + 1) * inv, v[i].get(4 * c + 2) * inv,
+                                         v[i].get(4 * c + 3) * inv);
+        *reinterpret_cast<uint4*>(tile + row * 128 + ((((lane & 3) * 2 + i) ^ (row & 7)) << 4)) = q;
+    }
+    if ((lane & 3) == 0) *reinterpret_cast<uint32_t*>(atom + row * 16) = s;   // rows from 16 on: no output reads them
+}
+
+template <bool FP8, int BN, int CTAS, bool OWN = false>
 __global__ void __launch_bounds__(kThreads, 1)
 k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
           const __grid_constant__ ProdJob j) {
-    using S = Shape<FP8, BN, CTAS>;
+    using S = Shape<FP8, BN, CTAS, OWN>;
+    static_assert(!OWN || (FP8 && BN == 16 && CTAS == 1 && S::kHalves == 1), "rows are quantised 16 at a time");
     constexpr int kStep = FP8 ? kStepBytes : kStepBytes / 2;   // contraction values per step
     constexpr int BM = kBM * CTAS;
     extern __shared__ uint8_t raw[];
@@ -612,13 +657,13 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     if (warp == 3) columns_alloc<CTAS>(&tmem_slot, S::kCols);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(full + i, 1);
+            mbar_init(full + i, OWN ? 3 : 1);
             mbar_init(empty + i, 1);
             mbar_init(fixed + i, CTAS);
             mbar_init(landed + i, 1);
         }
         for (int i = 0; i < kScaleSlots; ++i) {
-            mbar_init(scales_full + i, 1);
+            mbar_init(scales_full + i, OWN ? 2 : 1);
             mbar_init(scales_there + i, 1);
             mbar_init(scales_empty + i, 1);
             mbar_init(scales_here + i, 1);
@@ -766,7 +811,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                         mbar_arrive_expect_tx(landed + stage, S::kStage);
                         if (CTAS == 1 || rank == 0) mbar_arrive(full + stage);
                     } else if (!begun && (CTAS == 1 || rank == 0)) {
-                        mbar_arrive_expect_tx(full + stage, S::kStage * CTAS);
+                        mbar_arrive_expect_tx(full + stage, OWN ? S::kATile : S::kStage * CTAS);
                     }
                     if (begun) {
                     } else if (j.a_mn) {
@@ -774,7 +819,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     } else {
                         tma_3d<CTAS>(a, &ma, k, x.p0 + a_off, ea, bar);
                     }
-                    if (j.b_mn) {
+                    if (OWN) {
+                    } else if (j.b_mn) {
                         for (int c = 0; c < S::kBRows / 64; ++c)
                             tma_3d<CTAS>(b + c * 8192, &mb, x.q0 + b_off + c * 64, k, eb, bar);
                     } else {
@@ -817,7 +863,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     if (FP8 && byte == 0) ok = ok && wait(scales_full + slot, slot_phase);
                     if (!(ok = __all_sync(~0u, ok))) break;
                     fence_after_sync();
-                    const bool group_ends = FP8 && (byte == kGroupSteps - 1 || k + kStep >= x.k1);
+                    const bool group_ends = FP8 && (byte == S::kGroup - 1 || k + kStep >= x.k1);
                     if (elected()) {
                         const uint64_t da = desc_a + uint32_t(stage * (S::kStage >> 4));
                         const uint64_t db = desc_b + uint32_t(stage * (S::kStage >> 4));
@@ -866,7 +912,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 bool ok = true;
                 for (int t = first_tile; ok && t < tiles; t += stride) {
                     const Tile x = tile_at<BM, BN>(j, g, t, kStep);
-                    for (int k = x.k0; k < x.k1; k += kGroupSteps * kStep) {
+                    for (int k = x.k0; k < x.k1; k += S::kGroup * kStep) {
                         if (!(ok = wait(scales_here + slot, phase))) break;
                         arrive_first<CTAS>(scales_there + slot, rank, true);
                         if (++slot == kScaleSlots) slot = 0, phase ^= 1;
@@ -874,8 +920,10 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 }
             }
         }
-    } else if (warp == 2 || (FP8 && warp == 3)) {
-        [[maybe_unused]] int stage = 0;
+    } else if (warp == 2 || (FP8 && warp == 3) || (OWN && (warp == 8 || warp == 9))) {
+        [[maybe_unused]] const int turn = warp & 1, half = warp >> 3;   // which atoms; OWN: which rows
+        [[maybe_unused]] int stage = OWN ? turn : 0;
+        [[maybe_unused]] uint32_t stage_phase = 0;
         uint32_t phase = 0;
         [[maybe_unused]] bool ok = true;
         if constexpr (FP8) {
@@ -884,14 +932,19 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             const ScaleWay way_a = scale_way(j.sa, j.a_rows, j.grouping == kRowsA);
             const ScaleWay way_b = scale_way(j.sb, j.b_rows, j.grouping == kRowsB);
             RawScales raw_a, raw_b[S::kAtomsB];
+            OwnRows own;
             auto load = [&](const Tile& x, int k) {
                 const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
                 load_scales(raw_a, j.sa, way_a, ea, x.p0 + a_off, j.a_rows, k / kBlock, blocks);
+                if constexpr (OWN) {
+                    load_own(own, j, x, half, k);
+                } else {
 #pragma unroll
-                for (int i = 0; i < S::kAtomsB; ++i)
-                    load_scales(raw_b[i], j.sb, way_b, eb, x.q0 + 128 * i, j.b_rows, k / kBlock, blocks);
+                    for (int i = 0; i < S::kAtomsB; ++i)
+                        load_scales(raw_b[i], j.sb, way_b, eb, x.q0 + 128 * i, j.b_rows, k / kBlock, blocks);
+                }
             };
-            // The two warps take every other group each.
+            // The two warps (of OWN: two pairs) take every other group each.
             int t = first_tile, k = 0;
             Tile x{};
             // To the first step of a tile that has one, and from group to group.
@@ -904,24 +957,35 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 }
             };
             auto advance = [&] {
-                k += kGroupSteps * kStep;
+                k += S::kGroup * kStep;
                 if (k >= x.k1) {
                     t += stride;
                     settle();
                 }
             };
             settle();
-            if (warp == 3 && t < tiles) advance();
+            if (turn == 1 && t < tiles) advance();
             if (t < tiles) load(x, k);
-            int slot = warp - 2;
+            int slot = turn;
             for (bool more = t < tiles; more;) {
                 if (!__all_sync(~0u, wait(scales_empty + slot, phase ^ 1))) break;
                 uint8_t* dst = scales + slot * S::kScaleBytes;
-                store_scales(raw_a, way_a, dst);
+                if (!OWN || half == 0) store_scales(raw_a, way_a, dst);
+                if constexpr (OWN) {
+                    if (!__all_sync(~0u, wait(empty + stage, stage_phase ^ 1))) break;
+                    uint8_t* tile = ring + stage * S::kStage + S::kATile;
+                    if (j.values_type == kF16) store_own<__half>(own, half, tile, dst + kAtom);
+                    else store_own<__nv_bfloat16>(own, half, tile, dst + kAtom);
+                } else {
 #pragma unroll
-                for (int i = 0; i < S::kAtomsB; ++i) store_scales(raw_b[i], way_b, dst + (1 + i) * kAtom);
+                    for (int i = 0; i < S::kAtomsB; ++i) store_scales(raw_b[i], way_b, dst + (1 + i) * kAtom);
+                }
                 fence_async_smem();
                 __syncwarp();
+                if constexpr (OWN) {
+                    if (lane == 0) mbar_arrive(full + stage);
+                    if ((stage += 2) >= S::kStages) stage -= S::kStages, stage_phase ^= 1;
+                }
                 // The first CTA's warp also takes in the other one's word, an acquire of cluster scope that would
                 // cost the MMA warp 480 cycles per group.
                 if (CTAS == 2 && rank == 0 && !__all_sync(~0u, wait_all<CTAS>(scales_there + slot, phase))) break;
@@ -1112,10 +1176,10 @@ int sm_count(int device) {
     return known[device];
 }
 
-template <bool FP8, int BN, int CTAS>
+template <bool FP8, int BN, int CTAS, bool OWN = false>
 void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long long tiles, int device,
             cudaStream_t stream) {
-    using S = Shape<FP8, BN, CTAS>;
+    using S = Shape<FP8, BN, CTAS, OWN>;
     constexpr size_t most = S::kSmem + std::max(S::kBias, 2 * (kMaxGroups + 1) * sizeof(int));
     static_assert(most <= 227 * 1024, "shared memory of a CTA");
     const size_t lists = j.balance ? size_t(j.groups + 2 * j.by_lanes.d + 16) : 0;
@@ -1127,7 +1191,7 @@ void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long l
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[device]) {
-            AEISU_CUDA(cudaFuncSetAttribute(k_product<FP8, BN, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            AEISU_CUDA(cudaFuncSetAttribute(k_product<FP8, BN, CTAS, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             int(most)));
             ready[device] = true;
         }
@@ -1148,7 +1212,7 @@ void launch(const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long l
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    AEISU_CUDA(cudaLaunchKernelEx(&cfg, k_product<FP8, BN, CTAS>, a, b, j));
+    AEISU_CUDA(cudaLaunchKernelEx(&cfg, k_product<FP8, BN, CTAS, OWN>, a, b, j));
 }
 
 // Tile of a product: columns, and CTAs that share it.
@@ -1161,6 +1225,8 @@ struct TileShape {
 template <bool FP8>
 void launch_shape(TileShape s, const CUtensorMap& a, const CUtensorMap& b, const ProdJob& j, long long tiles, int device,
                   cudaStream_t stream) {
+    if constexpr (FP8)
+        if (j.values) return launch<true, 16, 1, true>(a, b, j, tiles, device, stream);
     if (s.ctas == 2) return launch<FP8, 256, 2>(a, b, j, tiles, device, stream);
     switch (s.bn) {
         case 16: return launch<FP8, 16, 1>(a, b, j, tiles, device, stream);
@@ -1271,10 +1337,30 @@ size_t product_workspace(int m, int n, int k, int device) {
     return p.split > p.cluster ? size_t(p.split) * m * n * sizeof(float) : 0;
 }
 
-void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
-             void* workspace, size_t workspace_bytes, bool after_quantize, int device, cudaStream_t stream) {
-    check_operand(a, &sa);
-    check_operand(b, &sb);
+namespace {
+
+constexpr int kOwnRows = 16;   // rows that a product quantises itself
+
+// Whether the kernel quantises the rows of x itself: few of them, 16-bit and aligned.
+bool takes_values(const MatrixRef& x, long long rows) {
+    return (x.type == kF16 || x.type == kBF16) && aligned(x.ptr, 16) && x.ld % 8 == 0 && x.cols % 8 == 0 &&
+           rows <= kOwnRows;
+}
+void give_values(ProdJob& j, const MatrixRef& x) {
+    j.values = x.ptr;
+    j.values_type = x.type;
+    j.values_ld = x.ld;
+}
+// x as the operand that the kernel makes of it.
+MatrixRef as_codes(const MatrixRef& x) {
+    MatrixRef m = x;
+    m.type = kE4M3;
+    return m;
+}
+
+void dense(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
+           void* workspace, size_t workspace_bytes, const MatrixRef* values, bool after_quantize, int device,
+           cudaStream_t stream) {
     require(a.batch == 1 && b.batch == 1 && a.cols == b.cols, "contraction sizes differ");
     require(out.ptr && out.type >= kF32 && out.type <= kBF16 && out.ld >= b.rows, "output is out of range");
     OnDevice on(device);
@@ -1300,6 +1386,10 @@ void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const S
     j.cluster = pl.cluster;
     j.after_quantize = after_quantize;
     j.early_a = after_quantize && pl.swap;
+    if (values) {
+        require(pl.swap && pl.tile.bn == kOwnRows, "rows are quantised 16 at a time");
+        give_values(j, *values);
+    }
     if (pl.split > pl.cluster) {
         j.out = workspace;
         j.out_type = kF32;
@@ -1315,7 +1405,7 @@ void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const S
     j.out_vec = whole_rows(j.out, j.out_type, j.out_ld, j.split_stride);
     const long long tiles = ceil_div(j.P, pl.tile.rows()) * ceil_div(j.Q, pl.tile.bn) * pl.split;
     require(tiles < (1LL << 30), "matrix is too large");
-    const CUtensorMap ma = operand_map(A, kBM), mb = operand_map(B, pl.tile.b_rows());
+    const CUtensorMap ma = operand_map(A, kBM), mb = values ? ma : operand_map(B, pl.tile.b_rows());
     launch_shape<true>(pl.tile, ma, mb, j, tiles, device, stream);
     if (pl.split > pl.cluster) {
         const long long n = (long long)a.rows * b.rows;
@@ -1326,10 +1416,9 @@ void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const S
     }
 }
 
-void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const ScaleRef* sb, const int* off,
-                     const ProductOut& out, bool zero_outside, bool after_quantize, int device, cudaStream_t stream) {
-    check_operand(x, sx);
-    check_operand(b, sb);
+void grouped(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const ScaleRef* sb, const int* off,
+             const ProductOut& out, bool zero_outside, const MatrixRef* values, bool after_quantize, int device,
+             cudaStream_t stream) {
     require(x.batch == 1 && !x.trans && x.cols == b.cols, "contraction sizes differ");
     require((sx != nullptr) == (sb != nullptr) && (sx || x.type == b.type), "operand types do not go together");
     require(off && b.batch <= kMaxGroups, "a grouped product has offsets and at most 1024 groups");
@@ -1374,6 +1463,10 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     j.split = j.cluster = 1;
     j.after_quantize = after_quantize;
     j.early_a = after_quantize && swap && fp8;
+    if (values) {
+        require(swap && tile.bn == kOwnRows, "rows are quantised 16 at a time");
+        give_values(j, *values);
+    }
     j.zero_outside = zero_outside;
     j.zero_rows = x.rows;
     j.out_vec = whole_rows(out.ptr, out.type, out.ld, 0);
@@ -1381,9 +1474,44 @@ void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b,
     const int high = swap ? tile.bn : tile.rows(), wide = swap ? tile.rows() : tile.bn;
     const long long tiles = (ceil_div(x.rows, high) + std::min(b.batch, x.rows)) * ceil_div(b.rows, wide);
     require(tiles < (1LL << 30), "matrix is too large");
-    const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM), mb = operand_map(B, B.trans ? 64 : tile.b_rows());
+    const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM), mb = values ? ma : operand_map(B, B.trans ? 64 : tile.b_rows());
     if (fp8) launch_shape<true>(tile, ma, mb, j, tiles, device, stream);
     else launch_shape<false>(tile, ma, mb, j, tiles, device, stream);
+}
+
+}  // namespace
+
+void product(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
+             void* workspace, size_t workspace_bytes, bool after_quantize, int device, cudaStream_t stream) {
+    check_operand(a, &sa);
+    check_operand(b, &sb);
+    dense(a, sa, b, sb, out, workspace, workspace_bytes, nullptr, after_quantize, device, stream);
+}
+
+bool product_of_values(const MatrixRef& x, const MatrixRef& b, const ScaleRef& sb, const ProductOut& out,
+                       void* workspace, size_t workspace_bytes, int device, cudaStream_t stream) {
+    if (!takes_values(x, x.rows) || b.rows <= x.rows) return false;
+    check_operand(b, &sb);
+    require(x.ptr && x.rows >= 1 && x.ld >= x.cols && !x.trans, "matrix sizes are out of range");
+    dense(as_codes(x), ScaleRef{sb.ptr, 0, x.rows, 0}, b, sb, out, workspace, workspace_bytes, &x, false, device, stream);
+    return true;
+}
+
+void grouped_product(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const ScaleRef* sb, const int* off,
+                     const ProductOut& out, bool zero_outside, bool after_quantize, int device, cudaStream_t stream) {
+    check_operand(x, sx);
+    check_operand(b, sb);
+    grouped(x, sx, b, sb, off, out, zero_outside, nullptr, after_quantize, device, stream);
+}
+
+bool grouped_product_of_values(const MatrixRef& x, const MatrixRef& b, const ScaleRef& sb, const int* off,
+                               const ProductOut& out, bool zero_outside, int device, cudaStream_t stream) {
+    if (!takes_values(x, ceil_div(x.rows, b.batch)) || b.rows < kBM) return false;
+    check_operand(b, &sb);
+    require(x.ptr && x.rows >= 1 && x.ld >= x.cols && !x.trans, "matrix sizes are out of range");
+    const ScaleRef none{sb.ptr, 0, x.rows, 0};
+    grouped(as_codes(x), &none, b, &sb, off, out, zero_outside, &x, false, device, stream);
+    return true;
 }
 
 void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* off, int groups, void* out,

@@ -58,6 +58,9 @@ size_t linear_workspace(int m, int n, int k, int pass, int device) {
 void linear_serve(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, const ProductOut& out, void* workspace,
                   size_t workspace_bytes, int device, cudaStream_t stream) {
     check_workspace(workspace, workspace_bytes, linear_workspace(x.rows, w.rows, x.cols, kServe, device));
+    // Few rows: one kernel does both (one token through 4,096 x 4,096: 12 us a call instead of 16, of which the
+    // GPU takes 9.5 either way).
+    if (product_of_values(x, w, sw, out, workspace, workspace_bytes, device, stream)) return;
     const Operand q = operand_at(workspace, kE4M3, x.rows, x.cols, 1);
     const size_t used = operand_bytes(x.rows, x.cols, 1);
     quantize_into(x, 1, q, nullptr, nullptr, device, stream);
@@ -116,6 +119,7 @@ size_t grouped_linear_workspace(int rows, int k) { return operand_bytes(rows, k,
 void grouped_linear(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, const int* off, const ProductOut& out,
                     bool zero_outside, void* workspace, size_t workspace_bytes, int device, cudaStream_t stream) {
     check_workspace(workspace, workspace_bytes, grouped_linear_workspace(x.rows, x.cols));
+    if (grouped_product_of_values(x, w, sw, off, out, zero_outside, device, stream)) return;
     const Operand q = operand_at(workspace, kE4M3, x.rows, x.cols, 1);
     quantize_into(x, 1, q, nullptr, nullptr, device, stream);
     grouped_product(q.m, &q.s, w, &sw, off, out, zero_outside, true, device, stream);

@@ -197,6 +197,23 @@ def test_linear_serving_matches_training_forward():
     assert torch.equal(y, B.matmul(B.quantize(x), kept, bias=b, dtype=torch.float16))
 
 
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17])
+@pytest.mark.parametrize("n, k", [(17, 8), (130, 200), (1000, 4096), (257, 1032), (64, 130)])
+def test_few_rows_are_quantised_alike(m, n, k):
+    # few aligned 16-bit rows are quantised inside the product, others by a kernel of their own: the same codes, so
+    # the same bits, whatever the rows hold
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = randn(m, k, dtype=dtype) * torch.exp2(torch.arange(m).float() - 8)[:, None].cuda().to(dtype)
+        w, b = B.quantize(randn(n, k, seed=1), rows=128), randn(n, seed=2)
+        if m > 4:
+            x[1], x[2, 0], x[3, k // 2:], x[4, -1] = 0, float("nan"), float("inf"), -float("inf")
+        for v in (x, torch.nn.functional.pad(x, (1, 8))[:, 1:k + 1]):
+            y = B.linear(v, w, b)
+            assert torch.equal(y.nan_to_num(1e9), B.matmul(B.quantize(v), w, bias=b, dtype=dtype).nan_to_num(1e9))
+        if m <= 4:
+            O.check_product(y, O.values(x), w.dequantize(), b)
+
+
 def test_linear_empty():
     x = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     w = randn(32, 64, dtype=torch.bfloat16).requires_grad_()
