@@ -23,23 +23,33 @@ from .block_fp8 import BlockFP8
 
 MAX_GROUPS = 1024
 _HALVES = (torch.float16, torch.bfloat16)
+_call = _lib.lib
+_pack = _lib.MATRIX.pack
 
 
-def _weights(weight):
-    """(tensor kept, aeisu_matrix) of weights [E, N, K] stored with either of the last two contiguous."""
-    flip = weight.transpose(1, 2)
-    if mx.row_stride(weight) is None and mx.row_stride(flip) is not None:
-        t, ld = mx.operand(flip)
+def _weights(weight, flip=False):
+    """(tensor kept, aeisu_matrix) of weights [E, N, K], or of their transposes [E, K, N], stored with either of
+    the last two dimensions contiguous."""
+    e, n, k = weight.shape
+    at = weight.data_ptr()
+    if weight.stride() == (n * k, k, 1) and k % 8 == 0 and at % 16 == 0 and (k > 1 or not flip):
+        rows, cols = (k, n) if flip else (n, k)
+        return weight, _pack(at, 0, mx.TYPES[weight.dtype], rows, cols, e, k, n * k, 0, flip)
+    if flip:
+        weight = weight.transpose(1, 2)
+    other = weight.transpose(1, 2)
+    if mx.row_stride(weight) is None and mx.row_stride(other) is not None:
+        t, ld = mx.operand(other)
         return t, mx.matrix(t, ld, transposed=True)
     t, ld = mx.operand(weight)
     return t, mx.matrix(t, ld)
 
 
-def _product(x, weight, offsets, out, zero_outside):
-    """x, weight: (tensors kept, aeisu_matrix)."""
+def _product(x, weight, offsets, out, ld, zero_outside):
+    """x, weight: (tensors kept, aeisu_matrix); ld: elements from row to row of out."""
     index = out.get_device()
-    _lib.check(_lib.lib().aeisu_grouped_product(x[1], weight[1], offsets.data_ptr(), zero_outside,
-                                                mx.matrix(out, mx.row_stride(out)), index, mx.stream(index)))
+    _lib.check(_call().aeisu_grouped_product(x[1], weight[1], offsets.data_ptr(), zero_outside, mx.matrix(out, ld), index,
+                                             mx.stream(index)))
     return out
 
 
@@ -51,11 +61,11 @@ def _rows(x):
 class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
-        ctx.save_for_backward(x, weight, offsets)
-        out = x.new_empty((x.shape[0], weight.shape[1]))
-        if x.shape[0] == 0:
-            return out
-        return _product(_rows(x), _weights(weight), offsets, out, True)
+        t, n = x.shape[0], weight.shape[1]
+        kept = _rows(x)      # an aligned copy serves the backward pass too
+        ctx.save_for_backward(kept[0], weight, offsets)
+        out = x.new_empty((t, n))
+        return _product(kept, _weights(weight), offsets, out, n, True) if t else out
 
     @staticmethod
     def backward(ctx, grad):
@@ -64,20 +74,20 @@ class _Grouped(torch.autograd.Function):
     @staticmethod
     def once(ctx, grad):
         x, weight, offsets = ctx.saved_tensors
-        if x.shape[0] == 0:
-            return torch.empty_like(x), torch.zeros_like(weight), None
+        t, k = x.shape
+        need_x, need_w, _ = ctx.needs_input_grad
+        if t == 0:
+            return x.new_empty((0, k)), torch.zeros_like(weight), None
         g = _rows(grad)
         gx = gw = None
-        if ctx.needs_input_grad[0]:
-            gx = x.new_empty(x.shape)
-            _product(g, _weights(weight.transpose(1, 2)), offsets, gx, True)
-        if ctx.needs_input_grad[1]:
+        if need_x:
+            gx = _product(g, _weights(weight, True), offsets, x.new_empty((t, k)), k, True)
+        if need_w:
             gw = weight.new_empty(weight.shape)
             kept = _rows(x)
             index = gw.get_device()
-            _lib.check(_lib.lib().aeisu_grouped_weight_gradient(g[1], kept[1], offsets.data_ptr(), weight.shape[0],
-                                                                gw.data_ptr(), mx.TYPES[gw.dtype], index,
-                                                                mx.stream(index)))
+            _lib.check(_call().aeisu_grouped_weight_gradient(g[1], kept[1], offsets.data_ptr(), weight.shape[0],
+                                                             gw.data_ptr(), mx.TYPES[gw.dtype], index, mx.stream(index)))
         return gx, gw, None
 
     twice = staticmethod(once_differentiable(lambda ctx, grad: _Grouped.once(ctx, grad)))
@@ -126,21 +136,21 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
         out = offsets.new_empty((t, n), dtype=dtype)
     if t == 0:
         return out
+    ld = n if new else mx.row_stride(out)
     offsets = offsets.contiguous()
     if not fp8:
-        return _product(_rows(x), _weights(weight), offsets, out, new)
+        return _product(_rows(x), _weights(weight), offsets, out, ld, new)
     if coded:
-        return _product(x.matrix(), weight.matrix(), offsets, out, new)
+        return _product(x.matrix(), weight.matrix(), offsets, out, ld, new)
     k = x.shape[1]
-    ld = mx.row_stride(x)
-    if ld is None:
+    stride = mx.row_stride(x)
+    if stride is None:
         x = x.detach().contiguous()
-        ld = k
-    size = _lib.lib().aeisu_grouped_linear_workspace(t, k)
+        stride = k
+    size = _call().aeisu_grouped_linear_workspace(t, k)
     ws, (codes, mw) = mx.scratch(size, x), weight.matrix()
-    _lib.check(_lib.lib().aeisu_grouped_linear(mx.matrix(x, ld), mw, offsets.data_ptr(), new,
-                                               mx.matrix(out, mx.row_stride(out)), ws.data_ptr(), size, index,
-                                               mx.stream(index)))
+    _lib.check(_call().aeisu_grouped_linear(mx.matrix(x, stride), mw, offsets.data_ptr(), new, mx.matrix(out, ld),
+                                            ws.data_ptr(), size, index, mx.stream(index)))
     return out
 
 
