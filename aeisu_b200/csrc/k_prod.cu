@@ -244,8 +244,9 @@ __device__ __forceinline__ bool elected() {
 }
 
 // The clock is read only once a first try has failed: the MMA warp's waits are part of every step.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-    return mbar_try_wait(bar, parity) || mbar_wait_bounded(bar, parity, &g_product_error, kErrWait);
+constexpr long long kWaitCycles = 4000000000LL;
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, long long more = 0) {
+    return mbar_try_wait(bar, parity) || mbar_wait_bounded(bar, parity, &g_product_error, kErrWait, kWaitCycles + more);
 }
 // As wait, for a phase that threads of the other CTA complete as well.  (An acquire on the barrier: a
 // fence of cluster scope here doubled the time of every step.)
@@ -263,7 +264,7 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
     if (done()) return true;
     const long long t0 = clock64();
     while (!done()) {
-        if (clock64() - t0 > 4000000000LL) {
+        if (clock64() - t0 > kWaitCycles) {
             atomicCAS(&g_product_error, 0, kErrWait);
             return false;
         }
@@ -1037,7 +1038,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 __syncwarp();
                 bias_q = x.q0;
             }
-            if (!__all_sync(~0u, wait(acc_full + acc, acc_phase))) break;
+            // A tile of a very long contraction takes its time: 20,000 cycles more for each step of about 500.
+            if (!__all_sync(~0u, wait(acc_full + acc, acc_phase, (x.k1 - x.k0) / kStep * 20000LL))) break;
             fence_after_sync();
             uint32_t v[S::kWide];
             if (x.k0 < x.k1) {
