@@ -67,7 +67,7 @@ struct ProdJob {
     int grouping, groups;
     const int* off;
     int a_mn, b_mn;              // operand stored with its rows contiguous (contraction strided)
-    uint32_t idesc;
+    uint32_t idesc;              // instruction descriptor without the columns
     ScaleRef sa, sb;
     int a_rows, b_rows;          // rows that carry scales, for clamping
     void* out;
@@ -365,6 +365,14 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
     return x;
 }
 
+// Columns that the MMAs of a tile compute: those that are stored, in whole steps of the instruction; a pair's
+// CTAs take half of these rows of B each.  (Rows stored with their contraction strided come in chunks of 64.)
+template <int BN, int CTAS>
+__device__ __forceinline__ int tile_columns(const ProdJob& j, const Tile& x) {
+    constexpr int kGrain = 16 * CTAS;
+    return j.b_mn ? BN : min(BN, (x.q1 - x.q0 + kGrain - 1) / kGrain * kGrain);
+}
+
 // ---- scales ------------------------------------------------------------------------------------
 
 // How the scales of an operand are read.
@@ -546,44 +554,53 @@ __device__ __forceinline__ void write_columns(const ProdJob& j, const uint32_t* 
         if (q0 + c < q1) out[(q0 + c) * j.out_ld + p] = rounded<T>(__uint_as_float(v[c]) + b);
 }
 
-// The parts of a tile, one in the shared memory of each of the cluster's CTAs as [column][128 rows],
-// added in their order; each CTA takes its share of the columns, a thread four rows at a time, with the
-// loads of all parts and of two columns under way at once.
+// A tile's part goes to the ring in the order of the output: [column][128 rows] where out[q][p], else [row][BN + 4
+// columns], whose four columns more keep the rows' 16-byte pieces in different banks.
+template <int BN, int W>
+__device__ __forceinline__ void put_part(const ProdJob& j, const uint32_t* v, uint8_t* ring, int row, int col) {
+    uint32_t* tile = reinterpret_cast<uint32_t*>(ring);
+    if (j.swapped) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) tile[(col + i) * kBM + row] = v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 4)
+            *reinterpret_cast<uint4*>(tile + row * (BN + 4) + col + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
+}
+// The parts of a tile, one in the shared memory of each of the cluster's CTAs, added in their order; each CTA
+// takes its share of the lines (rows or columns) of the output, a thread four neighbouring values, with the
+// loads of all parts and of two lines under way at once.
 template <int BN, int PARTS>
 __device__ __forceinline__ void join_cluster(const ProdJob& j, const Tile& x, int rank, uint32_t tile) {
-    constexpr int kShare = BN / PARTS, kAtOnce = 32 * kWriters / 32;   // columns; 32 threads for each
-    const int t = threadIdx.x - 128, r4 = (t & 31) * 4, p = x.p0 + r4;
+    const int lines = j.swapped ? BN : kBM, wide = j.swapped ? kBM : BN, pitch = j.swapped ? kBM : BN + 4;
+    const int line0 = j.swapped ? x.q0 : x.p0, line1 = j.swapped ? x.q1 : x.p1;      // of the output, and its values
+    const int at0 = j.swapped ? x.p0 : x.q0, at1 = j.swapped ? x.p1 : x.q1;
+    const int share = lines / PARTS, quads = wide / 4, t = threadIdx.x - 128;
     uint32_t part[PARTS];
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) part[i] = address_in(tile, i);
-    float pb[4] = {};
-    if (j.bias && j.swapped)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (p + i < x.p1) pb[i] = load_elem(j.bias, j.bias_type, p + i);
 #pragma unroll 2
-    for (int c = t >> 5; c < kShare; c += kAtOnce) {
-        const int col = rank * kShare + c, q = x.q0 + col;
-        if (q >= x.q1) continue;
+    for (int u = t; u < share * quads; u += 32 * kWriters) {
+        const int line = rank * share + u / quads, c = u % quads * 4, l = line0 + line, at = at0 + c;
+        if (l >= line1 || at >= at1) continue;
         float4 v[PARTS];
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                          : "=f"(v[i].x), "=f"(v[i].y), "=f"(v[i].z), "=f"(v[i].w)
-                         : "r"(part[i] + uint32_t(col * kBM + r4) * 4) : "memory");
+                         : "r"(part[i] + uint32_t(line * pitch + c) * 4) : "memory");
         float4 s = v[0];
 #pragma unroll
         for (int i = 1; i < PARTS; ++i) s.x += v[i].x, s.y += v[i].y, s.z += v[i].z, s.w += v[i].w;
-        const float qb = j.bias && !j.swapped ? load_elem(j.bias, j.bias_type, q) : 0.f;
         const float o[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (p + i < x.p1)
-                store_elem(j.out, j.out_type, j.swapped ? q * j.out_ld + p + i : (p + i) * j.out_ld + q, o[i] + qb + pb[i]);
+            if (at + i < at1)
+                store_elem(j.out, j.out_type, l * j.out_ld + at + i,
+                           o[i] + (j.bias ? load_elem(j.bias, j.bias_type, at + i) : 0.f));
     }
 }
-
-// ---- the kernel --------------------------------------------------------------------------------
 
 // Few rows quantised on the spot (OWN): a warp's half, eight rows, of the rows q0 .. q0 + 15 of the 16-bit B by
 // 128 columns from k on, four lanes to a row.  Loaded a step ahead, turned into codes of the stage's swizzled
@@ -771,7 +788,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                            : j.cluster > 1 ? rank * (tiles / j.split) + int(blockIdx.x) / j.cluster
                                            : int(blockIdx.x);
     const int stride = g.deal ? 1 : CTAS == 2 ? int(gridDim.x) / 2 : j.cluster > 1 ? tiles : int(gridDim.x);
-    const int a_off = CTAS == 2 ? rank * kBM : 0, b_off = CTAS == 2 ? rank * S::kBRows : 0;
+    const int a_off = CTAS == 2 ? rank * kBM : 0;
 
     // Warps 0 and 1 run their loops as whole warps and elect a lane for the copies and MMAs only: addresses
     // and descriptors then stay in uniform registers.  With one lane running the loop an MMA step took
@@ -798,6 +815,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             const Tile x = tile_at<BM, BN>(j, g, t, kStep);
             if (x.p0 < 0) continue;
             const int ea = j.grouping == kRowsB ? x.e : 0, eb = j.grouping == kRowsA ? x.e : 0;
+            const int b_off = CTAS == 2 ? rank * (tile_columns<BN, CTAS>(j, x) / 2) : 0;
             for (int k = x.k0; k < x.k1; k += kStep) {
                 if (!(ok = __all_sync(~0u, wait(empty + stage, phase ^ 1)))) break;
                 // A pair's copies all count on its first CTA's barrier.  Where rows have to be zeroed first, each
@@ -852,7 +870,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 const Tile x = tile_at<BM, BN>(j, g, t, kStep);
                 if (x.p0 < 0) continue;
                 if (!(ok = __all_sync(~0u, wait(acc_empty + acc, acc_phase ^ 1)))) break;
-                const uint32_t d = tmem + acc * BN;
+                const uint32_t d = tmem + acc * BN, idesc = j.idesc | uint32_t(tile_columns<BN, CTAS>(j, x) >> 3) << 17;
                 uint32_t byte = 0;
                 for (int k = x.k0; k < x.k1; k += kStep) {
                     if (j.grouping == kContraction && k + kStep > x.k1) {
@@ -876,13 +894,13 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
 #pragma unroll
                                 for (int i = 0; i <= S::kAtomsB; ++i) scales_to_tmem<CTAS>(sf + 4 * i, src + i * kAtom);
                             }
-                            const uint32_t id = j.idesc | (byte << 4) | (byte << 29);
+                            const uint32_t id = idesc | (byte << 4) | (byte << 29);
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 mma_block_scaled<CTAS>(d, da + i * 2, db + i * 2, id, sf, sf + 4, i ? 1 : more);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) mma_half<CTAS>(d, da + i * a_k, db + i * b_k, j.idesc, i ? 1 : more);
+                            for (int i = 0; i < 4; ++i) mma_half<CTAS>(d, da + i * a_k, db + i * b_k, idesc, i ? 1 : more);
                         }
                         commit_all<CTAS>(empty + stage);
                         if (group_ends) commit_all<CTAS>(scales_empty + slot);
@@ -1059,10 +1077,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             const int p0 = x.p0 + a_off + quad * 32, q0 = x.q0 + col;
             const long long base = x.part * j.split_stride + (j.grouping == kContraction ? x.e * j.out_batch : 0);
             if (CTAS == 1 && j.cluster > 1) {
-                // every MMA of this CTA is done with the ring: it takes the tile, column by column
-#pragma unroll
-                for (int i = 0; i < S::kWide; ++i)
-                    reinterpret_cast<uint32_t*>(ring)[(col + i) * kBM + quad * 32 + lane] = v[i];
+                // every MMA of this CTA is done with the ring
+                put_part<BN, S::kWide>(j, v, ring, quad * 32 + lane, col);
             } else if (j.swapped) {
                 if (j.out_type == kF32) write_columns<float, S::kWide>(j, v, base, p0 + lane, x.p1, q0, x.q1);
                 else if (j.out_type == kF16) write_columns<__half, S::kWide>(j, v, base, p0 + lane, x.p1, q0, x.q1);
@@ -1261,7 +1277,7 @@ TileShape choose_tile(long long row_tiles_of_128, int q, long long count, long l
 }
 
 uint32_t instruction(const MatrixRef& a, const MatrixRef& b, TileShape s) {
-    const uint32_t size = (uint32_t(s.bn >> 3) << 17) | (uint32_t(s.rows() >> 4) << 24);
+    const uint32_t size = uint32_t(s.rows() >> 4) << 24;
     if (is_code(a.type))
         return size | (uint32_t(a.type == kE5M2) << 7) | (uint32_t(b.type == kE5M2) << 10) | (1u << 23);
     const uint32_t f = a.type == kBF16 ? 1 : 0;
