@@ -94,7 +94,7 @@ def random_blocks(r, c, rows, dtype, seed):
 
 SIZES = [(1, 1, 1), (1, 16, 128), (1, 300, 4096), (2, 129, 130), (5, 17, 33), (16, 128, 512), (17, 1000, 640),
          (64, 100, 1100), (65, 200, 64), (127, 64, 255), (128, 256, 128), (129, 128, 257), (300, 1000, 520),
-         (513, 48, 32), (1030, 333, 700), (2000, 2050, 129)]
+         (513, 48, 32), (1030, 333, 700), (2000, 2050, 129), (100, 131, 1100), (200, 77, 4096), (90, 512, 2048)]
 
 
 @pytest.mark.parametrize("m, n, k", SIZES)
@@ -104,6 +104,27 @@ def test_matmul(m, n, k, types):
     O.check_product(B.matmul(a, b, dtype=torch.float32), a.dequantize(), b.dequantize())
     bias = randn(n, scale=100.0)
     O.check_product(B.matmul(a, b, bias=bias), a.dequantize(), b.dequantize(), bias)
+
+
+@pytest.mark.parametrize("m, n, k", [(64, 128, 20_000), (33, 17, 30_001), (1, 100, 40_000), (130, 120, 25_000)])
+def test_long_contractions_in_parts(m, n, k):
+    # few outputs: the contraction is cut over all SMs and the parts are joined by a second kernel
+    a, b, bias = random_blocks(m, k, 1, E4, 1), random_blocks(n, k, 1, E4, 2), randn(n, scale=1e4)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = B.matmul(a, b, bias=bias, dtype=dtype)
+        O.check_product(y, a.dequantize(), b.dequantize(), bias)
+        assert torch.equal(y, B.matmul(a, b, bias=bias, dtype=dtype))
+
+
+def test_gradients_of_a_narrow_layer_over_many_rows():
+    x, w = randn(20_011, 64, dtype=torch.bfloat16).requires_grad_(), randn(48, 64, seed=1, dtype=torch.bfloat16).requires_grad_()
+    b, g = randn(48, seed=2).requires_grad_(), randn(20_011, 48, seed=3, scale=1e-3, dtype=torch.bfloat16)
+    gx, gw, gb = torch.autograd.grad(B.linear(x, w, b), (x, w, b), g)
+    rows = torch.arange(0, 20_011, 97)
+    O.check_product(gx[rows.cuda()], O.values(g[rows.cuda()]), O.values(w.detach().t(), 128))
+    O.check_product(gw, O.values(g.t()), O.values(x.detach().t()))
+    s = g.double().cpu()
+    O.check(gb, s.sum(0), 20_012 * 2.0 ** -24 * s.abs().sum(0))
 
 
 @pytest.mark.parametrize("rows", [(1, 1), (128, 1), (128, 128)])

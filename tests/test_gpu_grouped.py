@@ -249,6 +249,22 @@ def test_weight_gradient_of_long_groups(sizes):
         O.check(first[i], want, acc + O.half_step(want.abs() + acc, torch.bfloat16))
 
 
+@pytest.mark.parametrize("k, n", [(2048, 1024), (2304, 2200), (8192, 96), (520, 2048)])
+@pytest.mark.parametrize("sizes", [[1500, 5, 0, 300, 64, 1], [3, 2, 900, 1, 0, 0, 40, 2, 800, 7], [256] * 6], ids=str)
+def test_weight_gradient_of_unequal_groups(sizes, k, n):
+    # more tiles than CTAs and one group far above the mean: tiles are dealt out, every one once
+    t, off = sum(sizes), bounds(sizes)
+    x, g = randn(t, k), randn(t, n, seed=1)
+    w = torch.zeros(len(sizes), n, k, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    (dw,) = torch.autograd.grad(grouped_matmul(x, w, off), w, g)
+    for i, (lo, hi) in enumerate(spans(off)):
+        a, b = g[lo:hi].double().t(), x[lo:hi].double()
+        terms, want = a.abs() @ b.abs(), a @ b
+        acc = (hi - lo + 1) * 2.0 ** -23 * terms
+        half = torch.maximum((want.abs() + acc) * 2.0 ** -8, torch.full_like(want, 1e-38))
+        assert bool(((dw[i].double() - want).abs() <= acc + half).all())
+
+
 def test_first_call_in_a_new_thread():
     # a thread without a CUDA context of its own, as autograd's
     from concurrent.futures import ThreadPoolExecutor
