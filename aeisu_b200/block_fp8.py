@@ -22,7 +22,9 @@ the batch), both operands in FP8; the bias gradient is summed in float32.  Only 
 codes of input and weight are kept for the backward pass.  Gradients of gradients are not computed.
 
 All tensors must be CUDA tensors on one device; work goes to that device's current stream and may be
-captured into a CUDA graph.  float64 is refused rather than computed at a lower precision.
+captured into a CUDA graph.  A backward pass is captured only while no eager graph of the same leaves
+lives: torch would make the capture wait for that graph's stream, and the capture fails.  float64 is
+refused rather than computed at a lower precision.
 """
 from __future__ import annotations
 

@@ -3,7 +3,8 @@
 The grouped layers of the controller give each channel group its own weights; here each *row* (a pixel
 of a tile, a token) belongs to one of E experts.  ``offsets`` [E + 1] bounds the groups: rows
 ``offsets[e] : offsets[e + 1]`` of x are multiplied by ``weight[e]``.  The bounds stay on the GPU: the
-call never waits for them, so it may be captured into a CUDA graph and replayed with other bounds.
+call never waits for them, so it may be captured into a CUDA graph and replayed with other bounds
+(a backward pass only while no eager graph of the same leaves lives, as for ``block_fp8``).
 
     y = grouped_matmul(x, weight, offsets)             # x [T, K], weight [E, N, K]: y [T, N]
 
