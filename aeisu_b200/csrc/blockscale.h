@@ -13,6 +13,7 @@ enum ElemType : int { kF32 = 0, kF16 = 1, kBF16 = 2, kE4M3 = 3, kE5M2 = 4 };
 inline int elem_bytes(int t) { return t == kF32 ? 4 : t <= kBF16 ? 2 : 1; }
 
 constexpr int kBlock = 128;        // values per scale along a row
+constexpr int kMaxSide = 0x7fffffff - 1024;   // rows or columns of a matrix
 constexpr int kMaxGroups = 1024;   // groups of one grouped product (offsets live in shared memory)
 
 // A batch of matrices [batch][rows][cols], cols contiguous unless `trans` (then rows are:

@@ -1,5 +1,6 @@
 // extern "C" boundary (include/aeisu.h).  Every entry point converts internal failures
 // into status codes and records the message for aeisu_last_error().
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <fstream>
@@ -61,8 +62,11 @@ void check_io(int n, int h, int w, unsigned flags) {
     aeisu::require(flags == AEISU_IO_HOST || flags == AEISU_IO_DEVICE, "unknown I/O flags");
 }
 
+// (Kernels count a tile beyond the last row or column in 32 bits.)
 aeisu::MatrixRef matrix(const aeisu_matrix* m) {
     aeisu::require(m != nullptr, "matrix pointer is null");
+    aeisu::require(m->rows <= aeisu::kMaxSide && m->cols <= aeisu::kMaxSide, "matrix sizes are out of range");
+    aeisu::require(reinterpret_cast<uintptr_t>(m->data) % aeisu::elem_bytes(m->type) == 0, "tensor pointer is misaligned");
     return {m->data, m->type, m->rows, m->cols, (long long)m->ld, m->batch, (long long)m->batch_stride, m->transposed != 0};
 }
 aeisu::ScaleRef scales_of(const aeisu_matrix* m) {
@@ -80,9 +84,19 @@ struct Scales {   // the scales of an FP8 operand, none for a 16-bit one
         }
     }
 };
-aeisu::ProductOut product_out(const aeisu_matrix* out, const void* bias, int bias_type) {
+aeisu::MatrixRef single(const aeisu_matrix* m) {
+    const aeisu::MatrixRef r = matrix(m);
+    aeisu::require(r.batch == 1, "a linear layer takes single matrices");
+    return r;
+}
+// The output of x[rows][k] and weight[cols][k].
+aeisu::ProductOut product_out(const aeisu_matrix* out, const void* bias, int bias_type, int rows, int cols) {
     aeisu::require(out != nullptr, "output pointer is null");
+    matrix(out);
+    aeisu::require(out->rows == rows && out->cols == cols && out->batch == 1 && !out->transposed,
+                   "output sizes are out of range");
     aeisu::require(!bias || (bias_type >= 0 && bias_type <= 2), "bias must be float32, float16 or bfloat16");
+    aeisu::require(reinterpret_cast<uintptr_t>(bias) % aeisu::elem_bytes(bias_type) == 0, "bias pointer is misaligned");
     return {const_cast<void*>(out->data), out->type, (long long)out->ld, bias, bias_type};
 }
 
@@ -302,7 +316,9 @@ int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, const aeisu_matr
     return guarded([&] {
         aeisu::require(codes != nullptr, "codes pointer is null");
         const aeisu::MatrixRef m = matrix(x);
-        aeisu::require(codes->rows == m.rows && codes->cols == m.cols && codes->batch == m.batch,
+        aeisu::require(block_rows == 1 || block_rows == 128, "blocks have 1 or 128 rows");
+        aeisu::require(codes->rows == m.rows && codes->cols == m.cols && codes->batch == m.batch &&
+                           codes->block_rows == block_rows && (!t_codes || t_codes->block_rows == block_rows),
                        "codes must have the sizes of the values");
         aeisu::require(!t_codes || (t_codes->rows == m.cols && t_codes->cols == m.rows && t_codes->batch == m.batch &&
                                     t_codes->type == codes->type),
@@ -317,7 +333,7 @@ int aeisu_block_quantize(const aeisu_matrix* x, int block_rows, const aeisu_matr
 }
 
 uint64_t aeisu_column_sum_workspace(int rows, int cols) {
-    return rows >= 1 && cols >= 1 ? aeisu::column_sum_partials(rows, cols) * sizeof(float) : 0;
+    return rows >= 1 && cols >= 1 && std::max(rows, cols) <= aeisu::kMaxSide ? aeisu::column_sum_partials(rows, cols) * sizeof(float) : 0;
 }
 
 int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* workspace, uint64_t workspace_bytes,
@@ -332,7 +348,7 @@ int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* works
 uint64_t aeisu_product_workspace(int m, int n, int k, int device) {
     uint64_t r = 0;
     guarded([&] {
-        aeisu::require(m >= 1 && n >= 1 && k >= 1, "matrix sizes are out of range");
+        aeisu::require(std::min({m, n, k}) >= 1 && std::max({m, n, k}) <= aeisu::kMaxSide, "matrix sizes are out of range");
         r = aeisu::product_workspace(m, n, k, device);
     });
     return r;
@@ -343,32 +359,33 @@ int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias
     return guarded([&] {
         const aeisu::MatrixRef ma = matrix(a), mb = matrix(b);
         aeisu::require(a->scales && b->scales, "FP8 operands, and only they, come with scales");
-        aeisu::product(ma, scales_of(a), mb, scales_of(b), product_out(out, bias, bias_type), workspace, size_t(workspace_bytes),
-                       false, device, static_cast<cudaStream_t>(stream));
+        aeisu::product(ma, scales_of(a), mb, scales_of(b), product_out(out, bias, bias_type, ma.rows, mb.rows),
+                       workspace, size_t(workspace_bytes), false, device, static_cast<cudaStream_t>(stream));
     });
 }
 
 uint64_t aeisu_linear_workspace(int m, int n, int k, int pass, int device) {
     uint64_t r = 0;
     guarded([&] {
-        aeisu::require(m >= 1 && n >= 1 && k >= 1 && pass >= 0 && pass <= 2, "matrix sizes are out of range");
+        aeisu::require(std::min({m, n, k}) >= 1 && std::max({m, n, k}) <= aeisu::kMaxSide && pass >= 0 && pass <= 2,
+                       "matrix sizes are out of range");
         r = aeisu::linear_workspace(m, n, k, pass, device);
     });
     return r;
 }
 
 uint64_t aeisu_linear_kept_bytes(int rows, int cols, int block_rows) {
-    if (rows < 1 || cols < 1 || (block_rows != 1 && block_rows != 128)) return 0;
+    if (rows < 1 || cols < 1 || std::max(rows, cols) > aeisu::kMaxSide || (block_rows != 1 && block_rows != 128)) return 0;
     return aeisu::transposed_codes_bytes(rows, cols, block_rows);
 }
 
 int aeisu_linear(const aeisu_matrix* x, const aeisu_matrix* weight, const void* bias, int bias_type,
                  const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
-        const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
+        const aeisu::MatrixRef mx = single(x), mw = single(weight);
         aeisu::require(mx.cols == mw.cols && mx.rows >= 1, "contraction sizes differ");
         aeisu::require(weight->scales != nullptr, "FP8 operands, and only they, come with scales");
-        aeisu::linear_serve(mx, mw, scales_of(weight), product_out(out, bias, bias_type), workspace,
+        aeisu::linear_serve(mx, mw, scales_of(weight), product_out(out, bias, bias_type, mx.rows, mw.rows), workspace,
                             size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
     });
 }
@@ -377,10 +394,10 @@ int aeisu_linear_forward(const aeisu_matrix* x, const aeisu_matrix* weight, cons
                          const aeisu_matrix* out, void* kept_x, void* kept_weight, void* workspace,
                          uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
-        const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
+        const aeisu::MatrixRef mx = single(x), mw = single(weight);
         aeisu::require(mx.cols == mw.cols && mx.rows >= 1 && mw.rows >= 1, "contraction sizes differ");
-        aeisu::linear_train_forward(mx, mw, product_out(out, bias, bias_type), kept_x, kept_weight, workspace,
-                                    size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
+        aeisu::linear_train_forward(mx, mw, product_out(out, bias, bias_type, mx.rows, mw.rows), kept_x, kept_weight,
+                                    workspace, size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -388,8 +405,8 @@ int aeisu_linear_backward(const aeisu_matrix* grad, int k, int code_type, const 
                           void* grad_x, int grad_x_type, void* grad_weight, int grad_weight_type, void* grad_bias,
                           int grad_bias_type, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
-        const aeisu::MatrixRef g = matrix(grad);
-        aeisu::require(g.rows >= 1 && g.cols >= 1, "matrix sizes are out of range");
+        const aeisu::MatrixRef g = single(grad);
+        aeisu::require(g.rows >= 1 && g.cols >= 1 && k <= aeisu::kMaxSide, "matrix sizes are out of range");
         aeisu::linear_train_backward(g, k, code_type, kept_x, kept_weight, grad_x, grad_x_type, grad_weight,
                                      grad_weight_type, grad_bias, grad_bias_type, workspace, size_t(workspace_bytes),
                                      device, static_cast<cudaStream_t>(stream));
@@ -397,17 +414,17 @@ int aeisu_linear_backward(const aeisu_matrix* grad, int k, int code_type, const 
 }
 
 uint64_t aeisu_grouped_linear_workspace(int rows, int k) {
-    return rows >= 1 && k >= 1 ? aeisu::grouped_linear_workspace(rows, k) : 0;
+    return rows >= 1 && k >= 1 && std::max(rows, k) <= aeisu::kMaxSide ? aeisu::grouped_linear_workspace(rows, k) : 0;
 }
 
 int aeisu_grouped_linear(const aeisu_matrix* x, const aeisu_matrix* weight, const int* offsets, int zero_outside,
                          const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
-        const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
+        const aeisu::MatrixRef mx = single(x), mw = matrix(weight);
         aeisu::require(mx.cols == mw.cols && mx.rows >= 1, "contraction sizes differ");
         aeisu::require(weight->scales != nullptr, "FP8 operands, and only they, come with scales");
-        aeisu::grouped_linear(mx, mw, scales_of(weight), offsets, product_out(out, nullptr, 0), zero_outside != 0,
-                              workspace, size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
+        aeisu::grouped_linear(mx, mw, scales_of(weight), offsets, product_out(out, nullptr, 0, mx.rows, mw.rows),
+                              zero_outside != 0, workspace, size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -416,8 +433,8 @@ int aeisu_grouped_product(const aeisu_matrix* x, const aeisu_matrix* weight, con
     return guarded([&] {
         const aeisu::MatrixRef mx = matrix(x), mw = matrix(weight);
         const Scales sx(x), sw(weight);
-        aeisu::grouped_product(mx, sx.ptr, mw, sw.ptr, offsets, product_out(out, nullptr, 0), zero_outside != 0, false, device,
-                               static_cast<cudaStream_t>(stream));
+        aeisu::grouped_product(mx, sx.ptr, mw, sw.ptr, offsets, product_out(out, nullptr, 0, mx.rows, mw.rows),
+                               zero_outside != 0, false, device, static_cast<cudaStream_t>(stream));
     });
 }
 

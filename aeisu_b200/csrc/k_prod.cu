@@ -1439,7 +1439,7 @@ void grouped(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const S
              cudaStream_t stream) {
     require(x.batch == 1 && !x.trans && x.cols == b.cols, "contraction sizes differ");
     require((sx != nullptr) == (sb != nullptr) && (sx || x.type == b.type), "operand types do not go together");
-    require(off && b.batch <= kMaxGroups, "a grouped product has offsets and at most 1024 groups");
+    require(off && aligned(off, 4) && b.batch <= kMaxGroups, "a grouped product has offsets and at most 1024 groups");
     require(out.ptr && out.type >= kF32 && out.type <= kBF16 && out.ld >= b.rows && !out.bias, "output is out of range");
     OnDevice on(device);
     const bool fp8 = sx != nullptr;
@@ -1538,8 +1538,8 @@ void grouped_weight_gradient(const MatrixRef& g, const MatrixRef& x, const int* 
     check_operand(x, nullptr);
     require(g.batch == 1 && x.batch == 1 && g.trans && x.trans && g.cols == x.cols && g.type == x.type,
             "contraction sizes differ");
-    require(off && groups >= 1 && groups <= kMaxGroups, "a grouped product has offsets and at most 1024 groups");
-    require(out && out_type >= kF32 && out_type <= kBF16, "output is out of range");
+    require(off && aligned(off, 4) && groups >= 1 && groups <= kMaxGroups, "a grouped product has offsets and at most 1024 groups");
+    require(out && out_type >= kF32 && out_type <= kBF16 && aligned(out, elem_bytes(out_type)), "output is out of range");
     OnDevice on(device);
     ProdJob j{};
     const TileShape tile = choose_tile(ceil_div(g.rows, kBM), x.rows, groups, ceil_div(ceil_div(g.cols, groups), kStepBytes / 2),

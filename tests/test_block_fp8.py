@@ -198,3 +198,33 @@ def test_matrix_layout_matches_the_header(lib):
     m = Matrix.from_buffer_copy(packed(data=1, scales=2, type=3, rows=4, cols=5, batch=6, ld=7, batch_stride=8, block_rows=9,
                                        transposed=10))
     assert [getattr(m, f) for f, _ in Matrix._fields_] == list(range(1, 11))
+
+
+def test_c_entries_refuse_what_leads_out_of_the_tensors(lib):
+    most = 2 ** 31 - 1
+    codes, half, out = packed(), packed(**HALF), packed(cols=8, ld=8, **HALF)
+    deep = packed(rows=most, ld=64, **HALF)
+    for call, text in (
+            (lambda: lib.aeisu_product(packed(rows=most), codes, None, 0, packed(rows=most, cols=8, ld=8, **HALF), None, 0, 0, None),
+             "sizes"),
+            (lambda: lib.aeisu_product(codes, codes, None, 0, packed(rows=7, cols=8, ld=8, **HALF), None, 0, 0, None), "output"),
+            (lambda: lib.aeisu_product(codes, codes, None, 0, packed(cols=7, ld=8, **HALF), None, 0, 0, None), "output"),
+            (lambda: lib.aeisu_product(codes, codes, None, 0, packed(data=4097, cols=8, ld=8, **HALF), None, 0, 0, None),
+             "misaligned"),
+            (lambda: lib.aeisu_product(codes, codes, 4098, 0, out, None, 0, 0, None), "misaligned"),
+            (lambda: lib.aeisu_block_quantize(deep, 1, packed(rows=most), None, 0, None), "sizes"),
+            (lambda: lib.aeisu_block_quantize(packed(data=4097, **HALF), 1, codes, None, 0, None), "misaligned"),
+            (lambda: lib.aeisu_block_quantize(half, 1, packed(block_rows=128), None, 0, None), "sizes"),
+            (lambda: lib.aeisu_column_sum(deep, 4096, 2, 4096, 1 << 40, 0, None), "sizes"),
+            (lambda: lib.aeisu_linear(packed(batch=2, batch_stride=512, **HALF), codes, None, 0, out, 4096, 1 << 20, 0, None), "single"),
+            (lambda: lib.aeisu_linear(half, codes, None, 0, packed(rows=9, cols=8, ld=8, **HALF), 4096, 1 << 20, 0, None), "output"),
+            (lambda: lib.aeisu_linear_forward(half, packed(batch=2, batch_stride=512, **HALF), None, 0, out, None, None, 4096,
+                                              1 << 20, 0, None), "single"),
+            (lambda: lib.aeisu_linear_backward(packed(batch=2, batch_stride=512, **HALF), 8, 3, None, None, None, 2, None, 2, None,
+                                               2, 4096, 1 << 20, 0, None), "single"),
+            (lambda: lib.aeisu_grouped_linear(packed(batch=2, batch_stride=512, **HALF), codes, 4096, 1, out, 4096, 1 << 20, 0,
+                                              None), "single"),
+            (lambda: lib.aeisu_grouped_product(half, half, 4096, 1, packed(rows=4, cols=8, ld=8, **HALF), 0, None), "output")):
+        assert call() == _lib.INVALID_ARG and text in _lib.last_error(), _lib.last_error()
+    assert lib.aeisu_linear_kept_bytes(most, 4, 1) == 0 and lib.aeisu_column_sum_workspace(most, 4) == 0
+    assert lib.aeisu_grouped_linear_workspace(4, most) == 0 and lib.aeisu_product_workspace(most, 4, 4, 0) == 0
