@@ -1120,18 +1120,38 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
     if (warp == 3) columns_free<CTAS>(tmem, S::kCols);
 }
 
-// out = sum of the parts in order, plus the bias of the column.
+// out = sum of the parts in order, plus the bias of the column.  G threads share an output: each adds a run of
+// parts, then the runs are added in order.  One where outputs are many; eight where parts are (144 parts of
+// 64 x 128: 7.2 us with one, whose loads follow one another, 3.7 with eight).
+template <int G>
 __global__ void __launch_bounds__(256) k_join_parts(const float* part, int parts, long long stride, int rows, int cols,
                                                     void* out, int out_type, long long out_ld, const void* bias,
                                                     int bias_type) {
+    constexpr int kOutputs = 256 / G;
+    __shared__ float sh[G][kOutputs];
     const long long n = (long long)rows * cols;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const int o = int(threadIdx.x) % kOutputs, run = int(threadIdx.x) / kOutputs, per = (parts + G - 1) / G;
+    const int first = run * per, last = min(parts, first + per);
+    for (long long i0 = (long long)blockIdx.x * kOutputs; i0 < n; i0 += (long long)gridDim.x * kOutputs) {
+        const long long i = i0 + o;
         float s = 0.f;
+        if (i < n) {
 #pragma unroll 16
-        for (int k = 0; k < parts; ++k) s += part[k * stride + i];
-        const int r = int(i / cols), c = int(i % cols);
-        if (bias) s += load_elem(bias, bias_type, c);
-        store_elem(out, out_type, r * out_ld + c, s);
+            for (int k = first; k < last; ++k) s += part[k * stride + i];
+        }
+        if constexpr (G > 1) {
+            sh[run][o] = s;
+            __syncthreads();
+            s = sh[0][o];
+#pragma unroll
+            for (int r = 1; r < G; ++r) s += sh[r][o];
+            __syncthreads();
+        }
+        if (i < n && run == 0) {
+            const int r = int(i / cols), c = int(i % cols);
+            if (bias) s += load_elem(bias, bias_type, c);
+            store_elem(out, out_type, r * out_ld + c, s);
+        }
     }
 }
 
@@ -1427,7 +1447,10 @@ void dense(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const Sca
     launch_shape<true>(pl.tile, ma, mb, j, tiles, device, stream);
     if (pl.split > pl.cluster) {
         const long long n = (long long)a.rows * b.rows;
-        k_join_parts<<<unsigned(std::min<long long>((n + 255) / 256, 148 * 8)), 256, 0, stream>>>(
+        const bool many = pl.split >= 32;
+        const auto join = many ? k_join_parts<8> : k_join_parts<1>;
+        const int per = many ? 32 : 256;
+        join<<<unsigned(std::min<long long>((n + per - 1) / per, 148 * 8)), 256, 0, stream>>>(
             static_cast<const float*>(workspace), pl.split, j.split_stride, a.rows, b.rows, out.ptr, out.type, out.ld,
             out.bias, out.bias_type);
         AEISU_CUDA(cudaGetLastError());

@@ -28,6 +28,10 @@ Operand operand_at(const void* buffer, int type, int rows, int cols, int block_r
     return {{p, type, rows, cols, code_ld(cols), 1, 0, false},
             {p + padded(size_t(rows) * code_ld(cols)), block_rows == 1 ? 0 : 7, per, 0}};
 }
+// Partial sums of the bias gradient.
+size_t sums_bytes(int m, int n) {
+    return padded(std::max(column_sum_partials(m, n), size_t((m + kBlock - 1) / kBlock) * n) * sizeof(float));
+}
 void* codes_of(const Operand& o) { return const_cast<void*>(o.m.ptr); }
 uint8_t* scales_of(const Operand& o) { return const_cast<uint8_t*>(o.s.ptr); }
 
@@ -50,9 +54,8 @@ size_t linear_workspace(int m, int n, int k, int pass, int device) {
     if (pass == kServe) return operand_bytes(m, k, 1) + product_workspace(m, n, k, device);
     if (pass == kTrainForward)
         return operand_bytes(m, k, 1) + operand_bytes(n, k, kBlock) + product_workspace(m, n, k, device);
-    return operand_bytes(m, n, 1) + operand_bytes(n, m, 1) +
-           std::max({product_workspace(m, k, n, device), product_workspace(n, k, m, device),
-                     std::max(column_sum_partials(m, n), size_t((m + kBlock - 1) / kBlock) * n) * sizeof(float)});
+    return operand_bytes(m, n, 1) + operand_bytes(n, m, 1) + sums_bytes(m, n) +
+           std::max(product_workspace(m, k, n, device), product_workspace(n, k, m, device));
 }
 
 void linear_serve(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, const ProductOut& out, void* workspace,
@@ -94,23 +97,24 @@ void linear_train_backward(const MatrixRef& grad, int k, int code_type, const vo
     ws += operand_bytes(m, n, 1);
     const Operand gt = operand_at(ws, code_type, n, m, 1);
     ws += operand_bytes(n, m, 1);
-    const size_t left = workspace_bytes - size_t(ws - static_cast<uint8_t*>(workspace));
-    // The bias gradient comes out of the pass that quantises both ways, or has one of its own.
+    // The bias gradient comes out of the pass that quantises both ways, and is joined when the products, which
+    // start under that pass, are on their way; or it has a pass of its own.
     float* sums = reinterpret_cast<float*>(ws);
+    ws += sums_bytes(m, n);
+    const size_t left = workspace_bytes - size_t(ws - static_cast<uint8_t*>(workspace));
     if (gb && !gw) column_sum(grad, gb, gb_type, sums, device, stream);
     if (gx || gw) quantize_into(grad, 1, g, gw ? &gt : nullptr, gb && gw ? sums : nullptr, device, stream);
-    if (gb && gw) {
-        OnDevice on(device);
-        join_sums(sums, (m + kBlock - 1) / kBlock, n, gb, gb_type, stream);
-    }
-    const bool after = !(gb && gw);   // the kernel before the next product is the quantiser
     if (gx) {
         const Operand wt = operand_at(kept_w, kE4M3, k, n, kBlock);
-        product(g.m, g.s, wt.m, wt.s, {gx, gx_type, k, nullptr, 0}, ws, left, after, device, stream);
+        product(g.m, g.s, wt.m, wt.s, {gx, gx_type, k, nullptr, 0}, ws, left, true, device, stream);
     }
     if (gw) {
         const Operand xt = operand_at(kept_x, kE4M3, k, m, 1);
-        product(gt.m, gt.s, xt.m, xt.s, {gw, gw_type, k, nullptr, 0}, ws, left, after && !gx, device, stream);
+        product(gt.m, gt.s, xt.m, xt.s, {gw, gw_type, k, nullptr, 0}, ws, left, !gx, device, stream);
+    }
+    if (gb && gw) {
+        OnDevice on(device);
+        join_sums(sums, (m + kBlock - 1) / kBlock, n, gb, gb_type, stream);
     }
 }
 
