@@ -41,6 +41,9 @@ constexpr int kWriters = 8;           // warps that write tiles out
 constexpr int kThreads = 128 + 32 * kWriters;
 constexpr int kRing = 201 * 1024 + 512;   // shared memory of the operand ring
 constexpr int kTurn = 2048;           // shared memory of a writer: 32 rows of 64 bytes
+// FP8 contractions up to here fill half of a step's rows: boxes of 64 bytes, two MMAs (170,496 x 64 -> 128: 18.5 us;
+// in rows of 128 bytes, half of them out of range, 23.1).
+constexpr int kNarrow = kStepBytes / 2;
 constexpr int kErrWait = 1;           // error code: a wait ran out
 constexpr int kAtom = 512;            // scales of 128 rows and four block columns
 constexpr int kScaleSlots = 4;        // atoms that are staged at a time (even: two warps fill them)
@@ -66,6 +69,7 @@ struct ProdJob {
     int P, Q, K;                 // rows of A, rows of B, contraction (whole sides; per batch entry)
     int grouping, groups;
     const int* off;
+    int narrow;                  // FP8, contraction of at most 64: a step stages 64 bytes of each row
     int a_mn, b_mn;              // operand stored with its rows contiguous (contraction strided)
     uint32_t idesc;              // instruction descriptor without the columns
     ScaleRef sa, sb;
@@ -124,6 +128,11 @@ struct Shape {
 __device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {
     return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) |
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// The same with rows of 64 swizzled bytes: eight rows per 512-byte atom.
+__device__ __forceinline__ uint64_t desc_narrow(uint32_t saddr) {
+    return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(512 >> 4) << 32) |
+           (uint64_t(1) << 46) | (uint64_t(4) << 61);
 }
 // Row-contiguous operand tile: chunks of 64 rows of the operand (128 swizzled bytes) by 64
 // contraction values, 8192 bytes from chunk to chunk, 1024 from eight contraction values to the next.
@@ -798,13 +807,14 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         uint32_t phase = 0;
         bool ok = true;
         long long issued = 0;
+        const int staged = FP8 && !OWN && j.narrow ? S::kStage / 2 : S::kStage;   // bytes per step
         // Weights are on their way before the quantiser has ended: A's copies of the first stages.
         int early = 0;
         if (CTAS == 1 && j.early_a && first_tile < tiles) {
             const Tile x = tile_at<BM, BN>(j, g, first_tile, kStep);
             if (elected())
                 for (int k = x.k0; k < x.k1 && early < S::kStages; k += kStep, ++early) {
-                    mbar_arrive_expect_tx(full + early, S::kStage);
+                    mbar_arrive_expect_tx(full + early, staged);
                     tma_3d<1>(smem_addr(ring) + early * S::kStage, &ma, k, x.p0, j.grouping == kRowsB ? x.e : 0,
                               smem_addr(full + early));
                 }
@@ -830,7 +840,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                         mbar_arrive_expect_tx(landed + stage, S::kStage);
                         if (CTAS == 1 || rank == 0) mbar_arrive(full + stage);
                     } else if (!begun && (CTAS == 1 || rank == 0)) {
-                        mbar_arrive_expect_tx(full + stage, OWN ? S::kATile : S::kStage * CTAS);
+                        mbar_arrive_expect_tx(full + stage, OWN ? S::kATile : staged * CTAS);
                     }
                     if (begun) {
                     } else if (j.a_mn) {
@@ -864,8 +874,9 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             bool ok = true;
             const uint32_t a_k = (j.a_mn ? 2048 : 32) >> 4, b_k = (j.b_mn ? 2048 : 32) >> 4;
             const uint32_t first_a = smem_addr(ring), first_b = first_a + S::kATile;
-            const uint64_t desc_a = j.a_mn ? desc_mnmajor(first_a) : desc_kmajor(first_a);
-            const uint64_t desc_b = j.b_mn ? desc_mnmajor(first_b) : desc_kmajor(first_b);
+            const bool narrow = FP8 && !OWN && j.narrow;
+            const uint64_t desc_a = narrow ? desc_narrow(first_a) : j.a_mn ? desc_mnmajor(first_a) : desc_kmajor(first_a);
+            const uint64_t desc_b = narrow ? desc_narrow(first_b) : j.b_mn ? desc_mnmajor(first_b) : desc_kmajor(first_b);
             for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BM, BN>(j, g, t, kStep);
                 if (x.p0 < 0) continue;
@@ -897,7 +908,8 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                             const uint32_t id = idesc | (byte << 4) | (byte << 29);
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                mma_block_scaled<CTAS>(d, da + i * 2, db + i * 2, id, sf, sf + 4, i ? 1 : more);
+                                if (i < 2 || !narrow)
+                                    mma_block_scaled<CTAS>(d, da + i * 2, db + i * 2, id, sf, sf + 4, i ? 1 : more);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) mma_half<CTAS>(d, da + i * a_k, db + i * b_k, idesc, i ? 1 : more);
@@ -1170,21 +1182,22 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return fn;
 }
 
-// Operand map: innermost the contiguous direction in boxes of 128 bytes, `high` of the other.
-CUtensorMap operand_map(const MatrixRef& m, int high) {
+// Operand map: innermost the contiguous direction in boxes of 128 bytes (narrow: 64), `high` of the other.
+CUtensorMap operand_map(const MatrixRef& m, int high, bool narrow = false) {
     const int eb = elem_bytes(m.type);
     const int inner = m.trans ? m.rows : m.cols, outer = m.trans ? m.cols : m.rows;
     CUtensorMap map{};
     const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(m.batch)};
     const long long batch = m.batch > 1 ? m.batch_stride : ((m.ld * outer * eb + 15) / 16 * 16) / eb;
     const cuuint64_t strides[2] = {cuuint64_t(m.ld) * eb, cuuint64_t(batch) * eb};
-    const cuuint32_t box[3] = {cuuint32_t(kStepBytes / eb), cuuint32_t(high), 1};
+    const cuuint32_t box[3] = {cuuint32_t((narrow ? kStepBytes / 2 : kStepBytes) / eb), cuuint32_t(high), 1};
     const cuuint32_t one[3] = {1, 1, 1};
     const CUtensorMapDataType type = m.type == kF16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                      : m.type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                        : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const CUresult r = encoder()(&map, type, 3, const_cast<void*>(m.ptr), dims, strides, box, one,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) fail(AEISU_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
     return map;
@@ -1443,7 +1456,8 @@ void dense(const MatrixRef& a, const ScaleRef& sa, const MatrixRef& b, const Sca
     j.out_vec = whole_rows(j.out, j.out_type, j.out_ld, j.split_stride);
     const long long tiles = ceil_div(j.P, pl.tile.rows()) * ceil_div(j.Q, pl.tile.bn) * pl.split;
     require(tiles < (1LL << 30), "matrix is too large");
-    const CUtensorMap ma = operand_map(A, kBM), mb = values ? ma : operand_map(B, pl.tile.b_rows());
+    j.narrow = !values && j.K <= kNarrow;
+    const CUtensorMap ma = operand_map(A, kBM, j.narrow), mb = values ? ma : operand_map(B, pl.tile.b_rows(), j.narrow);
     launch_shape<true>(pl.tile, ma, mb, j, tiles, device, stream);
     if (pl.split > pl.cluster) {
         const long long n = (long long)a.rows * b.rows;
@@ -1515,7 +1529,9 @@ void grouped(const MatrixRef& x, const ScaleRef* sx, const MatrixRef& b, const S
     const int high = swap ? tile.bn : tile.rows(), wide = swap ? tile.rows() : tile.bn;
     const long long tiles = (ceil_div(x.rows, high) + std::min(b.batch, x.rows)) * ceil_div(b.rows, wide);
     require(tiles < (1LL << 30), "matrix is too large");
-    const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM), mb = values ? ma : operand_map(B, B.trans ? 64 : tile.b_rows());
+    j.narrow = fp8 && !values && j.K <= kNarrow;
+    const CUtensorMap ma = operand_map(A, A.trans ? 64 : kBM, j.narrow);
+    const CUtensorMap mb = values ? ma : operand_map(B, B.trans ? 64 : tile.b_rows(), j.narrow);
     if (fp8) launch_shape<true>(tile, ma, mb, j, tiles, device, stream);
     else launch_shape<false>(tile, ma, mb, j, tiles, device, stream);
 }
