@@ -108,6 +108,24 @@ __device__ __forceinline__ float finite_max(Vals<T>& v) {
     return m;
 }
 
+// The same of the first eight values and of the last eight.
+template <typename T>
+__device__ __forceinline__ void finite_max2(Vals<T>& v, float& first, float& second) {
+    constexpr int n = sizeof(v.w) / 8;
+    auto largest = [&](int from) {
+        auto m = v.w[from];
+#pragma unroll
+        for (int i = 1; i < n; ++i) m = larger<T>(m, v.w[from + i]);
+        if constexpr (sizeof(T) == 4) return fmaxf(fabsf(m), 0.f);
+        else return fmaxf(first_of<T>(m), second_of<T>(m));
+    };
+    first = largest(0), second = largest(n);
+    if (isinf(first) || isinf(second)) {
+        infinities_to_nan(v);
+        first = largest(0), second = largest(n);
+    }
+}
+
 // Biased exponent of the scale.  amax = m 2^e with 0.5 <= m < 1 has the exponent field e + 126; the
 // largest code is 0.875 * 2^top, so s = 2^(e - top), doubled where m > 0.875.
 template <bool E5M2>

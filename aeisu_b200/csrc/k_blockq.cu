@@ -96,14 +96,17 @@ __global__ void __launch_bounds__(kThreads) k_quant_rows(QuantJob<T> j) {
 // pairs of 16-bit values at a time.  The transposed codes (four rows to a word) turn in shared memory; the
 // 16-byte chunk of a column is exclusive-or'ed with the column's octet, so that a warp's 32 words
 // fall in 32 banks.
-template <typename T, bool E5M2, bool VEC, bool TILE_SCALE, bool BOTH>
+// NARROW (at most 64 columns, one scale per row, both ways): the second run of eight columns is instead the same
+// columns 128 rows on, so that no lane idles: a CTA takes 256 rows, two blocks of the transpose.
+template <typename T, bool E5M2, bool VEC, bool TILE_SCALE, bool BOTH, bool NARROW = false>
 __global__ void __launch_bounds__(kThreads, !BOTH ? (sizeof(T) == 2 ? 4 : 3) : sizeof(T) == 4 && !TILE_SCALE ? 2 : 3)
 k_quant_tile(QuantJob<T> j) {
+    static_assert(!NARROW || (BOTH && !TILE_SCALE), "narrow matrices have a form of their own one way and by tiles");
     using P = typename Pair<T>::type;
     constexpr int kPairs = sizeof(Vals<T>) / 4, kPer = 16 / kPairs;   // pairs of a lane's row, values in one
     __shared__ P col_max[8][kBlock / kPer];
     __shared__ __align__(16) float col_inv[kBlock];
-    __shared__ uint8_t row_s[kBlock];
+    __shared__ uint8_t row_s[NARROW ? 2 * kBlock : kBlock];
     __shared__ float col_sum[TILE_SCALE || !BOTH ? 1 : 8][kBlock];
     __shared__ float tile_max[8];
     __shared__ __align__(16) uint32_t turn[BOTH ? kBlock * 32 : 4];
@@ -111,17 +114,16 @@ k_quant_tile(QuantJob<T> j) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, oct = lane & 7, sub = lane >> 3;
     const int col_blocks = (j.cols + kBlock - 1) / kBlock, row_blocks = (j.rows + kBlock - 1) / kBlock;
     const int rb = int(blockIdx.x / col_blocks), cb = int(blockIdx.x % col_blocks);
-    const int r0 = rb * kBlock, c0 = cb * kBlock, rw = warp * 16 + sub * 4;
+    const int r0 = rb * (NARROW ? 2 * kBlock : kBlock), c0 = cb * kBlock, rw = warp * 16 + sub * 4;
+    constexpr int kDown = NARROW ? kBlock : 0, kAside = NARROW ? 0 : 64;   // from a lane's first run to its second
     const T* x = j.x + blockIdx.y * j.batch_stride;
     Vals<T> v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = r0 + rw + i;
         v[i] = {};
-        if (r < j.rows) {
-            load8<T, VEC>(v[i], 0, x + r * j.ld, c0 + oct * 8, j.cols);
-            load8<T, VEC>(v[i], 1, x + r * j.ld, c0 + 64 + oct * 8, j.cols);
-        }
+        if (r < j.rows) load8<T, VEC>(v[i], 0, x + r * j.ld, c0 + oct * 8, j.cols);
+        if (r + kDown < j.rows) load8<T, VEC>(v[i], 1, x + (r + kDown) * j.ld, c0 + kAside + oct * 8, j.cols);
     }
     if constexpr (!TILE_SCALE && BOTH) {
         if (j.sums) {   // of the values as they are, infinities too
@@ -135,8 +137,12 @@ k_quant_tile(QuantJob<T> j) {
         }
     }
     float amax[4];
+    [[maybe_unused]] float amax2[4];   // NARROW: of the second run
 #pragma unroll
-    for (int i = 0; i < 4; ++i) amax[i] = finite_max(v[i]);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (NARROW) finite_max2(v[i], amax[i], amax2[i]);
+        else amax[i] = finite_max(v[i]);
+    }
     if constexpr (TILE_SCALE) {
         float m = fmaxf(fmaxf(amax[0], amax[1]), fmaxf(amax[2], amax[3]));
 #pragma unroll
@@ -148,6 +154,11 @@ k_quant_tile(QuantJob<T> j) {
 #pragma unroll
             for (int d = 1; d < 8; d <<= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(~0u, amax[i], d));
             if (oct == 0) row_s[rw + i] = uint8_t(scale_of<E5M2>(amax[i]));
+            if constexpr (NARROW) {
+#pragma unroll
+                for (int d = 1; d < 8; d <<= 1) amax2[i] = fmaxf(amax2[i], __shfl_xor_sync(~0u, amax2[i], d));
+                if (oct == 0) row_s[kBlock + rw + i] = uint8_t(scale_of<E5M2>(amax2[i]));
+            }
         }
         if constexpr (BOTH) {
 #pragma unroll
@@ -174,6 +185,8 @@ k_quant_tile(QuantJob<T> j) {
         if (threadIdx.x < kBlock) {
             if (r0 + int(threadIdx.x) < j.rows)
                 j.scales[(size_t(blockIdx.y) * col_blocks + cb) * j.rows + r0 + threadIdx.x] = row_s[threadIdx.x];
+            if (NARROW && r0 + kBlock + int(threadIdx.x) < j.rows)
+                j.scales[size_t(blockIdx.y) * j.rows + r0 + kBlock + threadIdx.x] = row_s[kBlock + threadIdx.x];
         } else if constexpr (BOTH) {
             const int c = threadIdx.x - kBlock;
             P m = col_max[0][c / kPer];
@@ -181,13 +194,14 @@ k_quant_tile(QuantJob<T> j) {
             for (int w = 1; w < 8; ++w) m = larger<T>(m, col_max[w][c / kPer]);
             const uint32_t s = scale_of<E5M2>(kPer == 2 && (c & 1) ? second_of<T>(m) : first_of<T>(larger<T>(m, m)));
             col_inv[c] = inverse_scale(s);
-            if (c0 + c < j.cols) {
-                j.t_scales[(size_t(blockIdx.y) * row_blocks + rb) * j.cols + c0 + c] = uint8_t(s);
+            const int block = NARROW ? 2 * rb + c / 64 : rb, column = NARROW ? c % 64 : c0 + c;
+            if (column < j.cols && block < row_blocks) {
+                j.t_scales[(size_t(blockIdx.y) * row_blocks + block) * j.cols + column] = uint8_t(s);
                 if (j.sums) {
                     float t = 0.f;
 #pragma unroll
                     for (int w = 0; w < 8; ++w) t += col_sum[w][c];
-                    j.sums[size_t(rb) * j.cols + c0 + c] = t;
+                    j.sums[size_t(block) * j.cols + column] = t;
                 }
             }
         }
@@ -195,11 +209,10 @@ k_quant_tile(QuantJob<T> j) {
     uint8_t* codes = j.codes + blockIdx.y * j.codes_batch;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int r = r0 + rw + i;
-        const float inv = inverse_scale(TILE_SCALE ? tile_s : scale_of<E5M2>(amax[i]));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int c = c0 + h * 64 + oct * 8;
+            const int r = r0 + rw + i + h * kDown, c = c0 + h * kAside + oct * 8;
+            const float inv = inverse_scale(TILE_SCALE ? tile_s : scale_of<E5M2>(NARROW && h ? amax2[i] : amax[i]));
             auto at = [&](int k) { return v[i].get(8 * h + k) * inv; };
             const uint2 q = make_uint2(codes4<E5M2>(at(0), at(1), at(2), at(3)), codes4<E5M2>(at(4), at(5), at(6), at(7)));
             if (r < j.rows && c < j.cols) *reinterpret_cast<uint2*>(codes + r * j.codes_ld + c) = q;
@@ -225,8 +238,9 @@ k_quant_tile(QuantJob<T> j) {
         for (int i = 0; i < 4; ++i) {
             const int at = i * kThreads + threadIdx.x, c = at >> 3, chunk = at & 7;
             const uint4 q = *reinterpret_cast<const uint4*>(turn + c * 32 + ((chunk ^ ((c >> 3) & 7)) << 2));
-            if (c0 + c < j.cols && r0 + chunk * 16 < j.rows)
-                *reinterpret_cast<uint4*>(t_codes + (c0 + c) * j.t_ld + r0 + chunk * 16) = q;
+            const int column = NARROW ? c % 64 : c0 + c, row = r0 + (NARROW ? c / 64 * kBlock : 0) + chunk * 16;
+            if (column < j.cols && row < j.rows)
+                *reinterpret_cast<uint4*>(t_codes + column * j.t_ld + row) = q;
         }
     }
 }
@@ -295,14 +309,20 @@ template <typename T, bool E5M2, bool VEC>
 void launch_quant(const QuantJob<T>& j, int block_rows, int batch, cudaStream_t stream) {
     const long long rows128 = (j.rows + 127) / 128, col_blocks = (j.cols + 127) / 128;
     const int cb = col_blocks >= 3 ? 4 : int(col_blocks);
+    // 256 rows to a CTA where 128 would make more CTAs than three on each of 148 SMs (bfloat16 x 64 both ways: 165,888
+    // rows 14.2 -> 10.2 us; 18,944 rows 3.6 us, 4.1 in this form).
+    const bool narrow = block_rows == 1 && j.t_codes && j.cols <= 64 && rows128 > 3 * 148;
     const long long grid = block_rows == 1 && !j.t_codes
-                               ? (j.rows * (long long)cb + 127) / 128 * ((col_blocks + cb - 1) / cb) : rows128 * col_blocks;
+                               ? (j.rows * (long long)cb + 127) / 128 * ((col_blocks + cb - 1) / cb)
+                           : narrow ? (rows128 + 1) / 2 : rows128 * col_blocks;
     require(grid < (1LL << 31), "matrix is too large");
     const dim3 g(unsigned(grid), unsigned(batch), 1);
     if (block_rows == 1 && !j.t_codes) {
         if (cb == 4) k_quant_rows<T, E5M2, VEC, 4><<<g, kThreads, 0, stream>>>(j);
         else if (cb == 2) k_quant_rows<T, E5M2, VEC, 2><<<g, kThreads, 0, stream>>>(j);
         else k_quant_rows<T, E5M2, VEC, 1><<<g, kThreads, 0, stream>>>(j);
+    } else if (narrow) {
+        k_quant_tile<T, E5M2, VEC, false, true, true><<<g, kThreads, 0, stream>>>(j);
     } else if (block_rows == 1) {
         k_quant_tile<T, E5M2, VEC, false, true><<<g, kThreads, 0, stream>>>(j);
     } else {

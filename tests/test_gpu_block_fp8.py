@@ -47,6 +47,35 @@ def test_quantize(m, k, dtype, rows):
         check_codes(t, x.t(), rows, codes)
 
 
+@pytest.mark.parametrize("m, k, dtype, codes", [
+    (57_000, 64, torch.bfloat16, E4), (57_100, 37, torch.float32, E4), (56_961, 8, torch.float16, E5)])
+def test_quantize_many_narrow_rows(m, k, dtype, codes):
+    # both row blocks of a CTA's 256 rows, with their special values in the first, the second and the last, half a block
+    x = randn(m, k + 3, dtype=dtype)[:, 2:k + 2] * torch.exp2(torch.randint(-6, 7, (m, 1))).cuda().to(dtype)
+    for r, v in ((3, float("inf")), (130, float("nan")), (200, -float("inf")), (m - 1, float("inf")), (m - 2, 0.0)):
+        x[r, r % k] = v
+    x[256:384], x[300] = 0, float("nan")
+    q, t = B.quantize_both(x, dtype=codes)
+    check_codes(q, x, 1, codes)
+    check_codes(t, x.t(), 1, codes)
+    q, t = B.quantize_both(x.contiguous(), dtype=codes)     # aligned rows
+    check_codes(q, x, 1, codes)
+    check_codes(t, x.t(), 1, codes)
+
+
+def test_gradients_of_a_narrow_layer_over_more_rows():
+    x, w = randn(60_011, 40, dtype=torch.float16).requires_grad_(), randn(64, 40, seed=1).requires_grad_()
+    b, g = randn(64, seed=2).requires_grad_(), randn(60_011, 64, seed=3, scale=1e-2, dtype=torch.float16)
+    y = B.linear(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
+    rows = torch.arange(0, 60_011, 211)
+    O.check_product(y.detach()[rows.cuda()], O.values(x.detach()[rows.cuda()]), O.values(w.detach(), 128), b.detach())
+    O.check_product(gx[rows.cuda()], O.values(g[rows.cuda()]), O.values(w.detach().t(), 128))
+    O.check_product(gw, O.values(g.t()), O.values(x.detach().t()))
+    s = g.double().cpu()
+    O.check(gb, s.sum(0), 60_012 * 2.0 ** -24 * s.abs().sum(0))
+
+
 def test_quantize_batch_and_strides():
     x = randn(3, 130, 200, dtype=torch.bfloat16)
     q = B.quantize(x, rows=128)
