@@ -65,7 +65,8 @@ void check_io(int n, int h, int w, unsigned flags) {
 // (Kernels count a tile beyond the last row or column in 32 bits.)
 aeisu::MatrixRef matrix(const aeisu_matrix* m) {
     aeisu::require(m != nullptr, "matrix pointer is null");
-    aeisu::require(m->rows <= aeisu::kMaxSide && m->cols <= aeisu::kMaxSide, "matrix sizes are out of range");
+    aeisu::require(m->rows >= 1 && m->cols >= 1 && m->batch >= 1 && m->rows <= aeisu::kMaxSide && m->cols <= aeisu::kMaxSide,
+                   "matrix sizes are out of range");
     aeisu::require(reinterpret_cast<uintptr_t>(m->data) % aeisu::elem_bytes(m->type) == 0, "tensor pointer is misaligned");
     return {m->data, m->type, m->rows, m->cols, (long long)m->ld, m->batch, (long long)m->batch_stride, m->transposed != 0};
 }
@@ -383,7 +384,7 @@ int aeisu_linear(const aeisu_matrix* x, const aeisu_matrix* weight, const void* 
                  const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
         const aeisu::MatrixRef mx = single(x), mw = single(weight);
-        aeisu::require(mx.cols == mw.cols && mx.rows >= 1, "contraction sizes differ");
+        aeisu::require(mx.cols == mw.cols, "contraction sizes differ");
         aeisu::require(weight->scales != nullptr, "FP8 operands, and only they, come with scales");
         aeisu::linear_serve(mx, mw, scales_of(weight), product_out(out, bias, bias_type, mx.rows, mw.rows), workspace,
                             size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
@@ -395,7 +396,7 @@ int aeisu_linear_forward(const aeisu_matrix* x, const aeisu_matrix* weight, cons
                          uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
         const aeisu::MatrixRef mx = single(x), mw = single(weight);
-        aeisu::require(mx.cols == mw.cols && mx.rows >= 1 && mw.rows >= 1, "contraction sizes differ");
+        aeisu::require(mx.cols == mw.cols, "contraction sizes differ");
         aeisu::linear_train_forward(mx, mw, product_out(out, bias, bias_type, mx.rows, mw.rows), kept_x, kept_weight,
                                     workspace, size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
     });
@@ -406,7 +407,7 @@ int aeisu_linear_backward(const aeisu_matrix* grad, int k, int code_type, const 
                           int grad_bias_type, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
         const aeisu::MatrixRef g = single(grad);
-        aeisu::require(g.rows >= 1 && g.cols >= 1 && k <= aeisu::kMaxSide, "matrix sizes are out of range");
+        aeisu::require(k <= aeisu::kMaxSide, "matrix sizes are out of range");
         aeisu::linear_train_backward(g, k, code_type, kept_x, kept_weight, grad_x, grad_x_type, grad_weight,
                                      grad_weight_type, grad_bias, grad_bias_type, workspace, size_t(workspace_bytes),
                                      device, static_cast<cudaStream_t>(stream));
@@ -421,7 +422,7 @@ int aeisu_grouped_linear(const aeisu_matrix* x, const aeisu_matrix* weight, cons
                          const aeisu_matrix* out, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     return guarded([&] {
         const aeisu::MatrixRef mx = single(x), mw = matrix(weight);
-        aeisu::require(mx.cols == mw.cols && mx.rows >= 1, "contraction sizes differ");
+        aeisu::require(mx.cols == mw.cols, "contraction sizes differ");
         aeisu::require(weight->scales != nullptr, "FP8 operands, and only they, come with scales");
         aeisu::grouped_linear(mx, mw, scales_of(weight), offsets, product_out(out, nullptr, 0, mx.rows, mw.rows),
                               zero_outside != 0, workspace, size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
