@@ -63,11 +63,12 @@ void check_io(int n, int h, int w, unsigned flags) {
 }
 
 // (Kernels count a tile beyond the last row or column in 32 bits.)
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 aeisu::MatrixRef matrix(const aeisu_matrix* m) {
     aeisu::require(m != nullptr, "matrix pointer is null");
     aeisu::require(m->rows >= 1 && m->cols >= 1 && m->batch >= 1 && m->rows <= aeisu::kMaxSide && m->cols <= aeisu::kMaxSide,
                    "matrix sizes are out of range");
-    aeisu::require(reinterpret_cast<uintptr_t>(m->data) % aeisu::elem_bytes(m->type) == 0, "tensor pointer is misaligned");
+    aeisu::require(aligned(m->data, aeisu::elem_bytes(m->type)), "tensor pointer is misaligned");
     return {m->data, m->type, m->rows, m->cols, (long long)m->ld, m->batch, (long long)m->batch_stride, m->transposed != 0};
 }
 aeisu::ScaleRef scales_of(const aeisu_matrix* m) {
@@ -90,14 +91,21 @@ aeisu::MatrixRef single(const aeisu_matrix* m) {
     aeisu::require(r.batch == 1, "a linear layer takes single matrices");
     return r;
 }
+// A tensor that results go to, float32, float16 or bfloat16; null where the call leaves that open.  Refused here, before
+// the call has enqueued anything.
+void check_result(const void* p, int type) {
+    aeisu::require(!p || (type >= aeisu::kF32 && type <= aeisu::kBF16), "output must be float32, float16 or bfloat16");
+    aeisu::require(!p || aligned(p, aeisu::elem_bytes(type)), "output pointer is misaligned");
+}
 // The output of x[rows][k] and weight[cols][k].
 aeisu::ProductOut product_out(const aeisu_matrix* out, const void* bias, int bias_type, int rows, int cols) {
     aeisu::require(out != nullptr, "output pointer is null");
     matrix(out);
-    aeisu::require(out->rows == rows && out->cols == cols && out->batch == 1 && !out->transposed,
+    aeisu::require(out->rows == rows && out->cols == cols && out->batch == 1 && !out->transposed && out->ld >= cols,
                    "output sizes are out of range");
+    check_result(out->data, out->type);
     aeisu::require(!bias || (bias_type >= 0 && bias_type <= 2), "bias must be float32, float16 or bfloat16");
-    aeisu::require(reinterpret_cast<uintptr_t>(bias) % aeisu::elem_bytes(bias_type) == 0, "bias pointer is misaligned");
+    aeisu::require(aligned(bias, aeisu::elem_bytes(bias_type)), "bias pointer is misaligned");
     return {const_cast<void*>(out->data), out->type, (long long)out->ld, bias, bias_type};
 }
 
@@ -342,6 +350,8 @@ int aeisu_column_sum(const aeisu_matrix* x, void* out, int out_type, void* works
     return guarded([&] {
         const aeisu::MatrixRef m = matrix(x);
         aeisu::require(workspace_bytes >= aeisu_column_sum_workspace(m.rows, m.cols), "workspace is too small");
+        aeisu::require(aligned(workspace, sizeof(float)), "workspace is misaligned");
+        check_result(out, out_type);
         aeisu::column_sum(m, out, out_type, static_cast<float*>(workspace), device, static_cast<cudaStream_t>(stream));
     });
 }
@@ -360,6 +370,7 @@ int aeisu_product(const aeisu_matrix* a, const aeisu_matrix* b, const void* bias
     return guarded([&] {
         const aeisu::MatrixRef ma = matrix(a), mb = matrix(b);
         aeisu::require(a->scales && b->scales, "FP8 operands, and only they, come with scales");
+        aeisu::require(aligned(workspace, sizeof(float)), "workspace is misaligned");
         aeisu::product(ma, scales_of(a), mb, scales_of(b), product_out(out, bias, bias_type, ma.rows, mb.rows),
                        workspace, size_t(workspace_bytes), false, device, static_cast<cudaStream_t>(stream));
     });
@@ -397,6 +408,7 @@ int aeisu_linear_forward(const aeisu_matrix* x, const aeisu_matrix* weight, cons
     return guarded([&] {
         const aeisu::MatrixRef mx = single(x), mw = single(weight);
         aeisu::require(mx.cols == mw.cols, "contraction sizes differ");
+        aeisu::require(aligned(kept_x, 16) && aligned(kept_weight, 16), "kept codes are misaligned");
         aeisu::linear_train_forward(mx, mw, product_out(out, bias, bias_type, mx.rows, mw.rows), kept_x, kept_weight,
                                     workspace, size_t(workspace_bytes), device, static_cast<cudaStream_t>(stream));
     });
@@ -408,6 +420,10 @@ int aeisu_linear_backward(const aeisu_matrix* grad, int k, int code_type, const 
     return guarded([&] {
         const aeisu::MatrixRef g = single(grad);
         aeisu::require(k <= aeisu::kMaxSide, "matrix sizes are out of range");
+        aeisu::require(aligned(kept_x, 16) && aligned(kept_weight, 16), "kept codes are misaligned");
+        check_result(grad_x, grad_x_type);
+        check_result(grad_weight, grad_weight_type);
+        check_result(grad_bias, grad_bias_type);
         aeisu::linear_train_backward(g, k, code_type, kept_x, kept_weight, grad_x, grad_x_type, grad_weight,
                                      grad_weight_type, grad_bias, grad_bias_type, workspace, size_t(workspace_bytes),
                                      device, static_cast<cudaStream_t>(stream));

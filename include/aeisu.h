@@ -316,7 +316,8 @@ int aeisu_reconstruct_backward_f32(const float* source, const float* metadata, c
  * k_prod.cu): operators for training and serving layers beside the controller's own.  All
  * pointers are device pointers of GPU `device`; every call only enqueues on `stream` and may be
  * captured into a CUDA graph.  Workspaces belong to the caller and are free again once the
- * call's work on the stream is done. */
+ * call's work on the stream is done; they start on 16-byte boundaries, tensors on multiples of their
+ * elements' size. */
 enum { AEISU_TYPE_F32 = 0, AEISU_TYPE_F16 = 1, AEISU_TYPE_BF16 = 2, AEISU_TYPE_E4M3 = 3, AEISU_TYPE_E5M2 = 4 };
 
 /* `batch` matrices of rows x cols: element (r, c) at r * ld + c, or at c * ld + r when

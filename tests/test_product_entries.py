@@ -35,3 +35,40 @@ def test_entries_refuse_empty_matrices(lib, empty):
                  lambda: lib.aeisu_block_quantize(few, 1, bad, None, 0, None),
                  lambda: lib.aeisu_product(bad, codes, None, 0, none, None, 0, 0, None)):
         refused(call, "sizes are out of range")
+
+
+@pytest.mark.parametrize("place, bad, text", [
+    ("grad_x", "pointer", "output"), ("grad_weight", "pointer", "output"), ("grad_bias", "pointer", "output"),
+    ("grad_x", "type", "output"), ("grad_weight", "type", "output"), ("grad_bias", "type", "output"),
+    ("kept_x", "pointer", "kept"), ("kept_weight", "pointer", "kept")])
+def test_linear_backward_refuses_what_it_cannot_store(lib, place, bad, text):
+    args = dict(kept_x=4096, kept_weight=4096, grad_x=4096, grad_weight=4096, grad_bias=4096)
+    types = dict(grad_x=0, grad_weight=0, grad_bias=0)
+    if bad == "type":
+        types[place] = 3
+    else:
+        args[place] += 2
+    refused(lambda: lib.aeisu_linear_backward(
+        packed(**HALF), 64, 3, args["kept_x"], args["kept_weight"], args["grad_x"], types["grad_x"], args["grad_weight"],
+        types["grad_weight"], args["grad_bias"], types["grad_bias"], 4096, 1 << 30, 0, None), text)
+
+
+def test_other_entries_refuse_what_they_cannot_store(lib):
+    codes, half, out = packed(), packed(**HALF), packed(cols=8, ld=8, **HALF)
+    ws = (4096, 1 << 30, 0, None)
+    fp8_out, narrow = packed(cols=8, ld=8), packed(cols=8, ld=7, **HALF)
+    for call, text in (
+            (lambda: lib.aeisu_column_sum(half, 4098, 0, *ws), "output"),
+            (lambda: lib.aeisu_column_sum(half, 4097, 2, *ws), "output"),
+            (lambda: lib.aeisu_column_sum(half, 4096, 3, *ws), "output"),
+            (lambda: lib.aeisu_column_sum(half, 4096, -1, *ws), "output"),
+            (lambda: lib.aeisu_column_sum(half, 4096, 2, 4098, 1 << 30, 0, None), "workspace"),
+            (lambda: lib.aeisu_product(codes, codes, None, 0, out, 4098, 1 << 30, 0, None), "workspace"),
+            (lambda: lib.aeisu_linear_forward(half, half, None, 0, out, 4104, None, *ws), "kept"),
+            (lambda: lib.aeisu_linear_forward(half, half, None, 0, out, None, 4104, *ws), "kept"),
+            (lambda: lib.aeisu_linear(half, codes, None, 0, fp8_out, *ws), "output"),
+            (lambda: lib.aeisu_linear(half, codes, None, 0, narrow, *ws), "output"),
+            (lambda: lib.aeisu_linear_forward(half, half, None, 0, fp8_out, None, None, *ws), "output"),
+            (lambda: lib.aeisu_grouped_linear(half, codes, 4096, 1, fp8_out, *ws), "output"),
+            (lambda: lib.aeisu_grouped_linear(half, codes, 4096, 1, narrow, *ws), "output")):
+        refused(call, text)
