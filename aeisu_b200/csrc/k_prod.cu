@@ -393,6 +393,18 @@ enum ScaleWay { kPerBlock, kPerRow, kPerRowWords };
 struct RawScales {
     uint32_t v[16];
 };
+// Scales may be the work of a quantiser that ran beside this kernel's start, so they are read by ordinary loads that
+// stay behind grid_dep_wait, not through the read-only path, which asks for data that no one writes meanwhile.
+__device__ __forceinline__ uint32_t load_scale(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t load_scale_word(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
 __device__ __forceinline__ void load_scales(RawScales& r, const ScaleRef& s, ScaleWay way, int e, int row0, int rows,
                                             int kb, int blocks) {
     const int lane = threadIdx.x & 31;
@@ -403,17 +415,17 @@ __device__ __forceinline__ void load_scales(RawScales& r, const ScaleRef& s, Sca
         // A tile of such an operand starts on a block of 128 rows or in its middle and does not leave it.
         const int at = min(row0, rows - 1) >> s.shift;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) r.v[b] = __ldg(col[b] + at);
+        for (int b = 0; b < 4; ++b) r.v[b] = load_scale(col[b] + at);
     } else if (way == kPerRowWords) {
         const int at = min(row0 + 4 * lane, rows - 4);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) r.v[b] = __ldg(reinterpret_cast<const uint32_t*>(col[b] + at));
+        for (int b = 0; b < 4; ++b) r.v[b] = load_scale_word(col[b] + at);
     } else {
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                r.v[4 * b + i] = __ldg(col[b] + (min(row0 + 32 * i + lane, rows - 1) >> s.shift));
+                r.v[4 * b + i] = load_scale(col[b] + (min(row0 + 32 * i + lane, rows - 1) >> s.shift));
     }
 }
 // The atom into shared memory: row r, block j at (r % 32) * 16 + (r / 32) * 4 + j.

@@ -1,0 +1,44 @@
+"""Block-scaled FP8 and grouped products at the edges of what they promise: operands quantised by the kernel
+just before, exact sums over many rows, the largest contractions and outputs, the state of bounded waits."""
+import ctypes as C
+
+import pytest
+import torch
+
+from aeisu_b200 import _lib, block_fp8 as B
+from aeisu_b200.grouped import grouped_matmul
+
+pytestmark = pytest.mark.gpu
+E4 = torch.float8_e4m3fn
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    code = C.c_int(-1)
+    _lib.check(_lib.lib().aeisu_product_status(0, C.byref(code)))
+    assert code.value == 0
+
+
+def randn(*shape, seed=0, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed * 7919 + sum(shape))
+    return torch.randn(shape, generator=g).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("m, k, n", [(40, 512, 384), (300, 1024, 640), (2000, 256, 512)])
+def test_products_read_the_scales_of_this_call(m, k, n):
+    # The product starts while the quantiser writes its operand's scales, into memory that the call before used: with
+    # inputs that differ by powers of two from call to call, a scale read too early is that of another call.
+    kept, off = B.quantize(randn(n, k, seed=1), rows=128), torch.tensor([0, m // 3, m], dtype=torch.int32).cuda()
+    experts = B.quantize(randn(2, n, k, seed=2), rows=128)
+    inputs = [randn(m, k) * 2.0 ** e * torch.exp2(torch.arange(m).cuda() % 5 - 2)[:, None].bfloat16() for e in (0, 9, -7)]
+    coded = [B.quantize(x) for x in inputs]
+    want = [(B.matmul(q, kept), grouped_matmul(q, experts, off)) for q in coded]
+    w, g = randn(n, k, seed=3).requires_grad_(), randn(m, n, seed=4)
+    grads = [torch.autograd.grad(B.linear(x, w), w, g)[0] for x in inputs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        out = [(B.linear(x, kept), grouped_matmul(x, experts, off), *torch.autograd.grad(B.linear(x, w), w, g))
+               for x in inputs]
+        for got, (y, z), gw in zip(out, want, grads):
+            assert torch.equal(got[0], y) and torch.equal(got[1], z) and torch.equal(got[2], gw)
