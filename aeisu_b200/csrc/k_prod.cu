@@ -326,7 +326,7 @@ __device__ __forceinline__ Tile tile_at(const ProdJob& j, const Groups& g, int t
         x.p0 = (first + t - col * (last ? int(j.by_rest.d) : kBand)) * BM;
         x.q0 = col * BN;
         x.k0 = x.part * j.steps_per_split * step;
-        x.k1 = min(j.K, x.k0 + j.steps_per_split * step);
+        x.k1 = x.k0 + min(j.K - x.k0, j.steps_per_split * step);   // (the last part's whole length may end beyond 2^31)
     } else if (j.grouping == kContraction) {
         // Groups from the longest to the shortest: the time of a tile goes by the rows of its group.
         int i;

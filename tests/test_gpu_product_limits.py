@@ -42,3 +42,16 @@ def test_products_read_the_scales_of_this_call(m, k, n):
                for x in inputs]
         for got, (y, z), gw in zip(out, want, grads):
             assert torch.equal(got[0], y) and torch.equal(got[1], z) and torch.equal(got[2], gw)
+
+
+@pytest.mark.parametrize("k", [2 ** 31 - 1025, 2 ** 31 - 12_000])
+def test_longest_contraction(k):
+    # 148 parts, the last of which would end beyond 2^31 if it were as long as the others: ones at both ends and around
+    # the middle, so that every product and sum is a whole number below 2^24
+    codes = torch.zeros(1, k, dtype=torch.uint8, device="cuda")
+    codes[:, :70_000] = 0x38                      # 1.0
+    codes[:, k // 2:k // 2 + 300] = 0x40          # 2.0
+    codes[:, -90_001:] = 0x38
+    scales = torch.full((-(-k // 128), 1), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    a = B.BlockFP8(codes.view(E4), scales)
+    assert float(B.matmul(a, a, dtype=torch.float32)) == 70_000 + 4 * 300 + 90_001
