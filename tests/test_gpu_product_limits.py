@@ -55,3 +55,24 @@ def test_longest_contraction(k):
     scales = torch.full((-(-k // 128), 1), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
     a = B.BlockFP8(codes.view(E4), scales)
     assert float(B.matmul(a, a, dtype=torch.float32)) == 70_000 + 4 * 300 + 90_001
+
+
+def unit_blocks(*shape, rows=1):
+    """An operand of ones."""
+    codes = torch.full(shape, 0x38, dtype=torch.uint8, device="cuda").view(E4)
+    lead, (r, c) = shape[:-2], shape[-2:]
+    scales = torch.full((*lead, -(-c // 128), -(-r // rows)), 127, dtype=torch.uint8, device="cuda")
+    return B.BlockFP8(codes, scales.view(torch.float8_e8m0fnu), rows)
+
+
+def used_memory(n, dtype):
+    """Leaves n elements of memory full of threes to the next allocation of their size."""
+    torch.full((n,), 3.0, device="cuda", dtype=dtype)
+
+
+def test_rows_in_no_group_of_more_than_two_to_the_31_bytes():
+    n = 2 ** 29
+    x, w = unit_blocks(3, 16), unit_blocks(1, n, 16, rows=128)
+    used_memory(3 * n, torch.float32)
+    y = grouped_matmul(x, w, torch.tensor([1, 2], dtype=torch.int32).cuda(), dtype=torch.float32)
+    assert bool((y[1] == 16).all()) and not y[0].any() and not y[2].any()
