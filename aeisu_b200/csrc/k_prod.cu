@@ -1116,10 +1116,10 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         }
         if (j.zero_outside) {
             // A warp takes a row at a time: the rows before the first group, then those behind the last.  (Bytes of a
-            // row may pass 2^31.)
+            // row, and the row after the last one, may pass 2^31.)
             const int before = bound[0], skip = bound[j.groups] - before, size = j.out_type == kF32 ? 4 : 2;
             constexpr int kWarps = 4 * S::kHalves;
-            for (int i = int(blockIdx.x) * kWarps + warp - 4; i < j.zero_rows - skip; i += int(gridDim.x) * kWarps) {
+            for (long long i = int(blockIdx.x) * kWarps + warp - 4; i < j.zero_rows - skip; i += int(gridDim.x) * kWarps) {
                 uint8_t* row = static_cast<uint8_t*>(j.out) + (i < before ? i : i + skip) * j.out_ld * size;
                 const long long bytes = (long long)j.cols * size, whole = j.out_vec ? bytes / 16 * 16 : 0;
                 for (long long c = lane * 16; c < whole; c += 32 * 16) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);

@@ -76,3 +76,15 @@ def test_rows_in_no_group_of_more_than_two_to_the_31_bytes():
     used_memory(3 * n, torch.float32)
     y = grouped_matmul(x, w, torch.tensor([1, 2], dtype=torch.int32).cuda(), dtype=torch.float32)
     assert bool((y[1] == 16).all()) and not y[0].any() and not y[2].any()
+
+
+def test_as_many_rows_in_no_group_as_there_may_be():
+    # one group of one row: the rows that the warps would take after the last ones lie beyond 2^31
+    t = 2 ** 31 - 1025
+    codes = torch.empty(t, 16, dtype=torch.uint8, device="cuda")
+    codes[:2] = 0x38
+    scales = torch.full((1, t), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    x, w = B.BlockFP8(codes.view(E4)[:, :1], scales), unit_blocks(1, 1, 1)
+    used_memory(t, torch.float16)
+    y = grouped_matmul(x, w, torch.tensor([1, 2], dtype=torch.int32).cuda(), dtype=torch.float16)
+    assert float(y[1]) == 1 and not y[:1].any() and not y[2:].any()
