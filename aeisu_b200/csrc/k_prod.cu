@@ -253,7 +253,8 @@ __device__ __forceinline__ bool elected() {
 }
 
 // The clock is read only once a first try has failed: the MMA warp's waits are part of every step.
-constexpr long long kWaitCycles = 4000000000LL;
+// A wait that lasts as long as many steps of a contraction takes kStepCycles more for each of them (they take about 540).
+constexpr long long kWaitCycles = 4000000000LL, kStepCycles = 20000;
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, long long more = 0) {
     return mbar_try_wait(bar, parity) || mbar_wait_bounded(bar, parity, &g_product_error, kErrWait, kWaitCycles + more);
 }
@@ -1043,14 +1044,16 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
             // (This warp waits on barriers that only these steps use: it is no part of the ring's flow, so a
             // barrier that every step passes could run two phases ahead of it.)
             uint32_t landed_phase = 0;
+            long long passed = 0;   // steps since the last wait: it goes on while they do
             for (int t = first_tile; ok && t < tiles; t += stride) {
                 const Tile x = tile_at<BM, BN>(j, g, t, kStep);
                 if (x.p0 < 0) continue;
-                for (int k = x.k0; k < x.k1; k += kStep) {
+                for (int k = x.k0; k < x.k1; k += kStep, ++passed) {
                     const int rows = x.k1 - k;
                     if (rows < kStep) {
-                        if (!(ok = __all_sync(~0u, wait(landed + stage, (landed_phase >> stage) & 1)))) break;
+                        if (!(ok = __all_sync(~0u, wait(landed + stage, (landed_phase >> stage) & 1, passed * kStepCycles)))) break;
                         landed_phase ^= 1u << stage;
+                        passed = 0;
                         // eight lanes to a row of 128 bytes
                         uint8_t* at = ring + stage * S::kStage + (lane & 7) * 16;
 #pragma unroll
@@ -1080,8 +1083,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                 __syncwarp();
                 bias_q = x.q0;
             }
-            // A tile of a very long contraction takes its time: 20,000 cycles more for each step of about 500.
-            if (!__all_sync(~0u, wait(acc_full + acc, acc_phase, (x.k1 - x.k0) / kStep * 20000LL))) break;
+            if (!__all_sync(~0u, wait(acc_full + acc, acc_phase, (x.k1 - x.k0) / kStep * kStepCycles))) break;
             fence_after_sync();
             uint32_t v[S::kWide];
             if (x.k0 < x.k1) {

@@ -88,3 +88,17 @@ def test_as_many_rows_in_no_group_as_there_may_be():
     used_memory(t, torch.float16)
     y = grouped_matmul(x, w, torch.tensor([1, 2], dtype=torch.int32).cuda(), dtype=torch.float16)
     assert float(y[1]) == 1 and not y[:1].any() and not y[2:].any()
+
+
+def test_weight_gradient_that_takes_more_than_two_seconds():
+    # One tile whose 8,281,251 steps take about 4.4e9 cycles: every wait that spans them has to last as long, that for
+    # the last, partial step too.  Ones among zeros, so that the sums are exact.
+    t = 530_000_005
+    x, g = (torch.zeros(t, 8, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    for i, r in enumerate((0, 63, 1_000_001, t - 6, t - 5, t - 1)):
+        x[r, i], g[r, i] = 1 + i, 2
+    w = torch.zeros(1, 8, 8, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = grouped_matmul(x, w, torch.tensor([0, t], dtype=torch.int32).cuda())
+    (gw,) = torch.autograd.grad(y, w, g)
+    want = torch.diag(torch.tensor([2.0, 4, 6, 8, 10, 12, 0, 0], dtype=torch.bfloat16, device="cuda"))
+    assert torch.equal(gw[0], want)
