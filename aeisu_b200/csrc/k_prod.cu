@@ -820,6 +820,7 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
         uint32_t phase = 0;
         bool ok = true;
         long long issued = 0;
+        uint32_t on_landed = 0, landed_phase = 0;   // by stage: its last copies count on `landed`, whose next phase is this
         const int staged = FP8 && !OWN && j.narrow ? S::kStage / 2 : S::kStage;   // bytes per step
         // Weights are on their way before the quantiser has ended: A's copies of the first stages.
         int early = 0;
@@ -870,15 +871,19 @@ k_product(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtens
                     }
                 }
                 __syncwarp();
+                on_landed = (on_landed & ~(1u << stage)) | uint32_t(tail) << stage;
+                landed_phase ^= uint32_t(tail) << stage;
                 ++issued;
                 if (++stage == S::kStages) stage = 0, phase ^= 1;
             }
         }
-        // Every copy has landed before the CTA may end: those that no MMA waited for are waited for here
-        // (a pair's by its first CTA; the other one cannot end before it).
-        for (int i = 0; !ok && (CTAS == 1 || rank == 0) && i < S::kStages && issued - i > 0; ++i) {
+        // Every copy has landed before the CTA may end: those that no MMA waited for are waited for here (a pair's by its
+        // first CTA, since the other one cannot end before it; those on `landed` by the CTA that they go to).
+        for (int i = 0; !ok && i < S::kStages && issued - i > 0; ++i) {
             const long long n = issued - 1 - i;
-            wait(full + n % S::kStages, uint32_t(n / S::kStages) & 1);
+            const int at = int(n % S::kStages);
+            if (on_landed >> at & 1) wait(landed + at, (landed_phase >> at & 1) ^ 1);
+            else if (CTAS == 1 || rank == 0) wait(full + at, uint32_t(n / S::kStages) & 1);
         }
     } else if (warp == 1) {
         if (CTAS == 1 || rank == 0) {
