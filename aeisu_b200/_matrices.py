@@ -4,6 +4,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -33,6 +34,14 @@ def need_cuda(name, *tensors):
         if t.get_device() != index:
             raise ValueError(f"{name}: the tensors must be on one device")
     return index
+
+
+def refuse_tangents(name, *tensors):
+    """An input of forward-mode differentiation is refused: its tangent would be lost in silence."""
+    if forward_ad._current_level >= 0:   # (the private name spares calls outside of it 0.7 us per tensor)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivatives")
 
 
 def row_stride(t):

@@ -19,7 +19,8 @@ accumulate in float32 and round once to the output's type; repeated calls give t
 ``linear`` trains: the input gradient is the product of the gradient's rows with the weight's blocks,
 the weight gradient that of the gradient's columns with the input's columns (blocks of 128 rows of
 the batch), both operands in FP8; the bias gradient is summed in float32.  Only the transposed FP8
-codes of input and weight are kept for the backward pass.  Gradients of gradients are not computed.
+codes of input and weight are kept for the backward pass.  Gradients of gradients and forward-mode
+derivatives are not computed: both are refused.
 
 All tensors must be CUDA tensors on one device; work goes to that device's current stream and may be
 captured into a CUDA graph.  A backward pass is captured only while no eager graph of the same leaves
@@ -259,6 +260,7 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def once(ctx, grad):
+        mx.refuse_tangents("linear", grad)
         x_type, w_type, b_type, grad_dtype = ctx.types
         (m, n, k), (need_x, need_w, need_b, _), index = ctx.sizes, ctx.needs_input_grad, grad.get_device()
         new = grad.new_zeros if m == 0 else grad.new_empty
@@ -303,6 +305,7 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
     shape, wide = x.shape, values.shape
     if len(shape) < 1 or len(wide) != 2 or shape[-1] != wide[1] or 0 in wide:
         raise ValueError("Expected x [..., K] and weight [N, K]")
+    mx.refuse_tangents("linear", x, None if serving else weight, bias)
     n, k = wide
     if bias is None:
         ready = None

@@ -74,6 +74,7 @@ class _Grouped(torch.autograd.Function):
 
     @staticmethod
     def once(ctx, grad):
+        mx.refuse_tangents("grouped_matmul", grad)
         x, weight, offsets = ctx.saved_tensors
         t, k = x.shape
         need_x, need_w, _ = ctx.needs_input_grad
@@ -126,6 +127,7 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
     if out is not None and (tuple(out.shape) != (t, n) or out.dtype != dtype or (t and mx.row_stride(out) is None) or
                             out.requires_grad):
         raise ValueError(f"Expected out [{t}, {n}] of {dtype} with contiguous rows and without gradient")
+    mx.refuse_tangents("grouped_matmul", None if coded else x, None if fp8 else weight, out)
     index = mx.need_cuda("grouped_matmul", x.codes if coded else x, weight.codes if fp8 else weight, offsets,
                          *(() if out is None else (out,)))
     if torch.is_grad_enabled() and ((not coded and x.requires_grad) or (not fp8 and weight.requires_grad)):

@@ -4,6 +4,7 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from aeisu_b200 import _lib, block_fp8 as B
 from aeisu_b200.grouped import grouped_matmul
@@ -102,3 +103,14 @@ def test_weight_gradient_that_takes_more_than_two_seconds():
     (gw,) = torch.autograd.grad(y, w, g)
     want = torch.diag(torch.tensor([2.0, 4, 6, 8, 10, 12, 0, 0], dtype=torch.bfloat16, device="cuda"))
     assert torch.equal(gw[0], want)
+
+
+def test_tangents_of_gradients_are_refused():
+    x, off = randn(8, 64), torch.tensor([0, 3, 8], dtype=torch.int32).cuda()
+    w, we = randn(32, 64, seed=1).requires_grad_(), randn(2, 32, 64, seed=2).requires_grad_()
+    for y, leaf in ((B.linear(x, w), w), (grouped_matmul(x, we, off), we)):
+        with forward_ad.dual_level():
+            g = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(ValueError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, g, retain_graph=True)
+            assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].isfinite().all()

@@ -1,9 +1,12 @@
 """The C entry points of block-scaled FP8 and grouped products, without a GPU: every argument that a
 kernel or the host arithmetic could not stand is refused before any of it runs."""
 import pytest
+import torch
+from torch.autograd import forward_ad
 
-from aeisu_b200 import _lib, build
-from test_block_fp8 import HALF, packed
+from aeisu_b200 import _lib, block_fp8 as B, build
+from aeisu_b200.grouped import grouped_matmul
+from test_block_fp8 import HALF, blocks, packed
 
 
 @pytest.fixture(scope="module")
@@ -72,3 +75,36 @@ def test_other_entries_refuse_what_they_cannot_store(lib):
             (lambda: lib.aeisu_grouped_linear(half, codes, 4096, 1, fp8_out, *ws), "output"),
             (lambda: lib.aeisu_grouped_linear(half, codes, 4096, 1, narrow, *ws), "output")):
         refused(call, text)
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias"])
+def test_linear_refuses_forward_mode_inputs(which):
+    t = dict(x=torch.randn(4, 64), weight=torch.randn(8, 64), bias=torch.randn(8))
+    with forward_ad.dual_level():
+        t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        for weight in (t["weight"], t["weight"].clone().requires_grad_(), blocks(8, 64, 128)):
+            if which == "weight" and weight is not t["weight"]:
+                continue
+            with pytest.raises(ValueError, match="forward-mode"):
+                B.linear(t["x"], weight, t["bias"])
+        with pytest.raises(ValueError, match="CUDA tensors"):     # no dual among them
+            B.linear(torch.randn(4, 64), torch.randn(8, 64))
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "out"])
+def test_grouped_products_refuse_forward_mode_inputs(which):
+    t = dict(x=torch.randn(6, 16).half(), weight=torch.randn(2, 8, 16).half())
+    off = torch.tensor([0, 2, 6], dtype=torch.int32)
+    if which == "out":
+        t["out"] = torch.zeros(6, 8).half()
+    with forward_ad.dual_level():
+        t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            grouped_matmul(t["x"], t["weight"], off, out=t.get("out"))
+        if which == "x":
+            with pytest.raises(ValueError, match="forward-mode"):
+                grouped_matmul(t["x"], blocks(8, 16, 128, lead=(2,)), off)
+    if which != "out":
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.func.jvp(lambda v: grouped_matmul(*(v if n == which else t[n] for n in ("x", "weight")), off),
+                           (t[which].detach().clone(),), (torch.ones_like(t[which]),))
