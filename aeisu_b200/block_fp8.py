@@ -26,9 +26,14 @@ All tensors must be CUDA tensors on one device; work goes to that device's curre
 captured into a CUDA graph.  A backward pass is captured only while no eager graph of the same leaves
 lives: torch would make the capture wait for that graph's stream, and the capture fails.  float64 is
 refused rather than computed at a lower precision.
+
+The waits inside the product kernel are bounded: one that makes no progress for about two seconds ends
+its kernel, whose outputs are then undefined.  ``check_products()`` waits for the device and raises if that
+has happened; call it where a program synchronises anyway.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 
 import torch
@@ -335,4 +340,22 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
     return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
 
 
-__all__ = ["BlockFP8", "quantize", "quantize_both", "matmul", "linear"]
+def check_products(device=None):
+    """Waits for a CUDA device (default: the current one); ``TimeoutError`` if a product kernel on it, of this module or
+    of ``grouped``, gave up a wait since the last call, so that outputs since then are undefined."""
+    if device is None or isinstance(device, int):
+        index = device
+    else:
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"check_products needs a CUDA device; got {device}")
+        index = device.index
+    if index is None:
+        index = torch.cuda.current_device()
+    code = ctypes.c_int(0)
+    _lib.check(_call().aeisu_product_status(index, ctypes.byref(code)))
+    if code.value:
+        raise TimeoutError(f"a product kernel on CUDA device {index} gave up a wait; outputs since the last check are undefined")
+
+
+__all__ = ["BlockFP8", "quantize", "quantize_both", "matmul", "linear", "check_products"]

@@ -12,6 +12,7 @@ Float weights (float16 or bfloat16, the type of x) train: gradients of x and wei
 the same kind, an expert without rows gets zeros.  BlockFP8 weights (``quantize(weight, rows=128)``)
 serve: x is quantised in the call, or given as BlockFP8.  Sums are held in float32 and rounded once.
 Rows in no group are zero, or, with ``out``, left as they were there.
+``block_fp8.check_products()`` tells whether a kernel gave up a wait.
 """
 from __future__ import annotations
 

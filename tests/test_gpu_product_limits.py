@@ -114,3 +114,9 @@ def test_tangents_of_gradients_are_refused():
             with pytest.raises(ValueError, match="forward-mode"):
                 torch.autograd.grad(y, leaf, g, retain_graph=True)
             assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].isfinite().all()
+
+
+def test_check_products_after_products():
+    for device in (None, 0, "cuda", torch.device("cuda", 0)):
+        B.matmul(unit_blocks(300, 640), unit_blocks(200, 640, rows=128))
+        assert B.check_products(device) is None

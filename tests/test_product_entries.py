@@ -108,3 +108,25 @@ def test_grouped_products_refuse_forward_mode_inputs(which):
         with pytest.raises(ValueError, match="forward-mode"):
             torch.func.jvp(lambda v: grouped_matmul(*(v if n == which else t[n] for n in ("x", "weight")), off),
                            (t[which].detach().clone(),), (torch.ones_like(t[which]),))
+
+
+def test_check_products_raises_what_the_library_reports(monkeypatch):
+    seen = []
+
+    class Library:
+        code = 1
+
+        def aeisu_product_status(self, index, code):
+            seen.append(index)
+            code._obj.value, self.code = self.code, 0
+            return _lib.OK
+
+    fake = Library()
+    monkeypatch.setattr(B, "_call", lambda: fake)
+    with pytest.raises(TimeoutError, match="device 2"):
+        B.check_products(2)
+    for device in (2, "cuda:3", torch.device("cuda", 4)):
+        B.check_products(device)
+    assert seen == [2, 2, 3, 4]
+    with pytest.raises(ValueError, match="CUDA device"):
+        B.check_products("cpu")
