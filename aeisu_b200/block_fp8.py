@@ -299,7 +299,7 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
     or a BlockFP8 kept from before, which serves without gradients.  The output has x's type; gradients
     have the types of their tensors.  ``grad_dtype`` is the FP8 type that the upstream gradient takes.
     """
-    serving = type(weight) is BlockFP8
+    serving = isinstance(weight, BlockFP8)
     if x.dtype not in mx.FLOATS:
         raise TypeError(f"linear takes float32, float16 or bfloat16; got {x.dtype}")
     if not serving and weight.dtype not in mx.FLOATS:

@@ -130,3 +130,17 @@ def test_check_products_raises_what_the_library_reports(monkeypatch):
     assert seen == [2, 2, 3, 4]
     with pytest.raises(ValueError, match="CUDA device"):
         B.check_products("cpu")
+
+
+def test_a_subclass_of_block_fp8_serves_everywhere():
+    class Named(B.BlockFP8):
+        pass
+
+    def named(q):
+        return Named(q.codes, q.scales, q.rows)
+
+    w, experts = named(blocks(8, 64, 128)), named(blocks(8, 64, 128, lead=(2,)))
+    x, off = torch.zeros(6, 64).half(), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: B.linear(x, w), lambda: B.matmul(named(blocks(6, 64)), w), lambda: grouped_matmul(x, experts, off)):
+        with pytest.raises(ValueError, match="CUDA tensors"):     # refused for that alone
+            call()
