@@ -45,15 +45,21 @@ def refuse_tangents(name, *tensors):
 
 
 def row_stride(t):
-    """Elements from row to row of a tensor whose rows are contiguous and do not overlap, else None."""
+    """Elements from row to row of a tensor whose rows are contiguous and do not overlap, else None; None too for a
+    view whose memory holds the negated values (the imaginary part of a conjugate)."""
     shape, strides = t.shape, t.stride()
     r, c = shape[-2], shape[-1]
-    if c > 1 and strides[-1] != 1:
+    if (c > 1 and strides[-1] != 1) or t.is_neg():
         return None
     ld = strides[-2] if r > 1 else c
     if ld < c or (len(shape) == 3 and shape[0] > 1 and strides[0] < (r - 1) * ld + c):
         return None
     return ld
+
+
+def plain(t):
+    """t, or a contiguous copy that holds its values as they are."""
+    return t.resolve_neg().contiguous()
 
 
 def matrix(t, ld, scales=None, rows=0, transposed=False):

@@ -163,7 +163,7 @@ def _quantize(x, rows, dtype, both):
     index = mx.need_cuda("quantize", x)
     ld = mx.row_stride(x)
     if ld is None:
-        x = x.detach().contiguous()
+        x = mx.plain(x.detach())
         ld = shape[-1]
     q, mq = _empty(x, tuple(shape), rows, dtype)
     t = mt = None
@@ -194,7 +194,7 @@ def _bias(bias, n):
         raise ValueError(f"Expected bias [{n}]")
     if bias.dtype not in mx.FLOATS:
         raise TypeError(f"bias must be float32, float16 or bfloat16; got {bias.dtype}")
-    return bias if n == 1 or bias.stride(0) == 1 else bias.contiguous()
+    return bias if (n == 1 or bias.stride(0) == 1) and not bias.is_neg() else mx.plain(bias)
 
 
 def matmul(a, b, *, bias=None, dtype=torch.bfloat16):
@@ -224,7 +224,7 @@ def _rows(x):
     """(tensor, aeisu_matrix) of values whose rows may start anywhere."""
     ld = mx.row_stride(x)
     if ld is None:
-        x = x.contiguous()
+        x = mx.plain(x)
         ld = x.shape[-1]
     return x, mx.matrix(x, ld)
 

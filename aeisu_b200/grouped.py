@@ -149,7 +149,7 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
     k = x.shape[1]
     stride = mx.row_stride(x)
     if stride is None:
-        x = x.detach().contiguous()
+        x = mx.plain(x.detach())
         stride = k
     size = _call().aeisu_grouped_linear_workspace(t, k)
     ws, (codes, mw) = mx.scratch(size, x), weight.matrix()

@@ -120,3 +120,35 @@ def test_check_products_after_products():
     for device in (None, 0, "cuda", torch.device("cuda", 0)):
         B.matmul(unit_blocks(300, 640), unit_blocks(200, 640, rows=128))
         assert B.check_products(device) is None
+
+
+def test_views_of_negated_memory():
+    # the imaginary part of a conjugate: its memory holds the values with the other sign
+    def imaginary(*shape, seed, dtype=torch.float32):
+        z = torch.view_as_complex(randn(*shape, 2, seed=seed, dtype=dtype)).conj().imag
+        assert z.is_neg()
+        return z, z.resolve_neg().clone()
+
+    off = torch.tensor([0, 3, 5], dtype=torch.int32).cuda()
+    for rows, cols in ((5, 1), (1, 1), (5, 40)):
+        x, x0 = imaginary(rows, cols, seed=1)
+        w, w0 = imaginary(24, cols, seed=2)
+        b, b0 = imaginary(24, seed=3)
+        one, one0 = imaginary(1, seed=4)
+        kept = B.quantize(w0, rows=128)
+        assert torch.equal(B.quantize(x).dequantize(), B.quantize(x0).dequantize())
+        assert torch.equal(B.linear(x, kept, b), B.linear(x0, kept, b0))
+        assert torch.equal(B.linear(x, w, b), B.linear(x0, w0, b0))
+        assert torch.equal(B.linear(x, w[:1], one), B.linear(x0, w0[:1], one0))
+        g, g0 = imaginary(rows, 24, seed=5)
+        leaf = w0.clone().requires_grad_()
+        grads = [torch.autograd.grad(B.linear(x0, leaf), leaf, v)[0] for v in (g, g0)]
+        assert torch.equal(*grads)
+        experts = B.quantize(torch.stack([w0, w0]), rows=128)
+        assert torch.equal(grouped_matmul(x, experts, off), grouped_matmul(x0, experts, off))
+        half, half0 = imaginary(rows, cols, seed=6, dtype=torch.float16)
+        we = torch.stack([w0, w0]).half()
+        assert torch.equal(grouped_matmul(half, we, off), grouped_matmul(half0, we, off))
+        out = imaginary(rows, 24, seed=7, dtype=torch.float16)[0]
+        with pytest.raises(ValueError, match="Expected out"):
+            grouped_matmul(half, we, off, out=out)
