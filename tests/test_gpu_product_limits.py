@@ -152,3 +152,52 @@ def test_views_of_negated_memory():
         out = imaginary(rows, 24, seed=7, dtype=torch.float16)[0]
         with pytest.raises(ValueError, match="Expected out"):
             grouped_matmul(half, we, off, out=out)
+
+
+def integers(*shape, most, seed, dtype):
+    g = torch.Generator().manual_seed(seed * 7919 + sum(shape))
+    return torch.randint(-most, most + 1, shape, generator=g).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("m, k, n, dtype", [
+    (60_011, 40, 64, torch.float16), (60_011, 37, 50, torch.bfloat16), (57_217, 8, 24, torch.float32),
+    (60_011, 200, 64, torch.bfloat16), (57_100, 64, 130, torch.float16), (20_011, 64, 48, torch.bfloat16)])
+def test_sums_over_many_rows_are_whole(m, k, n, dtype):
+    # Integers of at most three bits are exact in E4M3 and sums of their products stay below 2^24, so that a row block, a
+    # part or a CTA's half that is lost, or counted twice, changes the result.
+    x, w = integers(m, k, most=3, seed=1, dtype=dtype).requires_grad_(), integers(n, k, most=3, seed=2, dtype=torch.float32).requires_grad_()
+    b, g = integers(n, most=7, seed=3, dtype=torch.float32).requires_grad_(), integers(m, n, most=2, seed=4, dtype=dtype)
+    g[:128] = 1                                  # the first block and, below, the last rows do not cancel
+    g[-(m % 128 or 128):] = -2
+    x0, w0, g0 = (v.detach().double() for v in (x, w, g))
+    y = B.linear(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
+    assert torch.equal(y.detach(), (x0 @ w0.t() + b.detach().double()).to(dtype))
+    assert torch.equal(gx, (g0 @ w0).to(dtype))
+    assert torch.equal(gw.double(), g0.t() @ x0) and torch.equal(gb.double(), g0.sum(0))
+    # infinities and NaN stay in their columns of the bias' and the weight's gradient
+    g[m - 1, 1], g[300, 2], g[m // 2, n - 1] = float("inf"), float("nan"), -float("inf")
+    y = B.linear(x, w, b)
+    gx, gw2, gb2 = torch.autograd.grad(y, (x, w, b), g)
+    fine = torch.ones(n, dtype=torch.bool, device="cuda")
+    fine[[1, 2, n - 1]] = False
+    assert torch.equal(gw2[fine], gw[fine]) and bool(gw2[~fine].isnan().all())
+    assert torch.equal(gb2[fine], gb[fine])
+    assert float(gb2[1]) == float("inf") and float(gb2[n - 1]) == -float("inf") and bool(gb2[2].isnan())
+
+
+@pytest.mark.parametrize("m, n, ld", [(1, 1, 1), (63, 64, 64), (1000, 65, 72), (100_003, 37, 40), (130_000, 8, 8), (5, 4000, 4000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_column_sum_entry(m, n, ld, dtype):
+    x = integers(m, ld, most=7, seed=m, dtype=dtype)[:, :n]
+    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    lib = _lib.lib()
+    size = lib.aeisu_column_sum_workspace(m, n)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    want = x.double().sum(0)
+    for out_type in (torch.float32, torch.bfloat16):
+        out = torch.full((n,), 99.0, dtype=out_type, device="cuda")
+        mat = _lib.MATRIX.pack(x.data_ptr(), 0, types[dtype], m, n, 1, ld, 0, 0, 0)
+        _lib.check(lib.aeisu_column_sum(mat, out.data_ptr(), types[out_type], ws.data_ptr(), size, 0,
+                                        torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(out, want.to(out_type))
