@@ -55,7 +55,8 @@ def test_longest_contraction(k):
     codes[:, -90_001:] = 0x38
     scales = torch.full((-(-k // 128), 1), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
     a = B.BlockFP8(codes.view(E4), scales)
-    assert float(B.matmul(a, a, dtype=torch.float32)) == 70_000 + 4 * 300 + 90_001
+    got = float(B.matmul(a, a, dtype=torch.float32))
+    assert got == 70_000 + 4 * 300 + 90_001
 
 
 def unit_blocks(*shape, rows=1):
@@ -76,7 +77,8 @@ def test_rows_in_no_group_of_more_than_two_to_the_31_bytes():
     x, w = unit_blocks(3, 16), unit_blocks(1, n, 16, rows=128)
     used_memory(3 * n, torch.float32)
     y = grouped_matmul(x, w, torch.tensor([1, 2], dtype=torch.int32).cuda(), dtype=torch.float32)
-    assert bool((y[1] == 16).all()) and not y[0].any() and not y[2].any()
+    seen = [float(f(r)) for r in y for f in (torch.min, torch.max)]    # (a failing assert prints what it names)
+    assert seen == [0, 0, 16, 16, 0, 0]
 
 
 def test_as_many_rows_in_no_group_as_there_may_be():
@@ -88,7 +90,8 @@ def test_as_many_rows_in_no_group_as_there_may_be():
     x, w = B.BlockFP8(codes.view(E4)[:, :1], scales), unit_blocks(1, 1, 1)
     used_memory(t, torch.float16)
     y = grouped_matmul(x, w, torch.tensor([1, 2], dtype=torch.int32).cuda(), dtype=torch.float16)
-    assert float(y[1]) == 1 and not y[:1].any() and not y[2:].any()
+    seen = float(y[0]), float(y[1]), bool(y[2:].any())
+    assert seen == (0, 1, False)
 
 
 def test_weight_gradient_that_takes_more_than_two_seconds():
@@ -101,8 +104,7 @@ def test_weight_gradient_that_takes_more_than_two_seconds():
     w = torch.zeros(1, 8, 8, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     y = grouped_matmul(x, w, torch.tensor([0, t], dtype=torch.int32).cuda())
     (gw,) = torch.autograd.grad(y, w, g)
-    want = torch.diag(torch.tensor([2.0, 4, 6, 8, 10, 12, 0, 0], dtype=torch.bfloat16, device="cuda"))
-    assert torch.equal(gw[0], want)
+    assert gw[0].tolist() == torch.diag(torch.tensor([2.0, 4, 6, 8, 10, 12, 0, 0])).tolist()
 
 
 def test_tangents_of_gradients_are_refused():
