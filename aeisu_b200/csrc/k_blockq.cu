@@ -309,8 +309,10 @@ template <typename T, bool E5M2, bool VEC>
 void launch_quant(const QuantJob<T>& j, int block_rows, int batch, cudaStream_t stream) {
     const long long rows128 = (j.rows + 127) / 128, col_blocks = (j.cols + 127) / 128;
     const int cb = col_blocks >= 3 ? 4 : int(col_blocks);
-    // 256 rows to a CTA where 128 would make more CTAs than three on each of 148 SMs (bfloat16 x 64 both ways: 165,888
-    // rows 14.2 -> 10.2 us; 18,944 rows 3.6 us, 4.1 in this form).
+    // 256 rows to a CTA where 128 would make more CTAs than three on each of 148 SMs.  Both ways, 128 rows to a CTA
+    // and 256, us: bfloat16, 56,960 rows of 8 columns 6.6 and 4.7, of 64 7.2 and 5.4; 165,888 rows of 8 13.6 and 9.4, of
+    // 32 13.9 and 9.6, of 64 14.2 and 10.1; float32, 165,888 rows of 8 14.6 and 11.2, of 64 15.9 and 13.2.  Fewer rows lose:
+    // bfloat16, 18,944 rows of 64 3.6 and 4.1.
     const bool narrow = block_rows == 1 && j.t_codes && j.cols <= 64 && rows128 > 3 * 148;
     const long long grid = block_rows == 1 && !j.t_codes
                                ? (j.rows * (long long)cb + 127) / 128 * ((col_blocks + cb - 1) / cb)
