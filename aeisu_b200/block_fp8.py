@@ -37,6 +37,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -46,12 +47,15 @@ _E8M0 = torch.float8_e8m0fnu
 _call = _lib.lib
 _new = object.__new__
 _pack = _lib.MATRIX.pack
+_MOST = mx.MAX_SIDE
 
 
 @functools.lru_cache(maxsize=4096)
 def _sizes(shape, rows):
     """(row stride of the codes, shape of the codes' storage, shape of the scales)."""
     *lead, r, c = shape
+    if max(r, c) > _MOST:
+        raise mx.too_large(max(r, c))
     ld = -(-c // 16) * 16
     return ld, (*lead, r, ld), (*lead, mx.blocks(c), -(-r // rows))
 
@@ -156,6 +160,8 @@ def _quantize(x, rows, dtype, both):
         raise ValueError("Expected values [R, C] or [E, R, C]")
     if rows not in (1, mx.BLOCK):
         raise ValueError("blocks have 1 or 128 rows")
+    if shape[-2] > _MOST or shape[-1] > _MOST:
+        raise mx.too_large(max(shape[-2:]))
     if dtype not in mx.CODES:
         raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2; got {dtype}")
     if x.dtype not in mx.FLOATS:
@@ -265,7 +271,8 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def once(ctx, grad):
-        mx.refuse_tangents("linear", grad)
+        if forward_ad._current_level >= 0:
+            mx.refuse_tangents("linear", grad)
         x_type, w_type, b_type, grad_dtype = ctx.types
         (m, n, k), (need_x, need_w, need_b, _), index = ctx.sizes, ctx.needs_input_grad, grad.get_device()
         new = grad.new_zeros if m == 0 else grad.new_empty
@@ -310,26 +317,29 @@ def linear(x, weight, bias=None, *, grad_dtype=torch.float8_e4m3fn):
     shape, wide = x.shape, values.shape
     if len(shape) < 1 or len(wide) != 2 or shape[-1] != wide[1] or 0 in wide:
         raise ValueError("Expected x [..., K] and weight [N, K]")
-    mx.refuse_tangents("linear", x, None if serving else weight, bias)
+    if forward_ad._current_level >= 0:
+        mx.refuse_tangents("linear", x, None if serving else weight, bias)
     n, k = wide
+    m = shape[0] if len(shape) == 2 else shape[:-1].numel()
+    if m > _MOST or n > _MOST or k > _MOST:
+        raise mx.too_large(max(m, n, k))
     if bias is None:
         ready = None
         index = mx.need_cuda("linear", x, values)
     else:
         ready = _bias(bias, n)
         index = mx.need_cuda("linear", x, values, bias)
-    flat = x if len(shape) == 2 else x.reshape(shape[:-1].numel(), k)
+    flat = x if len(shape) == 2 else x.reshape(m, k)
     if torch.is_grad_enabled() and (x.requires_grad or (not serving and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         if serving:
             raise ValueError("FP8 weights serve without gradients: pass the float weight to train")
         y = _Linear.apply(flat, weight, ready, grad_dtype)
-    elif flat.shape[0] == 0:
+    elif m == 0:
         y = flat.new_empty(0, n)
     elif not serving:
         y = _forward(flat, weight, ready, None, None, index)
     else:
-        m = flat.shape[0]
         y = flat.new_empty((m, n))
         size = mx.linear_bytes(m, n, k, 0, index)
         ws = mx.scratch(size, flat)

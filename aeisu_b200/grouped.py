@@ -17,6 +17,7 @@ Rows in no group are zero, or, with ``out``, left as they were there.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -75,7 +76,8 @@ class _Grouped(torch.autograd.Function):
 
     @staticmethod
     def once(ctx, grad):
-        mx.refuse_tangents("grouped_matmul", grad)
+        if forward_ad._current_level >= 0:
+            mx.refuse_tangents("grouped_matmul", grad)
         x, weight, offsets = ctx.saved_tensors
         t, k = x.shape
         need_x, need_w, _ = ctx.needs_input_grad
@@ -111,6 +113,9 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
         raise TypeError("a BlockFP8 x needs BlockFP8 weights")
     if len(x.shape) != 2 or len(weight.shape) != 3 or x.shape[1] != weight.shape[2] or 0 in weight.shape:
         raise ValueError("Expected x [T, K] and weight [E, N, K]")
+    (t, k), n = x.shape, weight.shape[1]
+    if t > mx.MAX_SIDE or n > mx.MAX_SIDE or k > mx.MAX_SIDE:
+        raise mx.too_large(max(t, n, k))
     if weight.shape[0] > MAX_GROUPS:
         raise ValueError(f"at most {MAX_GROUPS} experts; got {weight.shape[0]}")
     if not fp8 and (weight.dtype not in _HALVES or x.dtype != weight.dtype):
@@ -124,11 +129,11 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
     dtype = (dtype or torch.bfloat16) if coded else x.dtype
     if dtype not in mx.FLOATS:
         raise TypeError(f"the result is float32, float16 or bfloat16; got {dtype}")
-    t, n = x.shape[0], weight.shape[1]
     if out is not None and (tuple(out.shape) != (t, n) or out.dtype != dtype or (t and mx.row_stride(out) is None) or
                             out.requires_grad):
         raise ValueError(f"Expected out [{t}, {n}] of {dtype} with contiguous rows and without gradient")
-    mx.refuse_tangents("grouped_matmul", None if coded else x, None if fp8 else weight, out)
+    if forward_ad._current_level >= 0:
+        mx.refuse_tangents("grouped_matmul", None if coded else x, None if fp8 else weight, out)
     index = mx.need_cuda("grouped_matmul", x.codes if coded else x, weight.codes if fp8 else weight, offsets,
                          *(() if out is None else (out,)))
     if torch.is_grad_enabled() and ((not coded and x.requires_grad) or (not fp8 and weight.requires_grad)):
@@ -146,7 +151,6 @@ def grouped_matmul(x, weight, offsets, *, out=None, dtype=None):
         return _product(_rows(x), _weights(weight), offsets, out, ld, new)
     if coded:
         return _product(x.matrix(), weight.matrix(), offsets, out, ld, new)
-    k = x.shape[1]
     stride = mx.row_stride(x)
     if stride is None:
         x = mx.plain(x.detach())

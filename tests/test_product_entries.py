@@ -144,3 +144,22 @@ def test_a_subclass_of_block_fp8_serves_everywhere():
     for call in (lambda: B.linear(x, w), lambda: B.matmul(named(blocks(6, 64)), w), lambda: grouped_matmul(x, experts, off)):
         with pytest.raises(ValueError, match="CUDA tensors"):     # refused for that alone
             call()
+
+
+def test_sides_beyond_32_bits_are_refused():
+    # (the packing of the C structure raised its own error there, and the library's for sides just above its limit)
+    for most in (2 ** 31 - 1024, 2 ** 32 + 5):
+        tall, wide = torch.zeros(1, 16).half().expand(most, 16), torch.zeros(16, 1).half().expand(16, most)
+        huge, w = torch.zeros(1, 1, 16).half().expand(1, most, 16), torch.zeros(1, 8, 16).half()
+        x, off, codes = torch.zeros(4, 16).half(), torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, 16).to(torch.float8_e4m3fn)
+        for call in (lambda: B.linear(tall, w[0]),
+                     lambda: B.linear(tall.expand(3, most, 16), w[0]),
+                     lambda: B.linear(x, huge[0]),
+                     lambda: B.quantize(tall),
+                     lambda: B.quantize_both(wide, rows=128),
+                     lambda: B.quantize(huge),
+                     lambda: B.BlockFP8(codes.expand(most, 16), blocks(1, 16).scales),
+                     lambda: grouped_matmul(tall, w, off),
+                     lambda: grouped_matmul(x, huge, off)):
+            with pytest.raises(ValueError, match="out of range"):
+                call()
