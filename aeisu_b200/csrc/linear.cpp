@@ -61,7 +61,7 @@ size_t linear_workspace(int m, int n, int k, int pass, int device) {
 void linear_serve(const MatrixRef& x, const MatrixRef& w, const ScaleRef& sw, const ProductOut& out, void* workspace,
                   size_t workspace_bytes, int device, cudaStream_t stream) {
     check_workspace(workspace, workspace_bytes, linear_workspace(x.rows, w.rows, x.cols, kServe, device));
-    // Few rows: one kernel does both (one token through 4,096 x 4,096, weights at hand as BlockFP8: 12.5 us from one
+    // Few rows: one kernel does both (one token through 4,096 x 4,096, weights at hand as BlockFP8: 12 us from one
     // Python call to the next instead of 16, of which the GPU takes 9.5 either way).
     if (product_of_values(x, w, sw, out, workspace, workspace_bytes, device, stream)) return;
     const Operand q = operand_at(workspace, kE4M3, x.rows, x.cols, 1);
